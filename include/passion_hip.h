@@ -460,6 +460,35 @@ int passion_prof_read(passion_prof_rec_t* rec, int cap);
  * (ROCm 7.2: hipEventElapsedTime refuses event nodes of a graph, so this returns -1 there) */
 int passion_prof_peek(passion_prof_rec_t* rec, int cap);
 
+/* ---- the residual step between two transformer blocks -------------------------------------
+ * u = post(h), r = x + scale * gate * u, y = pre(r): the end of one block and the norm of the next (reference code/models/mmformer.py:230-256,
+ * 284-300 has x + f(norm(x)); gate, scale and the norm after the block are this form's own).  x, r (and dr, dx): [B][N][C] of x_dtype; h, y (and dy, dh):
+ * [B][N][C] of h_dtype; (f32, f32), (f32, bf16) or (bf16, bf16).  post / pre: 0 none, 1 LayerNorm, 2 RMSNorm, with f32 [C] weights (NULL: 1) and
+ * biases (NULL: 0; LayerNorm only).  gate_mode: 0 none, 1 [B][C], 2 [B][N][C].  scale: f32 [C] or NULL.  1 <= C <= 8192, B <= 65530.
+ * stat: f32 [B][N][4] (NULL: not kept).  pre = 0: y is not written and may be NULL.
+ * Backward: dr / dy may be NULL (zero).  dgate: of gate's shape and dtype.  dw_* / db_* / dscale: f32 [C], overwritten, NULL: not wanted.
+ * part: passion_residual_norm_part_floats(B, N, C) floats.  Column sums are folded in a fixed order (no atomics). */
+int64_t passion_residual_norm_part_floats(int B, int N, int C);
+int passion_residual_norm_fwd(const void* x, int x_dtype, const void* h, int h_dtype, const float* w_post, const float* b_post, int post,
+                              float eps_post, const void* gate, int gate_mode, int gate_dtype, const float* scale, const float* w_pre,
+                              const float* b_pre, int pre, float eps_pre, int B, int N, int C, void* r, void* y, float* stat, void* stream);
+int passion_residual_norm_bwd(const void* x, int x_dtype, const void* h, int h_dtype, const float* w_post, const float* b_post, int post,
+                              const void* gate, int gate_mode, int gate_dtype, const float* scale, const float* w_pre, int pre,
+                              const float* stat, const void* dr, const void* dy, int B, int N, int C, void* dx, void* dh, void* dgate,
+                              float* dw_post, float* db_post, float* dw_pre, float* db_pre, float* dscale, float* part, void* stream);
+
+/* ---- distillation from a teacher's top K logits --------------------------------------------
+ * The form of temp_kl_loss_bs (reference code/utils/criterions.py:92-103) that keeps K of the teacher's V logits a row:
+ * loss[r] = T^2 sum_k p_k (log p_k - log softmax(logits / T)[index_k]), p = softmax(values / T) over the row's entries with 0 <= index < V.  A row without
+ * such an entry (or whose values are all -inf): loss 0, gradient 0.  logits [R][V] f32 / bf16, values [R][K] f32 / bf16, index [R][K] int32 or int64
+ * (index64); K <= passion_topk_distill_max_k().  lse: f32 [R], kept by the forward for the backward (NULL: loss only).
+ * Backward: dlogits = dloss[r] * d loss[r] / d logits, of logits' dtype; V > 512: both 16-byte aligned (-1005). */
+int passion_topk_distill_max_k(void);
+int passion_topk_distill_fwd(const void* logits, int dtype, const void* values, int values_dtype, const void* index, int index64, int64_t R, int V, int K,
+                             float temp, float* loss, float* lse, void* stream);
+int passion_topk_distill_bwd(const void* logits, int dtype, const void* values, int values_dtype, const void* index, int index64, int64_t R, int V, int K,
+                             float temp, const float* lse, const float* dloss, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

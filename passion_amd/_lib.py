@@ -170,6 +170,17 @@ SIGNATURES = {
     "passion_write_words": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     "passion_set_step_words": (None, [c_void_p]),
     "passion_stream_copy": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
+    "passion_residual_norm_part_floats": (c_int64, [c_int, c_int, c_int]),
+    "passion_residual_norm_fwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_void_p,
+                                          c_void_p, c_void_p, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "passion_residual_norm_bwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p,
+                                          c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "passion_topk_distill_max_k": (c_int, []),
+    "passion_topk_distill_fwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_int, c_float, c_void_p, c_void_p,
+                                         c_void_p]),
+    "passion_topk_distill_bwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_int, c_float, c_void_p, c_void_p,
+                                         c_void_p, c_void_p]),
     "passion_set_option": (c_int, [c_char_p, c_int]),
     "passion_prof_enable": (None, [c_int]),
     "passion_prof_filter": (None, [c_double, c_double]),

@@ -4,12 +4,14 @@ Internal activation layout is channels-last 5-D: (B, D, H, W, C) contiguous, f32
 torch is used for memory, streams and autograd bookkeeping only -- every op below runs a
 hand-written HIP kernel, and raises if the library or a GPU tensor is missing.
 """
+import contextlib
 from ctypes import byref, c_void_p
 
 import os
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -1699,6 +1701,191 @@ def region_gap(prob, mask, ys):
 
 def region_mix(prob, mask, w, ys):
     return RegionMixFn.apply(prob, mask, w, *ys)
+
+
+# ------------------------------------------------------------------------------------------------
+# the residual step between two transformer blocks, distillation from a teacher's top logits
+# ------------------------------------------------------------------------------------------------
+def _here(*tensors):
+    """all on one GPU, which is made the current one for the launch (a context manager)"""
+    ts = [t for t in tensors if t is not None]
+    L.require_gpu(*ts)
+    dev = ts[0].device
+    for t in ts[1:]:
+        if t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+    return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _norm_spec(m, C, dtype, what):
+    """(kind, weight, bias, eps) of an nn.LayerNorm / nn.RMSNorm over the last dimension; None: no norm"""
+    if m is None:
+        return 0, None, None, 0.0
+    kind = 1 if isinstance(m, torch.nn.LayerNorm) else 2 if isinstance(m, torch.nn.RMSNorm) else 0
+    if not kind or tuple(m.normalized_shape) != (C,):
+        raise ValueError(f"residual_norm: {what} has to be nn.LayerNorm({C}), nn.RMSNorm({C}) or None, got {m}")
+    eps = m.eps if m.eps is not None else torch.finfo(dtype).eps       # nn.RMSNorm's own default
+    f32 = lambda p: p if p is None or p.dtype == torch.float32 else p.float()
+    return kind, f32(m.weight), f32(m.bias) if kind == 1 else None, float(eps)
+
+
+def _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, meta, keep):
+    post, pre, eps1, eps2, gmode, B, N = meta
+    C = x.shape[-1]
+    r = torch.empty_like(x)
+    y = torch.empty_like(h) if pre else None
+    stat = torch.empty(B * N, 4, dtype=torch.float32, device=x.device) if keep else None
+    if x.numel():
+        with _here(x, h, gate, scale, w1, b1, w2, b2):
+            L.check(L.load().passion_residual_norm_fwd(_p(x), L.dtype_code(x.dtype), _p(h), L.dtype_code(h.dtype), _p(w1), _p(b1), post, eps1, _p(gate), gmode,
+                                                       L.dtype_code(gate.dtype) if gmode else 0, _p(scale), _p(w2), _p(b2), pre, eps2, B, N, C, _p(r),
+                                                       _p(y), _p(stat), L.stream_ptr()), "passion_residual_norm_fwd")
+    return r, y, stat
+
+
+class ResidualNormFn(torch.autograd.Function):
+    """csrc/residual_norm.hip: forward keeps the four row moments, backward forms r again from x and h"""
+
+    @staticmethod
+    def forward(ctx, x, h, gate, scale, w1, b1, w2, b2, meta):
+        r, y, stat = _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, meta, True)
+        ctx.save_for_backward(x, h, gate, scale, w1, b1, w2, stat)
+        ctx.meta, ctx.has_b2 = meta, b2 is not None
+        ctx.set_materialize_grads(False)
+        return (r, y) if meta[1] else r
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dr, dy=None):
+        x, h, gate, scale, w1, b1, w2, stat = ctx.saved_tensors
+        post, pre, _, _, gmode, B, N = ctx.meta
+        C, dev, need = x.shape[-1], x.device, ctx.needs_input_grad
+        if dr is None and dy is None:
+            return (None,) * 9
+        dr, dy = (t.to(like.dtype).contiguous() if t is not None else None for t, like in ((dr, x), (dy, h)))
+        dx, dh = torch.empty_like(x), torch.empty_like(h)
+        dgate = torch.empty_like(gate) if gmode and need[2] else None
+        # [scale, w1, b1, w2, b2], those that are there and wanted
+        there = (scale is not None, w1 is not None, b1 is not None, w2 is not None, ctx.has_b2)
+        want = [t and n for t, n in zip(there, need[3:8])]
+        if not x.numel():
+            cols = [torch.zeros(C, dtype=torch.float32, device=dev) if w else None for w in want]
+            return (dx, dh, dgate.zero_() if dgate is not None else None, *cols, None)
+        lib = L.load()
+        cols = [torch.empty(C, dtype=torch.float32, device=dev) if w else None for w in want]
+        with _here(x, h, gate, dr, dy):
+            part = torch.empty(lib.passion_residual_norm_part_floats(B, N, C), dtype=torch.float32, device=dev)
+            L.check(lib.passion_residual_norm_bwd(_p(x), L.dtype_code(x.dtype), _p(h), L.dtype_code(h.dtype), _p(w1), _p(b1), post, _p(gate), gmode,
+                                                  L.dtype_code(gate.dtype) if gmode else 0, _p(scale), _p(w2), pre, _p(stat), _p(dr), _p(dy), B, N, C,
+                                                  _p(dx), _p(dh), _p(dgate), _p(cols[1]), _p(cols[2]), _p(cols[3]), _p(cols[4]), _p(cols[0]), _p(part),
+                                                  L.stream_ptr()), "passion_residual_norm_bwd")
+        return (dx, dh, dgate, *cols, None)
+
+
+def residual_norm(x, h, post=None, pre=None, gate=None, scale=None):
+    """r = x + scale * gate * post(h), y = pre(r): the residual stream x past one block's output h and into the next block's norm, one launch each
+    way.  x, h: (..., C) of one shape, (f32, f32), (f32, bf16) or (bf16, bf16); post, pre: nn.LayerNorm / nn.RMSNorm over C or None; gate: (B, 1, C) with
+    a (B, N, C) x (one vector a sample, e.g. from a conditioning head), or of x's shape; scale: (C,) parameter (a learned residual scale).
+    -> (r, y), r of x's dtype, y of h's; with pre=None only r.  y is formed from r before its rounding.  1 <= C <= 8192."""
+    if x.shape != h.shape or x.dim() < 2:
+        raise ValueError(f"residual_norm: x {tuple(x.shape)} and h {tuple(h.shape)} have to be of one shape (..., C)")
+    if (x.dtype, h.dtype) not in ((torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16)):
+        raise ValueError(f"residual_norm: x {x.dtype} with h {h.dtype} is not supported")
+    C = x.shape[-1]
+    if not 1 <= C <= 8192:
+        raise ValueError(f"residual_norm: {C} channels, 1 to 8192 are supported")
+    post, w1, b1, eps1 = _norm_spec(post, C, h.dtype, "post")
+    pre, w2, b2, eps2 = _norm_spec(pre, C, x.dtype, "pre")
+    rows = x.numel() // C
+    B, N, gmode = 1, rows, 0
+    if gate is not None:
+        if gate.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"residual_norm: gate dtype {gate.dtype}")
+        if gate.shape == x.shape:
+            gmode = 2
+        elif x.dim() == 3 and gate.shape == (x.shape[0], 1, C):
+            gmode, B, N = 1, x.shape[0], x.shape[1]
+        else:
+            raise ValueError(f"residual_norm: gate {tuple(gate.shape)} has to be {tuple(x.shape)} or (B, 1, {C}) with x (B, N, {C})")
+    if scale is not None and tuple(scale.shape) != (C,):
+        raise ValueError(f"residual_norm: scale {tuple(scale.shape)} has to be ({C},)")
+    if N >= 2 ** 31 or B > 65530:
+        raise ValueError(f"residual_norm: {B} samples of {N} rows")
+    if scale is not None and scale.dtype != torch.float32:
+        scale = scale.float()
+    ins = [t.contiguous() if t is not None else None for t in (x, h, gate, scale, w1, b1, w2, b2)]
+    L.require_gpu(*ins)
+    meta = (post, pre, eps1, eps2, gmode, B, N)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins):
+        return ResidualNormFn.apply(*ins, meta)
+    r, y, _ = _residual_norm_fwd(*ins, meta, False)
+    return (r, y) if pre else r
+
+
+def _topk_distill_fwd(logits, values, index, temp, keep):
+    R, V = logits.shape
+    loss = torch.empty(R, dtype=torch.float32, device=logits.device)
+    lse = torch.empty(R, dtype=torch.float32, device=logits.device) if keep else None
+    if R:
+        with _here(logits, values, index):
+            L.check(L.load().passion_topk_distill_fwd(_p(logits), L.dtype_code(logits.dtype), _p(values), L.dtype_code(values.dtype), _p(index),
+                                                      int(index.dtype == torch.int64), R, V, index.shape[1], temp, _p(loss), _p(lse), L.stream_ptr()),
+                    "passion_topk_distill_fwd")
+    return loss, lse
+
+
+class TopkDistillFn(torch.autograd.Function):
+    """csrc/distill.hip: forward keeps one log-sum-exp a row, backward reads the logits once more"""
+
+    @staticmethod
+    def forward(ctx, logits, values, index, temp):
+        loss, lse = _topk_distill_fwd(logits, values, index, temp, True)
+        ctx.save_for_backward(logits, values, index, lse)
+        ctx.temp = temp
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, values, index, lse = ctx.saved_tensors
+        R, V = logits.shape
+        d = torch.empty_like(logits)
+        if R:
+            g = g.float().contiguous()
+            with _here(logits, g):
+                L.check(L.load().passion_topk_distill_bwd(_p(logits), L.dtype_code(logits.dtype), _p(values), L.dtype_code(values.dtype), _p(index),
+                                                          int(index.dtype == torch.int64), R, V, index.shape[1], ctx.temp, _p(lse), _p(g), _p(d),
+                                                          L.stream_ptr()), "passion_topk_distill_bwd")
+        return d, None, None, None
+
+
+def topk_distill(logits, values, index, temp=1.0):
+    """Distillation loss per row against a teacher of whom only the top K logits were kept: T^2 sum_k p_k (log p_k - log q[index_k]), p = softmax(values / T)
+    over the K entries, q = softmax(logits / T) over all V classes (kl_probs holds the student against the whole distribution).
+    logits (..., V) f32 / bf16; values (..., K) f32 / bf16 and index (..., K) int32 / int64 of the same leading shape, no gradient; K <= 1024.
+    -> (...) f32.  An entry whose index is not in [0, V) is absent (padding: -1); a row without entries has loss 0 and gradient 0, whatever its logits."""
+    if logits.dim() < 1 or values.shape != index.shape or values.shape[:-1] != logits.shape[:-1] or values.dim() != logits.dim():
+        raise ValueError(f"topk_distill: logits {tuple(logits.shape)}, values {tuple(values.shape)}, index {tuple(index.shape)} do not belong together")
+    V, K = logits.shape[-1], values.shape[-1]
+    if V < 1 or V >= 2 ** 31 or not 1 <= K <= 1024:
+        raise ValueError(f"topk_distill: {V} classes, {K} entries a row (1 to 1024)")
+    if index.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"topk_distill: index dtype {index.dtype}")
+    for t in (logits, values):
+        if t.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"topk_distill: dtype {t.dtype}")
+    temp = float(temp)
+    if not 0.0 < temp < float("inf"):
+        raise ValueError(f"topk_distill: temperature {temp}")
+    lead = logits.shape[:-1]
+    s = logits.reshape(-1, V).contiguous()
+    if s.data_ptr() % 16:
+        s = s.clone()
+    tv, ti = values.detach().reshape(-1, K).contiguous(), index.reshape(-1, K).contiguous()
+    L.require_gpu(s, tv, ti)
+    if torch.is_grad_enabled() and s.requires_grad:
+        return TopkDistillFn.apply(s, tv, ti, temp).reshape(lead)
+    return _topk_distill_fwd(s, tv, ti, temp, False)[0].reshape(lead)
 
 
 # ------------------------------------------------------------------------------------------------
