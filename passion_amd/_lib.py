@@ -181,6 +181,9 @@ SIGNATURES = {
                                          c_void_p]),
     "passion_topk_distill_bwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_int, c_float, c_void_p, c_void_p,
                                          c_void_p, c_void_p]),
+    "passion_rel_attn_workspace_floats": (c_int64, [c_int] * 15),
+    "passion_rel_attn_fwd": (c_int, [c_void_p] * 6 + [c_int] * 11 + [c_void_p, c_int, c_void_p, c_int, c_void_p, c_float] + [c_void_p] * 4),
+    "passion_rel_attn_bwd": (c_int, [c_void_p] * 6 + [c_int] * 11 + [c_void_p, c_int, c_void_p, c_int, c_void_p, c_float] + [c_void_p] * 9),
     "passion_set_option": (c_int, [c_char_p, c_int]),
     "passion_prof_enable": (None, [c_int]),
     "passion_prof_filter": (None, [c_double, c_double]),

@@ -1,0 +1,329 @@
+// Attention with a learned relative position bias, forward and backward: host side and the small kernels (the large ones: rel_attn_body.h).
+//
+// Tokens lie in raster order on a grid (gd, gh, gw); token t sits at cell t mod (gd gh gw) (further modalities repeat the grid), query i is token
+// q_start + i.  With o(i, j) the index of cell_i - cell_j among the (2 gd - 1)(2 gh - 1)(2 gw - 1) offsets:
+//     s_ij = scale q_i . k_j + table[buckets[o(i, j)]][head]       (masked keys and entries at or below -1e30 are excluded)
+//     p_i = softmax_j(s_ij), out_i = sum_j p_ij v_j                 (a row with nothing left: 0)
+// backward, from the saved row log-sum-exp, with nothing of size Nq x Nk in memory:
+//     delta_i = dout_i . out_i,  dS = p (dout v^T - delta),  dq = scale dS k,  dk = scale dS^T q,  dv = p^T dout,  dtable[c] = sum over pairs of bucket c of dS
+// The reference's SelfAttention (code/models/mmformer.py:192-227) has learned absolute positions instead; its tokens are such a grid.
+//
+// Two backward kernels as in flash_attn.hip: query-major (dq and the table's sums) and key-major (dk, dv: the heads that share a key / value head
+// sum in registers); both free of atomics between wavefronts.
+#include "common.h"
+#include "passion_hip.h"
+#include "rel_attn.h"
+
+namespace {
+
+constexpr int BOX_MAX = 4096;           // offsets whose table (and four histograms of it) fit LDS beside the tiles
+
+// e[h][o] = log2 units of the head's bias at offset o
+__global__ __launch_bounds__(256) void rel_expand_kernel(const void* table, int tdt, const int* buckets, int nb, int nd, int H, float* e) {
+    const int o = blockIdx.x * 256 + threadIdx.x;
+    if (o >= nd) return;
+    const int c = buckets ? buckets[o] : o;
+    for (int h = blockIdx.y; h < H; h += gridDim.y) e[(long)h * nd + o] = rel_log2_bias(table, tdt, c, nb, h, H);
+}
+
+__global__ __launch_bounds__(256) void rel_zero_kernel(float* p, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.f;
+}
+
+// delta[b][h][q] = dout . out: 16 lanes a row
+template <typename T>
+__global__ __launch_bounds__(256) void rel_delta_kernel(const T* o, const T* dout, float* delta, int B, int Nq, int H, int D) {
+    const long row = ((long)blockIdx.x * 256 + threadIdx.x) >> 4;             // (b Nq + q) H + h
+    const int c = (threadIdx.x & 15) * 8;
+    float s = 0.f;
+    if (row < (long)B * Nq * H && c < D) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const f32x4 a = load4(o + row * D + c + 4 * u), g = load4(dout + row * D + c + 4 * u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s = __builtin_fmaf(a[j], g[j], s);
+        }
+    }
+    s = group16_sum(s);
+    if ((threadIdx.x & 15) == 0 && row < (long)B * Nq * H) {
+        const long bq = row / H;
+        delta[((bq / Nq) * H + row % H) * Nq + bq % Nq] = s;
+    }
+}
+
+// merge of the split forward: 32 lanes a row, 4 columns a lane
+template <typename T>
+__global__ __launch_bounds__(256) void rel_combine_kernel(RelP p) {
+    const long rows = (long)p.B * p.H * p.Nq, row = (long)blockIdx.x * 8 + threadIdx.x / 32;       // (b H + h) Nq + q
+    const int d = (threadIdx.x & 31) * 4;
+    if (row >= rows) return;
+    float M = -INFINITY;
+    for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, p.pm[s * rows + row]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float w = __builtin_amdgcn_exp2f(p.pm[s * rows + row] - ref);          // an empty split: exp2(-inf) = 0
+        L = __builtin_fmaf(w, p.pl[s * rows + row], L);
+        if (d < p.D) {
+            const f32x4 v = load4(p.po + (s * rows + row) * p.D + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = __builtin_fmaf(w, v[j], a[j]);
+        }
+    }
+    const float f = L == 0.f ? 0.f : 1.f / L;
+    const long bh = row / p.Nq, q = row % p.Nq, b = bh / p.H, h = bh % p.H;
+    if (d < p.D) store4(static_cast<T*>(p.out) + ((b * p.Nq + q) * p.H + h) * p.D + d, (f32x4){a[0] * f, a[1] * f, a[2] * f, a[3] * f});
+    if (d == 0 && p.lse) p.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+}
+
+// G[h][o] = sum of the slab rows (b, tile) in order; four runs of rows a workgroup, joined in order.  line > 0: the rows are windows (row `tile`
+// begins at offset (gw - 1) + q_start + 32 tile - line + 1).  identity: written as the table's gradient at once
+struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, nd, tiles, line, base; };
+__global__ __launch_bounds__(256) void rel_fold_kernel(FoldP f) {
+    __shared__ float red[4][64];
+    const int o = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6, h = blockIdx.y;
+    const long n = (long)f.B * f.tiles, i0 = n * run / 4, i1 = n * (run + 1) / 4;
+    float s = 0.f;
+    if (o < f.nd)
+        for (long i = i0; i < i1; ++i) {
+            const int b = (int)(i / f.tiles), t = (int)(i % f.tiles);
+            const long u = f.line ? (long)o - f.base - 32L * t + f.line - 1 : o;
+            if (u >= 0 && u < f.len) s += f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + u];
+        }
+    red[run][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (run == 0 && o < f.nd) {
+        s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+        if (f.dt) {
+            if (f.tdt == PASSION_BF16) static_cast<bf16_t*>(f.dt)[(long)o * f.H + h] = (bf16_t)s;
+            else static_cast<float*>(f.dt)[(long)o * f.H + h] = s;
+        } else f.G[(long)h * f.nd + o] = s;
+    }
+}
+
+// dtable[c][h] = sum of G[h][o] over the offsets of bucket c.  Few buckets: a workgroup a bucket; many: a thread a bucket, the map in LDS
+template <typename TT>
+__global__ __launch_bounds__(256) void rel_bucket_few_kernel(const float* G, const int* buckets, TT* dt, int nd, int H) {
+    __shared__ float red[4];
+    const int c = blockIdx.x, h = blockIdx.y;
+    float s = 0.f;
+    for (int o = threadIdx.x; o < nd; o += 256) s += buckets[o] == c ? G[(long)h * nd + o] : 0.f;
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) dt[(long)c * H + h] = from_f32<TT>((red[0] + red[1]) + (red[2] + red[3]));
+}
+template <typename TT>
+__global__ __launch_bounds__(256) void rel_bucket_many_kernel(const float* G, const int* buckets, TT* dt, int nd, int nb, int H) {
+    __shared__ int bk[1024];
+    __shared__ float gv[1024];
+    const int c = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    float s = 0.f;
+    for (int o0 = 0; o0 < nd; o0 += 1024) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 1024; i += 256) {
+            bk[i] = o0 + i < nd ? buckets[o0 + i] : -1;
+            gv[i] = o0 + i < nd ? G[(long)h * nd + o0 + i] : 0.f;
+        }
+        __syncthreads();
+        for (int i = 0; i < 1024; ++i)
+            if (bk[i] == c) s += gv[i];
+    }
+    if (c < nb) dt[(long)c * H + h] = from_f32<TT>(s);
+}
+
+int blk_of(int dtype) { return dtype == PASSION_BF16 ? 64 : 32; }
+long tiles32(long n) { return (n + 31) / 32; }
+
+// which way to the bias: a 1D raster without wrap-around by windows, a small box of offsets from LDS, else from memory
+int bias_mode(const RelP& p) {
+    if (!p.table) return 0;
+    if (p.gd == 1 && p.gh == 1 && p.Nk <= p.gw && p.q0 + p.Nq <= p.gw) return 2;
+    return p.nd <= BOX_MAX ? 1 : 3;
+}
+// few query rows: all heads of a key / value head in one tile, the bias read straight from the table (an expansion of all offsets would cost more)
+bool few_rows(const RelP& p) { return (long)p.Nq * (p.H / p.Hkv) <= 32 && p.Nq <= 16; }
+
+// the forward's key ranges: enough wavefronts for two to four per SIMD ... of 1024 SIMDs, two blocks of keys each at least
+int pick_split(const RelP& p, int dtype) {
+    const long tiles = (p.pack ? tiles32((long)p.Nq * (p.H / p.Hkv)) * p.Hkv : tiles32(p.Nq) * p.H) * p.B;
+    const int nblk = (p.Nk + blk_of(dtype) - 1) / blk_of(dtype);
+    int s = 1;
+    while (tiles * s < 1024 && nblk / (2 * s) >= 2) s *= 2;
+    return s;
+}
+// wavefronts a workgroup: 4 share the staged tiles where that leaves every CU a workgroup and the rows fill them
+int pick_waves(long rows32, long others) { return rows32 >= 4 && rows32 * others >= 1024 ? 4 : 1; }
+
+int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start, const void* table, int tdt, const int* buckets, int nb,
+          const uint8_t* mask, float scale) {
+    if ((dtype != PASSION_F32 && dtype != PASSION_BF16) || B < 1 || B > 65535 || Nq < 1 || Nk < 1 || H < 1 || Hkv < 1 || H % Hkv || H > 65535) return -1003;
+    if (D < 8 || D > 128 || D % 8) return -1003;
+    if (Nq > (1 << 30) || Nk > (1 << 30) || q_start < 0 || q_start > (1 << 30)) return -1003;
+    if (table) {
+        if (gd < 1 || gh < 1 || gw < 1 || (tdt != PASSION_F32 && tdt != PASSION_BF16) || nb < 1) return -1003;
+        const int64_t a = 2LL * gd - 1, b = 2LL * gh - 1, c = 2LL * gw - 1;
+        if (a > (1 << 30) || b > (1 << 30) || c > (1LL << 31) || a * b > (1 << 30) || a * b * c > (1LL << 30)) return -1003;
+        p.gd = gd; p.gh = gh; p.gw = gw; p.vol = gd * gh * gw; p.nd = (int)(a * b * c);
+        p.omax = ((gd - 1) * (2 * gh - 1) + gh - 1) * (2 * gw - 1) + gw - 1;
+        if (!buckets && nb != p.nd) return -1003;
+        p.table = table; p.buckets = buckets; p.nb = nb; p.tdt = tdt;
+    }
+    p.B = B; p.Nq = Nq; p.Nk = Nk; p.H = H; p.Hkv = Hkv; p.D = D; p.q0 = q_start; p.mask = mask;
+    p.scale = scale; p.c = scale * 1.4426950408889634f;
+    p.nsplit = 1;
+    p.bias = bias_mode(p);
+    return 0;
+}
+
+// slab rows (per batch sample and head) and their length
+void slab_shape(const RelP& p, int dtype, int nw, long& tiles, long& len) {
+    if (p.bias == 1) { tiles = (p.Nq + 32 * nw - 1) / (32 * nw); len = p.nd; }
+    else if (p.bias == 2) { tiles = tiles32(p.Nq); len = (long)blk_of(dtype) * ((p.Nk + blk_of(dtype) - 1) / blk_of(dtype)) + 31; }
+    else { tiles = tiles32(p.Nq); len = p.nd; }
+}
+
+int run(const RelP& p, int dtype, int what, int nw, hipStream_t st) { return dtype == PASSION_BF16 ? rel_run_bf16(p, what, nw, st) : rel_run_f32(p, what, nw, st); }
+
+// layout of the workspaces, in floats
+struct Ws { long e, po, pm, pl, delta, slab, G, total; };
+Ws fwd_ws(RelP& p, int dtype) {
+    p.pack = few_rows(p) && p.H > p.Hkv;
+    if (p.bias && few_rows(p)) p.bias = 3;
+    p.nsplit = pick_split(p, dtype);
+    const long rows = (long)p.B * p.H * p.Nq;
+    Ws w{};
+    long at = 0;
+    auto take = [&](long n) { const long r = at; at += (n + 63) / 64 * 64; return r; };
+    w.e = take(p.bias && !few_rows(p) ? (long)p.H * p.nd : 0);
+    w.po = take(p.nsplit > 1 ? p.nsplit * rows * p.D : 0);
+    w.pm = take(p.nsplit > 1 ? p.nsplit * rows : 0);
+    w.pl = take(p.nsplit > 1 ? p.nsplit * rows : 0);
+    w.total = at;
+    return w;
+}
+Ws bwd_ws(RelP& p, int dtype, bool want_table, int nw) {
+    Ws w{};
+    long at = 0;
+    auto take = [&](long n) { const long r = at; at += (n + 63) / 64 * 64; return r; };
+    w.e = take(p.bias ? (long)p.H * p.nd : 0);
+    w.delta = take((long)p.B * p.H * p.Nq);
+    if (p.bias && want_table) {
+        long tiles, len;
+        slab_shape(p, dtype, nw, tiles, len);
+        w.slab = take((long)p.B * p.H * tiles * len);
+        w.G = take(p.buckets ? (long)p.H * p.nd : 0);
+    }
+    w.total = at;
+    return w;
+}
+int q_waves(const RelP& p) { return pick_waves(tiles32(p.Nq), (long)p.H * p.B); }
+
+int expand(RelP& p, float* e, hipStream_t st) {
+    hipLaunchKernelGGL(rel_expand_kernel, dim3((p.nd + 255) / 256, p.H < 8 ? p.H : 8), dim3(256), 0, st, p.table, p.tdt, p.buckets, p.nb, p.nd, p.H, e);
+    LAUNCH_RET();
+    p.e = e;
+    return 0;
+}
+bool misaligned(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0; }
+int strides(RelP& p, int dtype, const int64_t* sq, const int64_t* sk, const int64_t* sv) {
+    const int unit = dtype == PASSION_BF16 ? 8 : 4;
+    for (int i = 0; i < 3; ++i) {
+        if (sq[i] % unit || sk[i] % unit || sv[i] % unit) return -1005;
+        p.qs[i] = sq[i]; p.ks[i] = sk[i]; p.vs[i] = sv[i];
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int64_t passion_rel_attn_workspace_floats(int dtype, int backward, int B, int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start,
+                                                     int has_table, int has_buckets, int nb) {
+    RelP p{};
+    static const int dummy = 0;
+    const int rc = setup(p, dtype, B, Nq, Nk, H, Hkv, D, gd, gh, gw, q_start, has_table ? &dummy : nullptr, PASSION_F32, has_buckets ? &dummy : nullptr, nb, nullptr, 1.f);
+    if (rc) return rc;
+    return backward ? bwd_ws(p, dtype, true, q_waves(p)).total : fwd_ws(p, dtype).total;
+}
+
+extern "C" int passion_rel_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype, int B,
+                                    int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start, const void* table, int table_dtype, const int* buckets,
+                                    int nb, const uint8_t* mask, float scale, void* out, float* lse, float* workspace, void* stream) {
+    RelP p{};
+    int rc = setup(p, dtype, B, Nq, Nk, H, Hkv, D, gd, gh, gw, q_start, table, table_dtype, buckets, nb, mask, scale);
+    if (rc) return rc;
+    if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides) return -1003;
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || (workspace && misaligned(workspace))) return -1005;
+    if ((rc = strides(p, dtype, q_strides, k_strides, v_strides))) return rc;
+    p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse;
+    hipStream_t st = (hipStream_t)stream;
+    const Ws w = fwd_ws(p, dtype);
+    if (w.total && !workspace) return -1003;
+    if (p.bias && !few_rows(p) && (rc = expand(p, workspace + w.e, st))) return rc;
+    p.po = workspace + w.po; p.pm = workspace + w.pm; p.pl = workspace + w.pl;
+    const long rows32 = p.pack ? tiles32((long)p.Nq * (p.H / p.Hkv)) : tiles32(p.Nq);
+    if ((rc = run(p, dtype, 0, pick_waves(rows32, (long)(p.pack ? p.Hkv : p.H) * p.B * p.nsplit), st))) return rc;
+    if (p.nsplit > 1) {
+        const long rows = (long)p.B * p.H * p.Nq;
+        if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_combine_kernel<bf16_t>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL(rel_combine_kernel<float>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+        LAUNCH_RET();
+    }
+    return 0;
+}
+
+extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype, int B,
+                                    int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start, const void* table, int table_dtype, const int* buckets,
+                                    int nb, const uint8_t* mask, float scale, const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv, void* dtable,
+                                    float* workspace, void* stream) {
+    RelP p{};
+    int rc = setup(p, dtype, B, Nq, Nk, H, Hkv, D, gd, gh, gw, q_start, table, table_dtype, buckets, nb, mask, scale);
+    if (rc) return rc;
+    if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace || !q_strides || !k_strides || !v_strides || (dtable && !table)) return -1003;
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(dout) || misaligned(dq) || misaligned(dk) || misaligned(dv) || misaligned(workspace))
+        return -1005;
+    if ((rc = strides(p, dtype, q_strides, k_strides, v_strides))) return rc;
+    p.q = q; p.k = k; p.v = v; p.o = out; p.dout = dout; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
+    hipStream_t st = (hipStream_t)stream;
+    const int nw = q_waves(p);
+    const Ws w = bwd_ws(p, dtype, dtable != nullptr, nw);
+    if (p.bias && (rc = expand(p, workspace + w.e, st))) return rc;
+    p.delta = workspace + w.delta;
+    const long rows16 = (long)B * Nq * H * 16;
+    if (dtype == PASSION_BF16)
+        hipLaunchKernelGGL(rel_delta_kernel<bf16_t>, dim3((unsigned)((rows16 + 255) / 256)), dim3(256), 0, st, (const bf16_t*)out, (const bf16_t*)dout, p.delta, B, Nq, H, D);
+    else hipLaunchKernelGGL(rel_delta_kernel<float>, dim3((unsigned)((rows16 + 255) / 256)), dim3(256), 0, st, (const float*)out, (const float*)dout, p.delta, B, Nq, H, D);
+    LAUNCH_RET();
+    long tiles = 0, len = 0;
+    if (dtable) {
+        slab_shape(p, dtype, nw, tiles, len);
+        p.slab = workspace + w.slab;
+        p.slab_len = len;
+        if (p.bias == 3) {
+            hipLaunchKernelGGL(rel_zero_kernel, dim3(2048), dim3(256), 0, st, p.slab, (long)B * H * tiles * len);
+            LAUNCH_RET();
+        }
+    }
+    if ((rc = run(p, dtype, 1, nw, st))) return rc;
+    if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B), st))) return rc;
+    if (dtable) {
+        float* G = workspace + w.G;
+        const FoldP f{p.slab, G, buckets ? nullptr : dtable, len, table_dtype, B, H, p.nd, (int)tiles, p.bias == 2 ? blk_of(dtype) * ((Nk + blk_of(dtype) - 1) / blk_of(dtype)) : 0,
+                      p.gw - 1 + p.q0};
+        hipLaunchKernelGGL(rel_fold_kernel, dim3((p.nd + 63) / 64, H), dim3(256), 0, st, f);
+        LAUNCH_RET();
+        if (buckets) {
+            const bool few = nb <= 256;
+            if (table_dtype == PASSION_BF16) {
+                if (few) hipLaunchKernelGGL(rel_bucket_few_kernel<bf16_t>, dim3(nb, H), dim3(256), 0, st, G, buckets, (bf16_t*)dtable, p.nd, H);
+                else hipLaunchKernelGGL(rel_bucket_many_kernel<bf16_t>, dim3((nb + 255) / 256, H), dim3(256), 0, st, G, buckets, (bf16_t*)dtable, p.nd, nb, H);
+            } else {
+                if (few) hipLaunchKernelGGL(rel_bucket_few_kernel<float>, dim3(nb, H), dim3(256), 0, st, G, buckets, (float*)dtable, p.nd, H);
+                else hipLaunchKernelGGL(rel_bucket_many_kernel<float>, dim3((nb + 255) / 256, H), dim3(256), 0, st, G, buckets, (float*)dtable, p.nd, nb, H);
+            }
+            LAUNCH_RET();
+        }
+    }
+    return 0;
+}

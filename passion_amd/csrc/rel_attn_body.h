@@ -1,0 +1,603 @@
+// Kernels of attention with a learned relative position bias (host side and the mathematics: rel_attn.hip).  Included once per tensor type.
+//
+// Score tiles as in flash_attn.hip: S^T[key][q] = K . Q^T with 32x32 matrix instructions, a lane owns one query (column l & 31) and 16 of the
+// tile's 32 keys (rows (r & 3) + 8 (r >> 2) + 4 (l >> 5)), so a row's maximum and sum are in registers plus one exchange with lane l ^ 32, and
+// the probabilities are the B operand of the next product where they stand.  The key-major kernel is the mirror image.
+//   bf16: v_mfma_f32_32x32x16_bf16, 16 bytes of a row a lane and instruction; transposed operands by ds_read_b64_tr_b16.
+//   f32:  v_mfma_f32_32x32x2_f32, four instructions per 16 bytes (the four k pairs a lane's 16 bytes hold); accumulator register r as the B
+//         operand of one instruction, whose A operand is a plain b32 read of image row (r & 3) + 8 (r >> 2) + 4 (l >> 5).  Full f32 products.
+//
+// Bias of a pair, in log2 units, by its offset o(i, j) = pos(i) - pos(j) + const:
+//   BOX    the head's whole expanded table in LDS (up to 4096 offsets: grids up to 8 x 8 x 8 and a little beyond), one LDS read a score;
+//   LINE   a 1D raster: the offsets of a (query tile, key block) pair are one window of 32 NW + BLK - 1 values, staged with the block, and the LDS
+//          address of a score is a lane constant plus an immediate;
+//   GATHER one global read a score (L1 / L2), any grid.
+// Gradient of the table: sums of dS by offset, without atomics between wavefronts.  Every wavefront of the query-major kernel owns a histogram
+// and adds its dS in program order: BOX the whole table in LDS, LINE a sliding window of BLK + 31 values (BLK leave it for good after a block),
+// GATHER a slab row in global memory.  Slab rows are folded in order afterwards.
+#include "common.h"
+#include "passion_hip.h"
+#include "rel_attn.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LAZY = 8.0f;           // log2 units by which a block must exceed the running reference before it moves
+enum { NONE = 0, BOX = 1, LINE = 2, GATHER = 3 };
+
+template <typename T> constexpr int blk() { return sizeof(T) == 2 ? 64 : 32; }                       // rows staged a step
+template <typename T, int DP> constexpr int row_stride() { return DP * (int)sizeof(T) + 16; }        // row reads: 16 rows hit 16 bank groups
+// image that is only read transposed: bf16 wants 4 consecutive rows' 64 bytes in disjoint 16-bank windows (stride mod 256 = 64 or 192)
+template <typename T, int DP> constexpr int tr_stride() { return sizeof(T) == 4 ? DP * 4 + 16 : DP == 32 ? 64 : DP * 2 + 64; }
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) z[j] = 0.f;
+    return z;
+}
+__device__ __forceinline__ float half_max(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// acc += A . B over the k range of one 16-byte chunk a lane
+template <typename T> __device__ __forceinline__ f32x16 dot(u32x4 a, u32x4 b, f32x16 acc) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+    else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[t]), __uint_as_float(b[t]), acc, 0, 0, 0);
+        return acc;
+    }
+}
+// row fragment: lane (row r0 + (l & 31), half l >> 5), 16-byte chunk ch
+template <typename T> __device__ __forceinline__ u32x4 row_frag(const char* img, int stride, int r0, int ch, int lane) {
+    return *reinterpret_cast<const u32x4*>(img + (r0 + (lane & 31)) * stride + 32 * ch + 16 * (lane >> 5));
+}
+// out[dt] += (image rows r0 .. r0 + 31, columns 32 dt ..)^T . acc, acc an accumulator tile whose rows are those image rows
+template <typename T, int ND>
+__device__ __forceinline__ void tr_product(const char* img, int stride, int r0, const f32x16& acc, f32x16 (&out)[ND], int lane) {
+    if constexpr (sizeof(T) == 2) {
+        const int n = lane & 15, g = lane >> 4, h = g >> 1, q4 = n >> 2, pq = n & 3;
+        const char* base = img + (r0 + 4 * h + q4) * stride + (16 * (g & 1) + 4 * pq) * 2;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            bf16x8 b;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = (__bf16)acc[8 * s + j];
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+                const char* p0 = base + 16 * s * stride + dt * 64;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p0));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p0 + 8 * stride));
+                const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, out[dt], 0, 0, 0);
+            }
+        }
+    } else {
+        const char* base = img + (r0 + 4 * (lane >> 5)) * stride + (lane & 31) * 4;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+                out[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(base + ((r & 3) + 8 * (r >> 2)) * stride + dt * 128), acc[r], out[dt], 0, 0, 0);
+    }
+}
+
+// a tile of BLK rows x DP columns in registers, NT threads; rows past n (or masked: keep[row] = 0) and columns past D are zero
+template <typename T, int DP, int NT> struct Tile {
+    static constexpr int CPR = DP * (int)sizeof(T) / 16, N = blk<T>() * CPR / NT;
+    u32x4 r[N];
+    __device__ __forceinline__ void fetch(const T* base, long rowstride, int row0, int n, int D, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int ci = i * NT + tid, row = ci / CPR, c = ci % CPR;
+            r[i] = (u32x4){0u, 0u, 0u, 0u};
+            if (row0 + row < n && c * 16 < D * (int)sizeof(T))
+                r[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base + (long)(row0 + row) * rowstride) + c * 16);
+        }
+    }
+    __device__ __forceinline__ void commit(char* img, int stride, int tid, uint64_t valid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int ci = i * NT + tid, row = ci / CPR, c = ci % CPR;
+            *reinterpret_cast<u32x4*>(img + row * stride + c * 16) = (valid >> row) & 1 ? r[i] : (u32x4){0u, 0u, 0u, 0u};
+        }
+    }
+};
+
+// place of token t in the box of offsets (before the constant that makes differences non-negative)
+__device__ __forceinline__ int place(const RelP& p, int t) {
+    t %= p.vol;
+    const int z = t / (p.gh * p.gw), yx = t - z * (p.gh * p.gw), y = yx / p.gw, x = yx - y * p.gw;
+    return (z * (2 * p.gh - 1) + y) * (2 * p.gw - 1) + x;
+}
+// GATHER: bias of head `head` at offset o: the expanded table, or (few queries: no expansion pass) the table itself
+__device__ __forceinline__ float gather_bias(const RelP& p, int head, int o) {
+    if (p.e) return p.e[(long)head * p.nd + o];
+    return rel_log2_bias(p.table, p.tdt, p.buckets ? p.buckets[o] : o, p.nb, head, p.H);
+}
+
+// valid keys of a block of BLK, one bit each (every wavefront forms it for itself: lanes hold one key each)
+template <int BLKN>
+__device__ __forceinline__ uint64_t valid_keys(const RelP& p, int b, int key0, int lane) {
+    const int key = key0 + lane;
+    const bool ok = lane < BLKN && key < p.Nk && (!p.mask || p.mask[(long)b * p.Nk + key]);
+    return __ballot(ok);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// query-major: MODE 0 forward (out, lse or split partials), MODE 1 backward (dQ and the table's histogram).
+// grid (ceil(rows / (32 NW)) * nsplit, heads, B).  pack (forward, few queries): a workgroup's rows are the Nq queries of all the heads that
+// share a key / value head, so that K and V are read once for them
+template <typename T, int DP, int NW, int MODE, int BIAS>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_q_kernel(RelP p) {
+    constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
+    constexpr int RS = row_stride<T, DP>(), VS = MODE == 0 ? tr_stride<T, DP>() : RS;
+    constexpr int KIMG = BLKN * RS, VIMG = BLKN * VS, POS = BLKN * 4, WIN = (32 * NW + BLKN) * 4;
+    constexpr int BUF = KIMG + VIMG + (BIAS == LINE ? WIN : BIAS == NONE ? 0 : POS);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int b = blockIdx.z, rep = p.H / p.Hkv;
+    const int split = blockIdx.x % p.nsplit, tile = blockIdx.x / p.nsplit;
+    const int rows = p.pack ? p.Nq * rep : p.Nq;
+    const int row = (tile * NW + wv) * 32 + (lane & 31);
+    const bool qok = row < rows;
+    const int rowc = qok ? row : rows - 1;
+    const int head = p.pack ? blockIdx.y * rep + rowc / p.Nq : blockIdx.y, qi = p.pack ? rowc % p.Nq : rowc;
+    const int hk = p.pack ? blockIdx.y : blockIdx.y / rep;
+    const T* kb_ = static_cast<const T*>(p.k) + (long)b * p.ks[0] + (long)hk * p.ks[2];
+    const T* vb_ = static_cast<const T*>(p.v) + (long)b * p.vs[0] + (long)hk * p.vs[2];
+    const int nblk_all = (p.Nk + BLKN - 1) / BLKN;
+    const int kb0 = (int)((long)split * nblk_all / p.nsplit), kb1 = (int)((long)(split + 1) * nblk_all / p.nsplit);
+    const long orow = ((long)b * p.Nq + qi) * p.H + head, lrow = ((long)b * p.H + head) * p.Nq + qi;
+
+    u32x4 qf[NCH], df[MODE == 1 ? NCH : 1];
+    {
+        const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)qi * p.qs[1] + (long)head * p.qs[2]);
+        const char* dp = MODE == 1 ? reinterpret_cast<const char*>(static_cast<const T*>(p.dout) + orow * p.D) : nullptr;
+#pragma unroll
+        for (int s = 0; s < NCH; ++s) {
+            const bool in = qok && (32 * s + 16 * h) < p.D * (int)sizeof(T);
+            qf[s] = (u32x4){0u, 0u, 0u, 0u};
+            if (in) qf[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s + 16 * h);
+            if (MODE == 1) {
+                df[s] = (u32x4){0u, 0u, 0u, 0u};
+                if (in) df[s] = *reinterpret_cast<const u32x4*>(dp + 32 * s + 16 * h);
+            }
+        }
+    }
+    float lse2 = INFINITY, dlt = 0.f;                       // no such query: p = exp2(. - inf) = 0
+    if (MODE == 1 && qok) { lse2 = p.lse[lrow]; dlt = p.delta[lrow]; }
+    const int aq = (BIAS == BOX || BIAS == GATHER) ? place(p, p.q0 + qi) + p.omax : 0;      // offset of a pair = aq - place(key)
+
+    // LDS behind the two buffers: BOX: the head's table, then the wavefronts' histograms; LINE backward: the sliding histograms
+    float* tab = reinterpret_cast<float*>(lds + 2 * BUF);
+    float* hist = BIAS == BOX ? tab + p.nd + wv * p.nd : tab + wv * (BLKN + 32);
+    float* ghist = nullptr;
+    if (BIAS == BOX) {
+        for (int i = tid; i < p.nd; i += NT) tab[i] = p.e[(long)blockIdx.y * p.nd + i];
+        if (MODE == 1 && p.slab) for (int i = lane; i < p.nd; i += 64) hist[i] = 0.f;
+    }
+    if (MODE == 1 && BIAS == LINE) {
+        for (int i = lane; i < BLKN + 32; i += 64) hist[i] = 0.f;
+    }
+    if (MODE == 1 && BIAS != NONE && BIAS != BOX) {
+        const int tiles = (p.Nq + 31) / 32;
+        ghist = p.slab + (((long)b * p.H + blockIdx.y) * tiles + min(tile * NW + wv, tiles - 1)) * p.slab_len;
+    }
+    const bool wave_on = tile * NW + wv < (rows + 31) / 32;       // a wavefront without a row stages tiles and keeps out of the rest
+
+    f32x16 o[ND];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) o[dt] = zero16();
+    float l_run = 0.f, m_run = -INFINITY;
+
+    Tile<T, DP, NT> kt_, vt_;
+    uint64_t vnext = 0;
+    constexpr int NWIN = (32 * NW + BLKN + NT - 1) / NT;
+    float win[BIAS == LINE ? NWIN : 1];
+    int kpos = 0;
+    auto fetch = [&](int kb) {
+        kt_.fetch(kb_, p.ks[1], kb * BLKN, p.Nk, p.D, tid);
+        vt_.fetch(vb_, p.vs[1], kb * BLKN, p.Nk, p.D, tid);
+        vnext = valid_keys<BLKN>(p, b, kb * BLKN, lane);
+        if (BIAS == LINE) {
+            // window value w <-> offset of (query tile 0 of the workgroup, last key of the block) + w
+            const int first = p.q0 + tile * NW * 32 - (kb * BLKN + BLKN - 1) + p.gw - 1;
+#pragma unroll
+            for (int i = 0; i < NWIN; ++i) {
+                const int at = first + i * NT + tid;
+                win[i] = (i * NT + tid < 32 * NW + BLKN && at >= 0 && at < p.nd) ? p.e[(long)blockIdx.y * p.nd + at] : 0.f;
+            }
+        }
+        if ((BIAS == BOX || BIAS == GATHER) && tid < BLKN) kpos = place(p, min(kb * BLKN + tid, p.Nk - 1));
+    };
+    auto commit = [&](char* buf) {
+        kt_.commit(buf, RS, tid, vnext);
+        vt_.commit(buf + KIMG, VS, tid, vnext);
+        if (BIAS == LINE) {
+#pragma unroll
+            for (int i = 0; i < NWIN; ++i)
+                if (i * NT + tid < 32 * NW + BLKN) reinterpret_cast<float*>(buf + KIMG + VIMG)[i * NT + tid] = win[i];
+        }
+        if ((BIAS == BOX || BIAS == GATHER) && tid < BLKN) reinterpret_cast<int*>(buf + KIMG + VIMG)[tid] = kpos;
+    };
+    if (kb0 < kb1) {
+        fetch(kb0);
+        commit(lds);
+    }
+    uint64_t valid = vnext;
+    __syncthreads();
+
+    for (int kb = kb0; kb < kb1; ++kb) {
+        const char* kimg = lds + ((kb - kb0) & 1) * BUF;
+        const char* vimg = kimg + KIMG;
+        if (kb + 1 < kb1) fetch(kb + 1);
+        if (valid && wave_on) {
+            f32x16 st[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                st[kt] = zero16();
+#pragma unroll
+                for (int s = 0; s < NCH; ++s) st[kt] = dot<T>(row_frag<T>(kimg, RS, kt * 32, s, lane), qf[s], st[kt]);
+            }
+            // ---- scores in log2 units: scale * log2(e) * s + bias
+            const float* wl = reinterpret_cast<const float*>(vimg + VIMG) + (32 * wv + (lane & 31) + BLKN - 1 - 4 * h);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    int off[4];
+                    if (BIAS == BOX || BIAS == GATHER) {
+                        const int4 kp = *reinterpret_cast<const int4*>(vimg + VIMG + (kt * 32 + 8 * g4 + 4 * h) * 4);
+                        off[0] = aq - kp.x; off[1] = aq - kp.y; off[2] = aq - kp.z; off[3] = aq - kp.w;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 4 * g4 + j;
+                        if (BIAS == NONE) st[kt][r] *= p.c;
+                        else {
+                            const float bias = BIAS == LINE ? wl[-(kt * 32 + 8 * g4 + j)] : BIAS == BOX ? tab[off[j]] : gather_bias(p, head, off[j]);
+                            st[kt][r] = __builtin_fmaf(st[kt][r], p.c, bias);
+                        }
+                    }
+                }
+            if (valid != (BLKN == 64 ? ~0ull : 0xffffffffull)) {
+                const uint64_t vh = valid >> (4 * h);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!((vh >> (kt * 32 + (r & 3) + 8 * (r >> 2))) & 1)) st[kt][r] = -INFINITY;
+            }
+            if (MODE == 0) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[kt][r]);
+                mx = half_max(mx);
+                const bool move = mx > m_run + LAZY;                              // first key of a row: m_run = -inf
+                if (__any(move)) {
+                    const float m_new = move ? mx : m_run;
+                    const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+                    m_run = m_new;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+                }
+                const float ref = m_run == -INFINITY ? 0.f : m_run;                // nothing left of the row so far: exp2(-inf - 0) = 0
+                float psum = 0.f;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        st[kt][r] = __builtin_amdgcn_exp2f(st[kt][r] - ref);
+                        psum += st[kt][r];
+                    }
+                l_run += psum;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) tr_product<T, ND>(vimg, VS, kt * 32, st[kt], o, lane);
+            } else {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    f32x16 dp = zero16();
+#pragma unroll
+                    for (int s = 0; s < NCH; ++s) dp = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], dp);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) st[kt][r] = __builtin_amdgcn_exp2f(st[kt][r] - lse2) * (dp[r] - dlt);
+                    if (BIAS != NONE && p.slab) {
+                        float* hl = hist + ((lane & 31) + BLKN - 1 - 4 * h);
+#pragma unroll
+                        for (int g4 = 0; g4 < 4; ++g4) {
+                            int4 kp;
+                            if (BIAS == BOX || BIAS == GATHER) kp = *reinterpret_cast<const int4*>(vimg + VIMG + (kt * 32 + 8 * g4 + 4 * h) * 4);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int r = 4 * g4 + j;
+                                const int o_ = aq - (j == 0 ? kp.x : j == 1 ? kp.y : j == 2 ? kp.z : kp.w);
+                                if (BIAS == LINE) __hip_atomic_fetch_add(hl - (kt * 32 + 8 * g4 + j), st[kt][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                                else if (BIAS == BOX) __hip_atomic_fetch_add(hist + o_, st[kt][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                                else unsafeAtomicAdd(ghist + o_, st[kt][r]);
+                            }
+                        }
+                    }
+                    tr_product<T, ND>(kimg, RS, kt * 32, st[kt], o, lane);
+                }
+            }
+        }
+        if (MODE == 1 && BIAS == LINE && p.slab && wave_on) {
+            // offsets that no later block reaches leave the window; 31 move on
+            const int up = BLKN * (nblk_all - 1 - kb);
+            const float mv = lane < 31 ? hist[lane] : 0.f;
+            if (lane < BLKN) ghist[up + 31 + lane] = hist[31 + lane];
+            if (kb == nblk_all - 1) {
+                if (lane < 31) ghist[lane] = mv;
+            } else {
+                __builtin_amdgcn_wave_barrier();
+                if (lane < BLKN) hist[lane] = 0.f;
+                if (lane < 31) hist[BLKN + lane] = mv;
+            }
+        }
+        if (kb + 1 < kb1) commit(lds + ((kb + 1 - kb0) & 1) * BUF);
+        valid = vnext;
+        __syncthreads();
+    }
+
+    if (MODE == 0) {
+        const float l = half_sum(l_run);
+        if (p.nsplit > 1) {
+            if (qok) {
+                const long at = (long)split * p.B * p.H * p.Nq + lrow;
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const int d = dt * 32 + 8 * g4 + 4 * h;
+                        if (d < p.D) store4(p.po + at * p.D + d, (f32x4){o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]});
+                    }
+                if (h == 0) { p.pm[at] = m_run; p.pl[at] = l; }
+            }
+            return;
+        }
+        if (qok) {
+            const float f = l == 0.f ? 0.f : 1.f / l;                              // a row without a key: 0
+            T* dst = static_cast<T*>(p.out) + orow * p.D;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int d = dt * 32 + 8 * g4 + 4 * h;
+                    if (d < p.D) store4(dst + d, (f32x4){o[dt][4 * g4] * f, o[dt][4 * g4 + 1] * f, o[dt][4 * g4 + 2] * f, o[dt][4 * g4 + 3] * f});
+                }
+            if (h == 0 && p.lse) p.lse[lrow] = l == 0.f ? INFINITY : m_run + __builtin_amdgcn_logf(l);
+        }
+    } else {
+        if (qok) {
+            T* dst = static_cast<T*>(p.dq) + orow * p.D;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int d = dt * 32 + 8 * g4 + 4 * h;
+                    if (d < p.D)
+                        store4(dst + d, (f32x4){o[dt][4 * g4] * p.scale, o[dt][4 * g4 + 1] * p.scale, o[dt][4 * g4 + 2] * p.scale, o[dt][4 * g4 + 3] * p.scale});
+                }
+        }
+        if (BIAS == BOX && p.slab) {                 // the workgroup's histograms in wavefront order (the loop ended on a barrier)
+            float* dst = p.slab + (((long)b * p.H + blockIdx.y) * gridDim.x + tile) * p.slab_len;
+            const float* h0 = tab + p.nd;
+            for (int i = tid; i < p.nd; i += NT) {
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) s += h0[w * p.nd + i];
+                dst[i] = s;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// key-major backward: dK, dV.  grid (ceil(Nk / (32 NW)), Hkv, B); a wavefront owns 32 keys and walks the queries of all the heads that share its
+// key / value head, BLK at a time: their gradients sum in registers
+template <typename T, int DP, int NW, int BIAS>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_k_kernel(RelP p) {
+    constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
+    constexpr int RS = row_stride<T, DP>(), IMG = BLKN * RS, WIN = (32 * NW + BLKN) * 4;
+    constexpr int BUF = 2 * IMG + 2 * BLKN * 4 + (BIAS == LINE ? WIN : BIAS == NONE ? 0 : BLKN * 4);
+    extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][Q image | dO image | lse | delta | window or places], BOX: the table
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int hk = blockIdx.y, b = blockIdx.z, rep = p.H / p.Hkv;
+    const int k0 = blockIdx.x * NW * 32, key = k0 + wv * 32 + (lane & 31), keyc = min(key, p.Nk - 1);
+    const bool kok = key < p.Nk && (!p.mask || p.mask[(long)b * p.Nk + keyc]);
+    const int nqb = (p.Nq + BLKN - 1) / BLKN, steps = nqb * rep;
+
+    u32x4 kf[NCH], vf[NCH];
+    {
+        const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + (long)b * p.ks[0] + (long)keyc * p.ks[1] + (long)hk * p.ks[2]);
+        const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + (long)b * p.vs[0] + (long)keyc * p.vs[1] + (long)hk * p.vs[2]);
+#pragma unroll
+        for (int s = 0; s < NCH; ++s) {
+            kf[s] = vf[s] = (u32x4){0u, 0u, 0u, 0u};
+            if (kok && 32 * s + 16 * h < p.D * (int)sizeof(T)) {
+                kf[s] = *reinterpret_cast<const u32x4*>(kp + 32 * s + 16 * h);
+                vf[s] = *reinterpret_cast<const u32x4*>(vp + 32 * s + 16 * h);
+            }
+        }
+    }
+    const int ak = (BIAS == BOX || BIAS == GATHER) ? p.omax - place(p, keyc) : 0;
+    float* tab = reinterpret_cast<float*>(lds + 2 * BUF);
+    const bool any = __syncthreads_or(kok);                             // a workgroup whose keys are all masked has only zeros to store
+
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
+
+    Tile<T, DP, NT> qt_, dt_;
+    float lr = 0.f, tr = 0.f;
+    int qpos = 0;
+    constexpr int NWIN = (32 * NW + BLKN + NT - 1) / NT;
+    float win[BIAS == LINE ? NWIN : 1];
+    auto fetch = [&](int it) {
+        const int head = hk * rep + it / nqb, q0 = (it % nqb) * BLKN;
+        qt_.fetch(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)head * p.qs[2], p.qs[1], q0, p.Nq, p.D, tid);
+        dt_.fetch(static_cast<const T*>(p.dout) + ((long)b * p.Nq * p.H + head) * p.D, (long)p.H * p.D, q0, p.Nq, p.D, tid);
+        if (tid < BLKN) {
+            const bool ok = q0 + tid < p.Nq;
+            const long lrow = ((long)b * p.H + head) * p.Nq + q0 + tid;
+            lr = ok ? p.lse[lrow] : INFINITY;                           // queries past the end: p = 0
+            tr = ok ? p.delta[lrow] : 0.f;
+            if (BIAS == BOX || BIAS == GATHER) qpos = place(p, p.q0 + min(q0 + tid, p.Nq - 1));
+        }
+        if (BIAS == LINE) {
+            const int first = p.q0 + q0 - (k0 + 32 * NW - 1) + p.gw - 1;
+#pragma unroll
+            for (int i = 0; i < NWIN; ++i) {
+                const int at = first + i * NT + tid;
+                win[i] = (i * NT + tid < 32 * NW + BLKN && at >= 0 && at < p.nd) ? p.e[(long)head * p.nd + at] : 0.f;
+            }
+        }
+    };
+    auto commit = [&](char* buf) {
+        qt_.commit(buf, RS, tid, ~0ull);
+        dt_.commit(buf + IMG, RS, tid, ~0ull);
+        float* side = reinterpret_cast<float*>(buf + 2 * IMG);
+        if (tid < BLKN) {
+            side[tid] = lr;
+            side[BLKN + tid] = tr;
+            if (BIAS == BOX || BIAS == GATHER) reinterpret_cast<int*>(side)[2 * BLKN + tid] = qpos;
+        }
+        if (BIAS == LINE) {
+#pragma unroll
+            for (int i = 0; i < NWIN; ++i)
+                if (i * NT + tid < 32 * NW + BLKN) side[2 * BLKN + i * NT + tid] = win[i];
+        }
+    };
+    if (any) {
+        fetch(0);
+        commit(lds);
+        for (int it = 0; it < steps; ++it) {
+            const int head = hk * rep + it / nqb;
+            if (BIAS == BOX && it % nqb == 0)                              // the next head's table (the last step ended on a barrier)
+                for (int i = tid; i < p.nd; i += NT) tab[i] = p.e[(long)head * p.nd + i];
+            if (it == 0 || (BIAS == BOX && it % nqb == 0)) __syncthreads();
+            const char* qimg = lds + (it & 1) * BUF;
+            const char* dimg = qimg + IMG;
+            const float* lsev = reinterpret_cast<const float*>(qimg + 2 * IMG);
+            const float* dltv = lsev + BLKN;
+            const float* wl = lsev + 2 * BLKN + (32 * NW - 1 - (wv * 32 + (lane & 31)) + 4 * h);
+            if (it + 1 < steps) fetch(it + 1);
+#pragma unroll
+            for (int qt = 0; qt < KT; ++qt) {
+                f32x16 sa = zero16(), da = zero16();
+#pragma unroll
+                for (int s = 0; s < NCH; ++s) {
+                    sa = dot<T>(row_frag<T>(qimg, RS, qt * 32, s, lane), kf[s], sa);
+                    da = dot<T>(row_frag<T>(dimg, RS, qt * 32, s, lane), vf[s], da);
+                }
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int r0 = qt * 32 + 8 * g4 + 4 * h;
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(lsev + r0), d4 = *reinterpret_cast<const f32x4*>(dltv + r0);
+                    int4 qp;
+                    if (BIAS == BOX || BIAS == GATHER) qp = *reinterpret_cast<const int4*>(lsev + 2 * BLKN + r0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 4 * g4 + j;
+                        float x;
+                        if (BIAS == NONE) x = sa[r] * p.c;
+                        else {
+                            const int o_ = ak + (j == 0 ? qp.x : j == 1 ? qp.y : j == 2 ? qp.z : qp.w);
+                            const float bias = BIAS == LINE ? wl[qt * 32 + 8 * g4 + j] : BIAS == BOX ? tab[o_] : gather_bias(p, head, o_);
+                            x = __builtin_fmaf(sa[r], p.c, bias);
+                        }
+                        const float pr = __builtin_amdgcn_exp2f(x - l4[j]);
+                        sa[r] = pr * (da[r] - d4[j]);                   // dS
+                        da[r] = pr;                                     // P   (a lane's columns are its own key's: a masked key's are not stored)
+                    }
+                }
+                tr_product<T, ND>(dimg, RS, qt * 32, da, dv, lane);
+                tr_product<T, ND>(qimg, RS, qt * 32, sa, dk, lane);
+            }
+            if (it + 1 < steps) commit(lds + ((it + 1) & 1) * BUF);
+            __syncthreads();
+        }
+    }
+    if (key < p.Nk) {
+        const long at = (((long)b * p.Nk + key) * p.Hkv + hk) * p.D;
+        const float f = kok ? p.scale : 0.f, g = kok ? 1.f : 0.f;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const int d = dt * 32 + 8 * g4 + 4 * h;
+                if (d >= p.D) continue;
+                f32x4 a = {0.f, 0.f, 0.f, 0.f}, c = a;
+                if (kok) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { a[j] = dk[dt][4 * g4 + j] * f; c[j] = dv[dt][4 * g4 + j] * g; }
+                }
+                store4(static_cast<T*>(p.dk) + at + d, a);
+                store4(static_cast<T*>(p.dv) + at + d, c);
+            }
+    }
+}
+
+template <typename K> int grant_lds(K kern, int bytes) {
+    if (bytes > 64 * 1024) HIP_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return 0;
+}
+
+template <typename T, int DP, int NW, int MODE, int BIAS>
+int launch_q(const RelP& p, hipStream_t st) {
+    constexpr int BLKN = blk<T>(), RS = row_stride<T, DP>(), VS = MODE == 0 ? tr_stride<T, DP>() : RS;
+    int bytes = 2 * (BLKN * (RS + VS) + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
+    if (BIAS == BOX) bytes += p.nd * 4 * (MODE == 1 && p.slab ? 1 + NW : 1);
+    if (BIAS == LINE && MODE == 1) bytes += NW * (BLKN + 32) * 4;
+    const int rc = grant_lds(rel_q_kernel<T, DP, NW, MODE, BIAS>, bytes);
+    if (rc) return rc;
+    const int rows = p.pack ? p.Nq * (p.H / p.Hkv) : p.Nq;
+    hipLaunchKernelGGL((rel_q_kernel<T, DP, NW, MODE, BIAS>), dim3((rows + 32 * NW - 1) / (32 * NW) * p.nsplit, p.pack ? p.Hkv : p.H, p.B), dim3(64 * NW), bytes, st, p);
+    LAUNCH_RET();
+    return 0;
+}
+template <typename T, int DP, int NW, int BIAS>
+int launch_k(const RelP& p, hipStream_t st) {
+    constexpr int BLKN = blk<T>(), RS = row_stride<T, DP>();
+    int bytes = 2 * (2 * BLKN * RS + 2 * BLKN * 4 + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
+    if (BIAS == BOX) bytes += p.nd * 4;
+    const int rc = grant_lds(rel_k_kernel<T, DP, NW, BIAS>, bytes);
+    if (rc) return rc;
+    hipLaunchKernelGGL((rel_k_kernel<T, DP, NW, BIAS>), dim3((p.Nk + 32 * NW - 1) / (32 * NW), p.Hkv, p.B), dim3(64 * NW), bytes, st, p);
+    LAUNCH_RET();
+    return 0;
+}
+
+template <typename T, int DP, int NW>
+int pick_bias(const RelP& p, int what, hipStream_t st) {
+#define REL_ONE(BIAS) (what == 0 ? launch_q<T, DP, NW, 0, BIAS>(p, st) : what == 1 ? launch_q<T, DP, NW, 1, BIAS>(p, st) : launch_k<T, DP, NW, BIAS>(p, st))
+    switch (p.bias) {
+        case NONE: return REL_ONE(NONE);
+        case BOX: return REL_ONE(BOX);
+        case LINE: return REL_ONE(LINE);
+        default: return REL_ONE(GATHER);
+    }
+#undef REL_ONE
+}
+template <typename T, int DP>
+int pick_nw(const RelP& p, int what, int nw, hipStream_t st) { return nw == 4 ? pick_bias<T, DP, 4>(p, what, st) : pick_bias<T, DP, 1>(p, what, st); }
+
+}  // namespace

@@ -5,7 +5,8 @@ torch is used for memory, streams and autograd bookkeeping only -- every op belo
 hand-written HIP kernel, and raises if the library or a GPU tensor is missing.
 """
 import contextlib
-from ctypes import byref, c_void_p
+import math
+from ctypes import byref, c_int64, c_void_p
 
 import os
 
@@ -1886,6 +1887,159 @@ def topk_distill(logits, values, index, temp=1.0):
     if torch.is_grad_enabled() and s.requires_grad:
         return TopkDistillFn.apply(s, tv, ti, temp).reshape(lead)
     return _topk_distill_fwd(s, tv, ti, temp, False)[0].reshape(lead)
+
+
+# ------------------------------------------------------------------------------------------------
+# attention with a learned relative position bias
+# ------------------------------------------------------------------------------------------------
+def _grid3(grid):
+    g = (grid,) if isinstance(grid, int) else tuple(int(n) for n in grid)
+    if not 1 <= len(g) <= 3 or any(n < 1 for n in g):
+        raise ValueError(f"token grid {grid}: one to three positive sizes")
+    return (1,) * (3 - len(g)) + g
+
+
+def relative_buckets(grid, num_buckets, max_distance=128, device=None):
+    """bucket of every offset of a token grid, for rel_attention: per axis num_buckets two-sided buckets, a quarter of them exact on either side and the rest
+    spaced by the logarithm up to max_distance; axes of size 1 have one bucket, several axes their product.
+    -> (int32 tensor of the grid's offsets, number of buckets)"""
+    if num_buckets < 2 or num_buckets % 2 or max_distance < 1:
+        raise ValueError(f"relative_buckets: {num_buckets} buckets up to {max_distance}")
+    total, out = 1, torch.zeros((), dtype=torch.float64)
+    for n in _grid3(grid):
+        if n == 1:
+            out = out.unsqueeze(-1)
+            continue
+        off = torch.arange(1 - n, n, dtype=torch.float64)
+        half, exact = num_buckets // 2, max(1, num_buckets // 4)
+        a = off.abs()
+        far = exact + (torch.log(a.clamp(min=1) / exact) / math.log(max(max_distance, exact + 1) / exact) * (half - exact)).floor()
+        b = torch.where(a < exact, a, far.clamp(max=half - 1)) + half * (off > 0)
+        out = out.unsqueeze(-1) * num_buckets + b
+        total *= num_buckets
+    return out.reshape(-1).to(torch.int32).to(device), total
+
+
+def _rel_view(t):
+    """t as the kernels read it: dense last dimension, rows on 16-byte points; a copy where it is not"""
+    unit = 16 // t.element_size()
+    if t.stride(3) != 1 or any(s % unit for s in t.stride()[:3]) or t.data_ptr() % 16 or t.shape[3] % unit:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _rel_args(q, k, v, table, buckets, mask, meta):
+    grid, q_start, scale, nb = meta
+    st = [(c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
+    return (_p(q), st[0], _p(k), st[1], _p(v), st[2], L.dtype_code(q.dtype), q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], *grid, q_start,
+            _p(table), L.dtype_code(table.dtype) if table is not None else 0, _p(buckets), nb, _p(mask), scale)
+
+
+def _rel_workspace(q, k, table, buckets, meta, backward):
+    grid, q_start, _, nb = meta
+    n = L.load().passion_rel_attn_workspace_floats(L.dtype_code(q.dtype), backward, q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], *grid, q_start,
+                                                   int(table is not None), int(buckets is not None), nb)
+    if n < 0:
+        raise L.PassionHipError(f"passion_rel_attn_workspace_floats failed with code {n}")
+    return torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+
+
+def _rel_attention_fwd(q, k, v, table, buckets, mask, meta, keep):
+    B, Nq, H, D = q.shape
+    out = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device) if keep else None
+    if out.numel() == 0 or k.shape[1] == 0:
+        return out.zero_(), lse
+    with _here(q, k, v, table, buckets, mask):
+        ws = _rel_workspace(q, k, table, buckets, meta, 0)
+        L.check(L.load().passion_rel_attn_fwd(*_rel_args(q, k, v, table, buckets, mask, meta), _p(out), _p(lse), _p(ws), L.stream_ptr()), "passion_rel_attn_fwd")
+    return out, lse
+
+
+class RelAttentionFn(torch.autograd.Function):
+    """csrc/rel_attn.hip: forward keeps the row log-sum-exp, backward recomputes the probabilities"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, mask, meta):
+        out, lse = _rel_attention_fwd(q, k, v, table, buckets, mask, meta, True)
+        ctx.save_for_backward(q, k, v, table, buckets, mask, out, lse)
+        ctx.meta = meta
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, buckets, mask, out, lse = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dtable = torch.empty_like(table) if table is not None and ctx.needs_input_grad[3] else None
+        if out.numel() == 0 or k.shape[1] == 0:
+            return (*(t.zero_() if t is not None else None for t in (dq, dk, dv, dtable)), None, None, None)
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        with _here(q, dout):
+            ws = _rel_workspace(q, k, table, buckets, ctx.meta, 1)
+            L.check(L.load().passion_rel_attn_bwd(*_rel_args(q, k, v, table, buckets, mask, ctx.meta), _p(out), _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(dtable),
+                                                  _p(ws), L.stream_ptr()), "passion_rel_attn_bwd")
+        return dq, dk, dv, dtable, None, None, None
+
+
+def rel_attention(q, k, v, table=None, grid=None, buckets=None, key_mask=None, scale=None, q_start=0):
+    """softmax(scale q k^T + bias) v with a learned bias by relative position (attention() is the form without positions).
+    q (B, Nq, H, D); k, v (B, Nk, Hkv, D), Hkv a divisor of H (query head h reads key / value head h // (H // Hkv)); f32 or bf16, D a multiple of 8 up to 128; any strides
+    (views whose rows are dense and 16-byte aligned are read in place, others copied).
+    table (buckets, H) f32 / bf16: learned, receives its gradient (summed in f32; with bf16 q, k, v to the accuracy of their products).  grid: the token raster (one to three
+    sizes); token t lies at cell t mod prod(grid), so several modalities over the same cells share their positions; query i is token q_start + i.  buckets: int32 / int64,
+    bucket of each of the prod(2 n - 1) offsets (see relative_buckets), None: one table row per offset, in raster order of (query cell - key cell).  A bucket outside the table has no bias, an entry
+    at or below -1e30 excludes its pairs.  key_mask (B, Nk) bool / uint8: False = the key does not take part, whatever its k and v hold.  A query without a key gives 0 and zero gradients.
+    scale: default D ** -0.5.  One query against many keys (a new token) runs split over the keys.  -> (B, Nq, H, D)."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"rel_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
+    B, Nq, H, D = q.shape
+    Nk, Hkv = k.shape[1:3]
+    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"rel_attention: dtypes {q.dtype}, {k.dtype}, {v.dtype}")
+    if D < 8 or D > 128 or D % 8:
+        raise ValueError(f"rel_attention: head width {D} (a multiple of 8 up to 128)")
+    if H < 1 or Hkv < 1 or H % Hkv or H > 65535 or B > 65535 or max(Nq, Nk) > 2 ** 30:
+        raise ValueError(f"rel_attention: {B} x {H} heads on {Hkv} key / value heads, {Nq} x {Nk} tokens")
+    q_start = int(q_start)
+    if not 0 <= q_start <= 2 ** 30:
+        raise ValueError(f"rel_attention: q_start {q_start}")
+    g, nb = (1, 1, 1), 0
+    if table is not None:
+        if grid is None:
+            raise ValueError("rel_attention: a table needs the token grid")
+        g = _grid3(grid)
+        offsets = math.prod(2 * n - 1 for n in g)
+        if offsets > 2 ** 30:
+            raise ValueError(f"rel_attention: grid {g} has {offsets} offsets")
+        if table.dim() != 2 or table.shape[1] != H or table.shape[0] < 1 or table.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"rel_attention: table {tuple(table.shape)} {table.dtype} for {H} heads")
+        if buckets is None:
+            if table.shape[0] != offsets:
+                raise ValueError(f"rel_attention: table of {table.shape[0]} rows without buckets, grid {g} has {offsets} offsets")
+        elif tuple(buckets.shape) != (offsets,) or buckets.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"rel_attention: buckets {tuple(buckets.shape)} {buckets.dtype}, grid {g} has {offsets} offsets")
+        table = table.contiguous()
+        nb = table.shape[0]
+        if buckets is not None:
+            buckets = buckets.contiguous() if buckets.dtype == torch.int32 else buckets.clamp(-1, 2 ** 31 - 1).int()
+    elif buckets is not None:
+        raise ValueError("rel_attention: buckets without a table")
+    if key_mask is not None:
+        if tuple(key_mask.shape) != (B, Nk) or key_mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"rel_attention: key_mask {tuple(key_mask.shape)} {key_mask.dtype}")
+        key_mask = key_mask.contiguous()
+    scale = float(D ** -0.5 if scale is None else scale)
+    L.require_gpu(q, k, v, table, buckets, key_mask)
+    q, k, v = _rel_view(q), _rel_view(k), _rel_view(v)
+    meta = (g, q_start, scale, nb)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
+        return RelAttentionFn.apply(q, k, v, table, buckets, key_mask, meta)
+    return _rel_attention_fwd(q, k, v, table, buckets, key_mask, meta, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------
