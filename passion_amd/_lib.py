@@ -227,18 +227,14 @@ def check(rc, what):
 
 HOST_EXT_PATH = os.path.join(_HERE, "lib", "_passion_host.so")
 _host = None
+_host_mod = None
 
 
-def host():
-    """The C++ host extension (csrc/host_ext.cpp: autograd nodes of the conv block and the InstanceNorm statistics), bound
-    to the entry points of the library load() returned.  PASSION_HOST_EXT=0 selects the Python autograd.Functions in ops.py
-    instead (same C ABI underneath; kept for A/B timing of the host path)."""
-    global _host
-    if _host is not None:
-        return _host or None
-    if os.environ.get("PASSION_HOST_EXT", "1") == "0":
-        _host = False
-        return None
+def _host_module():
+    """the built C++ host extension, bound to the entry points of the library load() returned (once)"""
+    global _host_mod
+    if _host_mod is not None:
+        return _host_mod
     lib = load()
     if not os.path.exists(HOST_EXT_PATH):
         raise PassionHipError(f"{HOST_EXT_PATH} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
@@ -253,8 +249,30 @@ def host():
     mod.bind(addr("passion_conv3d_fwd"), addr("passion_conv3d_bwd"), addr("passion_conv_bwd_scratch_floats"),
              addr("passion_instnorm_stats"), addr("passion_instnorm_scratch_doubles"), addr("passion_conv3d_fwd_stats"),
              addr("passion_conv3d_fwd_grouped"), addr("passion_conv3d_bwd_grouped"))
-    _host = mod
+    mod.bind_token_ops([addr(n) for n in ("passion_rel_attn_workspace_floats", "passion_rel_attn_fwd", "passion_rel_attn_bwd",
+                                          "passion_residual_norm_part_floats", "passion_residual_norm_fwd", "passion_residual_norm_bwd",
+                                          "passion_topk_distill_fwd", "passion_topk_distill_bwd")])
+    _host_mod = mod
     return mod
+
+
+def host():
+    """The C++ host extension (csrc/host_ext.cpp: autograd nodes of the conv block and the InstanceNorm statistics), bound
+    to the entry points of the library load() returned.  PASSION_HOST_EXT=0 selects the Python autograd.Functions in ops.py
+    instead (same C ABI underneath; kept for A/B timing of the host path)."""
+    global _host
+    if _host is not None:
+        return _host or None
+    if os.environ.get("PASSION_HOST_EXT", "1") == "0":
+        _host = False
+        return None
+    _host = _host_module()
+    return _host
+
+
+def token_ops():
+    """the autograd nodes of the token operators (csrc/host_token_ops.cpp); they have no Python form"""
+    return _host_mod if _host_mod is not None else _host_module()
 
 
 def dtype_code(t):

@@ -4,15 +4,13 @@ Internal activation layout is channels-last 5-D: (B, D, H, W, C) contiguous, f32
 torch is used for memory, streams and autograd bookkeeping only -- every op below runs a
 hand-written HIP kernel, and raises if the library or a GPU tensor is missing.
 """
-import contextlib
 import math
-from ctypes import byref, c_int64, c_void_p
+from ctypes import byref, c_void_p
 
 import os
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -1707,15 +1705,21 @@ def region_mix(prob, mask, w, ys):
 # ------------------------------------------------------------------------------------------------
 # the residual step between two transformer blocks, distillation from a teacher's top logits
 # ------------------------------------------------------------------------------------------------
-def _here(*tensors):
-    """all on one GPU, which is made the current one for the launch (a context manager)"""
-    ts = [t for t in tensors if t is not None]
-    L.require_gpu(*ts)
-    dev = ts[0].device
-    for t in ts[1:]:
-        if t.device != dev:
+def _one_device(*tensors):
+    """all that are there on one GPU"""
+    L.require_gpu(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
             raise ValueError(f"tensors on {dev} and {t.device} in one call")
-    return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _dense(t):
+    """contiguous and on a 16-byte point, as the kernels read whole tensors"""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _norm_spec(m, C, dtype, what):
@@ -1728,59 +1732,6 @@ def _norm_spec(m, C, dtype, what):
     eps = m.eps if m.eps is not None else torch.finfo(dtype).eps       # nn.RMSNorm's own default
     f32 = lambda p: p if p is None or p.dtype == torch.float32 else p.float()
     return kind, f32(m.weight), f32(m.bias) if kind == 1 else None, float(eps)
-
-
-def _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, meta, keep):
-    post, pre, eps1, eps2, gmode, B, N = meta
-    C = x.shape[-1]
-    r = torch.empty_like(x)
-    y = torch.empty_like(h) if pre else None
-    stat = torch.empty(B * N, 4, dtype=torch.float32, device=x.device) if keep else None
-    if x.numel():
-        with _here(x, h, gate, scale, w1, b1, w2, b2):
-            L.check(L.load().passion_residual_norm_fwd(_p(x), L.dtype_code(x.dtype), _p(h), L.dtype_code(h.dtype), _p(w1), _p(b1), post, eps1, _p(gate), gmode,
-                                                       L.dtype_code(gate.dtype) if gmode else 0, _p(scale), _p(w2), _p(b2), pre, eps2, B, N, C, _p(r),
-                                                       _p(y), _p(stat), L.stream_ptr()), "passion_residual_norm_fwd")
-    return r, y, stat
-
-
-class ResidualNormFn(torch.autograd.Function):
-    """csrc/residual_norm.hip: forward keeps the four row moments, backward forms r again from x and h"""
-
-    @staticmethod
-    def forward(ctx, x, h, gate, scale, w1, b1, w2, b2, meta):
-        r, y, stat = _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, meta, True)
-        ctx.save_for_backward(x, h, gate, scale, w1, b1, w2, stat)
-        ctx.meta, ctx.has_b2 = meta, b2 is not None
-        ctx.set_materialize_grads(False)
-        return (r, y) if meta[1] else r
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dr, dy=None):
-        x, h, gate, scale, w1, b1, w2, stat = ctx.saved_tensors
-        post, pre, _, _, gmode, B, N = ctx.meta
-        C, dev, need = x.shape[-1], x.device, ctx.needs_input_grad
-        if dr is None and dy is None:
-            return (None,) * 9
-        dr, dy = (t.to(like.dtype).contiguous() if t is not None else None for t, like in ((dr, x), (dy, h)))
-        dx, dh = torch.empty_like(x), torch.empty_like(h)
-        dgate = torch.empty_like(gate) if gmode and need[2] else None
-        # [scale, w1, b1, w2, b2], those that are there and wanted
-        there = (scale is not None, w1 is not None, b1 is not None, w2 is not None, ctx.has_b2)
-        want = [t and n for t, n in zip(there, need[3:8])]
-        if not x.numel():
-            cols = [torch.zeros(C, dtype=torch.float32, device=dev) if w else None for w in want]
-            return (dx, dh, dgate.zero_() if dgate is not None else None, *cols, None)
-        lib = L.load()
-        cols = [torch.empty(C, dtype=torch.float32, device=dev) if w else None for w in want]
-        with _here(x, h, gate, dr, dy):
-            part = torch.empty(lib.passion_residual_norm_part_floats(B, N, C), dtype=torch.float32, device=dev)
-            L.check(lib.passion_residual_norm_bwd(_p(x), L.dtype_code(x.dtype), _p(h), L.dtype_code(h.dtype), _p(w1), _p(b1), post, _p(gate), gmode,
-                                                  L.dtype_code(gate.dtype) if gmode else 0, _p(scale), _p(w2), pre, _p(stat), _p(dr), _p(dy), B, N, C,
-                                                  _p(dx), _p(dh), _p(dgate), _p(cols[1]), _p(cols[2]), _p(cols[3]), _p(cols[4]), _p(cols[0]), _p(part),
-                                                  L.stream_ptr()), "passion_residual_norm_bwd")
-        return (dx, dh, dgate, *cols, None)
 
 
 def residual_norm(x, h, post=None, pre=None, gate=None, scale=None):
@@ -1814,50 +1765,10 @@ def residual_norm(x, h, post=None, pre=None, gate=None, scale=None):
         raise ValueError(f"residual_norm: {B} samples of {N} rows")
     if scale is not None and scale.dtype != torch.float32:
         scale = scale.float()
-    ins = [t.contiguous() if t is not None else None for t in (x, h, gate, scale, w1, b1, w2, b2)]
-    L.require_gpu(*ins)
-    meta = (post, pre, eps1, eps2, gmode, B, N)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins):
-        return ResidualNormFn.apply(*ins, meta)
-    r, y, _ = _residual_norm_fwd(*ins, meta, False)
-    return (r, y) if pre else r
-
-
-def _topk_distill_fwd(logits, values, index, temp, keep):
-    R, V = logits.shape
-    loss = torch.empty(R, dtype=torch.float32, device=logits.device)
-    lse = torch.empty(R, dtype=torch.float32, device=logits.device) if keep else None
-    if R:
-        with _here(logits, values, index):
-            L.check(L.load().passion_topk_distill_fwd(_p(logits), L.dtype_code(logits.dtype), _p(values), L.dtype_code(values.dtype), _p(index),
-                                                      int(index.dtype == torch.int64), R, V, index.shape[1], temp, _p(loss), _p(lse), L.stream_ptr()),
-                    "passion_topk_distill_fwd")
-    return loss, lse
-
-
-class TopkDistillFn(torch.autograd.Function):
-    """csrc/distill.hip: forward keeps one log-sum-exp a row, backward reads the logits once more"""
-
-    @staticmethod
-    def forward(ctx, logits, values, index, temp):
-        loss, lse = _topk_distill_fwd(logits, values, index, temp, True)
-        ctx.save_for_backward(logits, values, index, lse)
-        ctx.temp = temp
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, values, index, lse = ctx.saved_tensors
-        R, V = logits.shape
-        d = torch.empty_like(logits)
-        if R:
-            g = g.float().contiguous()
-            with _here(logits, g):
-                L.check(L.load().passion_topk_distill_bwd(_p(logits), L.dtype_code(logits.dtype), _p(values), L.dtype_code(values.dtype), _p(index),
-                                                          int(index.dtype == torch.int64), R, V, index.shape[1], ctx.temp, _p(lse), _p(g), _p(d),
-                                                          L.stream_ptr()), "passion_topk_distill_bwd")
-        return d, None, None, None
+    ins = [_dense(t) for t in (x, h, gate, scale, w1, b1, w2, b2)]
+    _one_device(*ins)
+    out = L.token_ops().residual_norm(*ins, [post, pre, gmode, B, N], [eps1, eps2])
+    return (out[0], out[1]) if pre else out[0]
 
 
 def topk_distill(logits, values, index, temp=1.0):
@@ -1879,14 +1790,10 @@ def topk_distill(logits, values, index, temp=1.0):
     if not 0.0 < temp < float("inf"):
         raise ValueError(f"topk_distill: temperature {temp}")
     lead = logits.shape[:-1]
-    s = logits.reshape(-1, V).contiguous()
-    if s.data_ptr() % 16:
-        s = s.clone()
+    s = _dense(logits.reshape(-1, V))
     tv, ti = values.detach().reshape(-1, K).contiguous(), index.reshape(-1, K).contiguous()
-    L.require_gpu(s, tv, ti)
-    if torch.is_grad_enabled() and s.requires_grad:
-        return TopkDistillFn.apply(s, tv, ti, temp).reshape(lead)
-    return _topk_distill_fwd(s, tv, ti, temp, False)[0].reshape(lead)
+    _one_device(s, tv, ti)
+    return L.token_ops().topk_distill(s, tv, ti, temp).reshape(lead)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -1922,68 +1829,10 @@ def relative_buckets(grid, num_buckets, max_distance=128, device=None):
 
 def _rel_view(t):
     """t as the kernels read it: dense last dimension, rows on 16-byte points; a copy where it is not"""
-    unit = 16 // t.element_size()
-    if t.stride(3) != 1 or any(s % unit for s in t.stride()[:3]) or t.data_ptr() % 16 or t.shape[3] % unit:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+    a, b, c, d = t.stride()
+    if d != 1 or (a | b | c) % (16 // t.element_size()) or t.data_ptr() % 16:
+        return _dense(t)
     return t
-
-
-def _rel_args(q, k, v, table, buckets, mask, meta):
-    grid, q_start, scale, nb = meta
-    st = [(c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
-    return (_p(q), st[0], _p(k), st[1], _p(v), st[2], L.dtype_code(q.dtype), q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], *grid, q_start,
-            _p(table), L.dtype_code(table.dtype) if table is not None else 0, _p(buckets), nb, _p(mask), scale)
-
-
-def _rel_workspace(q, k, table, buckets, meta, backward):
-    grid, q_start, _, nb = meta
-    n = L.load().passion_rel_attn_workspace_floats(L.dtype_code(q.dtype), backward, q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], *grid, q_start,
-                                                   int(table is not None), int(buckets is not None), nb)
-    if n < 0:
-        raise L.PassionHipError(f"passion_rel_attn_workspace_floats failed with code {n}")
-    return torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-
-
-def _rel_attention_fwd(q, k, v, table, buckets, mask, meta, keep):
-    B, Nq, H, D = q.shape
-    out = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device) if keep else None
-    if out.numel() == 0 or k.shape[1] == 0:
-        return out.zero_(), lse
-    with _here(q, k, v, table, buckets, mask):
-        ws = _rel_workspace(q, k, table, buckets, meta, 0)
-        L.check(L.load().passion_rel_attn_fwd(*_rel_args(q, k, v, table, buckets, mask, meta), _p(out), _p(lse), _p(ws), L.stream_ptr()), "passion_rel_attn_fwd")
-    return out, lse
-
-
-class RelAttentionFn(torch.autograd.Function):
-    """csrc/rel_attn.hip: forward keeps the row log-sum-exp, backward recomputes the probabilities"""
-
-    @staticmethod
-    def forward(ctx, q, k, v, table, buckets, mask, meta):
-        out, lse = _rel_attention_fwd(q, k, v, table, buckets, mask, meta, True)
-        ctx.save_for_backward(q, k, v, table, buckets, mask, out, lse)
-        ctx.meta = meta
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, table, buckets, mask, out, lse = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dtable = torch.empty_like(table) if table is not None and ctx.needs_input_grad[3] else None
-        if out.numel() == 0 or k.shape[1] == 0:
-            return (*(t.zero_() if t is not None else None for t in (dq, dk, dv, dtable)), None, None, None)
-        dout = dout.contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
-        with _here(q, dout):
-            ws = _rel_workspace(q, k, table, buckets, ctx.meta, 1)
-            L.check(L.load().passion_rel_attn_bwd(*_rel_args(q, k, v, table, buckets, mask, ctx.meta), _p(out), _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(dtable),
-                                                  _p(ws), L.stream_ptr()), "passion_rel_attn_bwd")
-        return dq, dk, dv, dtable, None, None, None
 
 
 def rel_attention(q, k, v, table=None, grid=None, buckets=None, key_mask=None, scale=None, q_start=0):
@@ -2034,12 +1883,8 @@ def rel_attention(q, k, v, table=None, grid=None, buckets=None, key_mask=None, s
             raise ValueError(f"rel_attention: key_mask {tuple(key_mask.shape)} {key_mask.dtype}")
         key_mask = key_mask.contiguous()
     scale = float(D ** -0.5 if scale is None else scale)
-    L.require_gpu(q, k, v, table, buckets, key_mask)
-    q, k, v = _rel_view(q), _rel_view(k), _rel_view(v)
-    meta = (g, q_start, scale, nb)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
-        return RelAttentionFn.apply(q, k, v, table, buckets, key_mask, meta)
-    return _rel_attention_fwd(q, k, v, table, buckets, key_mask, meta, False)[0]
+    _one_device(q, k, v, table, buckets, key_mask)
+    return L.token_ops().rel_attention(_rel_view(q), _rel_view(k), _rel_view(v), table, buckets, key_mask, [*g, q_start, nb], scale)
 
 
 # ------------------------------------------------------------------------------------------------
