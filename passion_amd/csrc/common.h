@@ -86,6 +86,28 @@ __device__ __forceinline__ float group16_sum(float v) {
     return v;
 }
 
+// Sum over aligned groups of w lanes (a power of two up to 64, uniform), valid in every lane, without the LDS pipe: quads by DPP, 8 and 16 by the mirrors
+// of a half row and a row (every lane of the mirrored part holds the same sum), rows by v_permlane16_swap / v_permlane32_swap.
+__device__ __forceinline__ float lanes_sum(float v, int w) {
+#define LANES_DPP(ctrl) v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), ctrl, 0xf, 0xf, false))
+    if (w > 1) LANES_DPP(0xB1);            // quad_perm [1, 0, 3, 2]
+    if (w > 2) LANES_DPP(0x4E);            // quad_perm [2, 3, 0, 1]
+    if (w > 4) LANES_DPP(0x141);           // row_half_mirror
+    if (w > 8) LANES_DPP(0x140);           // row_mirror
+#undef LANES_DPP
+    if (w > 16) {
+        const unsigned u = __float_as_uint(v);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (w > 32) {
+        const unsigned u = __float_as_uint(v);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
 // Hand-over of a few words between workgroups of one kernel (per-workgroup partial sums -> the workgroup that arrives last):
 // RELAXED ATOMIC stores / loads at agent scope (sc1: coherent across the XCDs' L2s) + a ticket counter, ordered by the
 // s_waitcnt of __syncthreads().  NOT __threadfence(): an agent-scope release fence writes back every dirty line of the XCD's L2

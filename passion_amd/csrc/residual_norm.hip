@@ -34,305 +34,394 @@ struct RnP {
     int gmode, gdt;                           // gate: 0 none, 1 per sample, 2 per token; its dtype
     float eps1, eps2;
     int chunk;                                // rows of one sample per workgroup
+    int wanted;                               // backward: bit i: slot i of part is folded afterwards
 };
 
-// channel j of thread t of a row: 8 t + j where rows are 16-byte aligned (VEC), else j TPR + t (neighbouring threads, neighbouring channels)
-template <bool VEC> __device__ __forceinline__ int chan(int t, int j, int tpr) { return VEC ? 8 * t + j : j * tpr + t; }
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
+__device__ __forceinline__ f32x8 all8(float v) { return (f32x8){v, v, v, v, v, v, v, v}; }
+
+// the 8 channels of thread t of a row: 8 t .. 8 t + 7 where rows are 16-byte aligned (VEC), else j TPR + t (neighbouring threads, neighbouring channels);
+// channels past C are 0
 template <typename T, bool VEC>
-__device__ __forceinline__ void ldv(const T* p, int t, int tpr, int C, float (&v)[VPT]) {
+__device__ __forceinline__ f32x8 ldv(const T* p, int t, int tpr, int C) {
+    f32x8 v = all8(0.f);
     if constexpr (VEC) {
         if (8 * t < C) {
-            if constexpr (sizeof(T) == 2) VecIO<bf16_t, 8>::load(reinterpret_cast<const bf16_t*>(p) + 8 * t, v);
-            else {
-                const f32x4 a = load4(reinterpret_cast<const float*>(p) + 8 * t), b = load4(reinterpret_cast<const float*>(p) + 8 * t + 4);
+            if constexpr (sizeof(T) == 2) {
+                const uint4 u = *reinterpret_cast<const uint4*>(p + 8 * t);
+                v = (f32x8){__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u),
+                            __uint_as_float(u.z << 16), __uint_as_float(u.z & 0xffff0000u), __uint_as_float(u.w << 16), __uint_as_float(u.w & 0xffff0000u)};
+            } else {
+                const f32x4 a = load4(p + 8 * t), b = load4(p + 8 * t + 4);
+                v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        }
+    } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+        for (int j = 0; j < VPT; ++j)
+            if (j * tpr + t < C) v[j] = to_f32(p[j * tpr + t]);
+    }
+    return v;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void stv(T* p, int t, int tpr, int C, f32x8 v) {
+    if constexpr (VEC) {
+        if (8 * t < C) {
+            store4(p + 8 * t, __builtin_shufflevector(v, v, 0, 1, 2, 3));
+            store4(p + 8 * t + 4, __builtin_shufflevector(v, v, 4, 5, 6, 7));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if (j * tpr + t < C) p[j * tpr + t] = from_f32<T>(v[j]);
+    }
+}
+template <> __device__ __forceinline__ void stv<bf16_t, true>(bf16_t* p, int t, int, int C, f32x8 v) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    if (8 * t < C) *reinterpret_cast<b8*>(p + 8 * t) = __builtin_convertvector(v, b8);
+}
+// A row as it arrives, converted where it is used: the next step's rows are requested before this step's arithmetic and its barriers
+template <typename T, bool VEC> struct Raw {
+    static constexpr int N = VEC ? (int)sizeof(T) * 2 : 8;
+    unsigned a[N];
+    __device__ __forceinline__ void load(const T* row, int t, int tpr, int C) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) {
+                uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                if (row && 8 * t < C) u = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row + 8 * t) + 16 * i);
+                a[4 * i] = u.x; a[4 * i + 1] = u.y; a[4 * i + 2] = u.z; a[4 * i + 3] = u.w;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) v[j] = 0.f;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) { const int c = chan<false>(t, j, tpr); v[j] = c < C ? to_f32(p[c]) : 0.f; }
-    }
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void stv(T* p, int t, int tpr, int C, const float (&v)[VPT]) {
-    if constexpr (VEC) {
-        if (8 * t < C) {
-            if constexpr (sizeof(T) == 2) VecIO<bf16_t, 8>::store(reinterpret_cast<bf16_t*>(p) + 8 * t, v);
-            else {
-                store4(reinterpret_cast<float*>(p) + 8 * t, (f32x4){v[0], v[1], v[2], v[3]});
-                store4(reinterpret_cast<float*>(p) + 8 * t + 4, (f32x4){v[4], v[5], v[6], v[7]});
+            for (int j = 0; j < 8; ++j) {
+                a[j] = 0u;
+                if (row && j * tpr + t < C) {
+                    if constexpr (sizeof(T) == 2) a[j] = reinterpret_cast<const uint16_t*>(row)[j * tpr + t];
+                    else a[j] = reinterpret_cast<const unsigned*>(row)[j * tpr + t];
+                }
             }
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) { const int c = chan<false>(t, j, tpr); if (c < C) p[c] = from_f32<T>(v[j]); }
     }
-}
+    __device__ __forceinline__ f32x8 get() const {
+        f32x8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(a[j]);
+            else if constexpr (!VEC) v[j] = __uint_as_float(a[j] << 16);
+            else v[j] = __uint_as_float(j & 1 ? a[j / 2] & 0xffff0000u : a[j / 2] << 16);
+        }
+        return v;
+    }
+};
 // a gate row: its dtype is a run-time flag (uniform over the launch)
 template <bool VEC>
-__device__ __forceinline__ void ldg(const void* p, int dt, long row, int t, int tpr, int C, float (&v)[VPT]) {
-    if (dt == PASSION_BF16) ldv<bf16_t, VEC>(static_cast<const bf16_t*>(p) + row * C, t, tpr, C, v);
-    else ldv<float, VEC>(static_cast<const float*>(p) + row * C, t, tpr, C, v);
+__device__ __forceinline__ f32x8 ldg(const void* p, int dt, long row, int t, int tpr, int C) {
+    if (dt == PASSION_BF16) return ldv<bf16_t, VEC>(static_cast<const bf16_t*>(p) + row * C, t, tpr, C);
+    return ldv<float, VEC>(static_cast<const float*>(p) + row * C, t, tpr, C);
 }
 template <bool VEC>
-__device__ __forceinline__ void ldc(const float* p, float other, int t, int tpr, int C, float (&v)[VPT]) {
-    if (p) ldv<float, VEC>(p, t, tpr, C, v);
-    else {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) v[j] = other;
-    }
-}
+__device__ __forceinline__ f32x8 ldc(const float* p, float other, int t, int tpr, int C) { return p ? ldv<float, VEC>(p, t, tpr, C) : all8(other); }
 
-// two sums over the threads of a row.  red: [rows of the workgroup][2 wavefront slots ...], one use per barrier interval
-__device__ __forceinline__ void row_sum2(float& a, float& b, int tpr, float* red, int wv) {
-    const int w = tpr < 64 ? tpr : 64;
-    for (int o = w >> 1; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
-    if (tpr <= 64) return;
-    const int nw = tpr >> 6, w0 = wv / nw * nw;
-    if ((threadIdx.x & 63) == 0) { red[2 * wv] = a; red[2 * wv + 1] = b; }
-    __syncthreads();
-    a = b = 0.f;
-    for (int i = 0; i < nw; ++i) { a += red[2 * (w0 + i)]; b += red[2 * (w0 + i) + 1]; }
-}
+__device__ __forceinline__ float sum8(f32x8 v) { return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])); }
 
-// mean and 1 / sqrt(variance + eps) (LayerNorm) or 0 and 1 / sqrt(mean square + eps) of a row; nval: the thread's channels inside C,
-// nwave: those of the whole wavefront's part of the row
-__device__ __forceinline__ void moments(const float (&v)[VPT], int nval, float nwave, int kind, float eps, float invC, int tpr, float* red, int wv,
-                                        float& mean, float& rstd) {
-    float s = 0.f, q = 0.f;
-    if (kind == 2) {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) q = __builtin_fmaf(v[j], v[j], q);
-        row_sum2(s, q, tpr, red, wv);
-        mean = 0.f;
-        rstd = 1.f / sqrtf(q * invC + eps);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) s += v[j];                      // channels past C hold 0
-    const int w = tpr < 64 ? tpr : 64;
-    for (int o = w >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    const float mw = tpr <= 64 ? s * invC : (nwave > 0.f ? s / nwave : 0.f);
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) { const float d = v[j] - mw; if (j < nval) q = __builtin_fmaf(d, d, q); }
-    for (int o = w >> 1; o > 0; o >>= 1) q += __shfl_xor(q, o, 64);
-    if (tpr > 64) {
-        const int nw = tpr >> 6, w0 = wv / nw * nw;
-        if ((threadIdx.x & 63) == 0) { red[3 * wv] = s; red[3 * wv + 1] = q; red[3 * wv + 2] = nwave; }
-        __syncthreads();
-        s = 0.f;
-        for (int i = 0; i < nw; ++i) s += red[3 * (w0 + i)];
-        mean = s * invC;
-        q = 0.f;
-        for (int i = 0; i < nw; ++i) {
-            const float n = red[3 * (w0 + i) + 2], d = n > 0.f ? red[3 * (w0 + i)] / n - mean : 0.f;
-            q += __builtin_fmaf(n * d, d, red[3 * (w0 + i) + 1]);
-        }
-    } else mean = mw;
-    rstd = 1.f / sqrtf(q * invC + eps);
-}
-
-struct RowThread { int t, sub, rpb, nval; float nwave; };
+struct RowThread { int t, sub, rpb, wv, w0, nw, tpr, lanes; float nwave, invC, invW; f32x8 in; };
 template <bool VEC>
 __device__ __forceinline__ RowThread row_thread(int tpr, int C) {
     RowThread a;
+    a.tpr = tpr;
     a.t = threadIdx.x & (tpr - 1);
     a.sub = threadIdx.x / tpr;
     a.rpb = blockDim.x / tpr;
-    if (VEC) a.nval = 8 * a.t < C ? 8 : 0;
-    else a.nval = C > a.t ? min(VPT, (C - a.t + tpr - 1) / tpr) : 0;
-    float n = (float)a.nval;
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-    a.nwave = n;                                      // used where a row spans wavefronts only
+    a.wv = threadIdx.x >> 6;
+    a.nw = tpr > 64 ? tpr >> 6 : 1;
+    a.w0 = a.wv / a.nw * a.nw;
+    a.lanes = tpr < 64 ? tpr : 64;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) a.in[j] = (VEC ? 8 * a.t + j : j * tpr + a.t) < C ? 1.f : 0.f;      // the thread's channels inside C
+    a.nwave = lanes_sum(sum8(a.in), 64);                 // those of the whole wavefront (used where a row spans wavefronts)
+    a.invC = 1.f / (float)C;
+    a.invW = a.nwave > 0.f ? 1.f / a.nwave : 0.f;
     return a;
 }
 
-// grid (row chunks, B)
-template <typename TX, typename TH, bool VEC, int NT>
-__global__ __launch_bounds__(NT) void rn_fwd_kernel(RnP p, int tpr) {
-    __shared__ float red[2][16 * 3];
-    const int wv = threadIdx.x >> 6, C = p.C, b = blockIdx.y;
-    const RowThread a = row_thread<VEC>(tpr, C);
-    const float invC = 1.f / (float)C;
-    float w1[VPT], b1[VPT], w2[VPT], b2[VPT], sc[VPT], g[VPT];
-    ldc<VEC>(p.w1, 1.f, a.t, tpr, C, w1);
-    ldc<VEC>(p.b1, 0.f, a.t, tpr, C, b1);
-    ldc<VEC>(p.w2, 1.f, a.t, tpr, C, w2);
-    ldc<VEC>(p.b2, 0.f, a.t, tpr, C, b2);
-    ldc<VEC>(p.scale, 1.f, a.t, tpr, C, sc);
-    if (p.gmode == 1) {
-        ldg<VEC>(p.gate, p.gdt, b, a.t, tpr, C, g);
+// two sums over the threads of each of NR rows; red: 2 NR floats a wavefront, in use until the second barrier after this one
+template <int NR>
+__device__ __forceinline__ void row_sum2(float (&x)[NR], float (&y)[NR], const RowThread& a, float* red) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) sc[j] *= g[j];
+    for (int u = 0; u < NR; ++u) { x[u] = lanes_sum(x[u], a.lanes); y[u] = lanes_sum(y[u], a.lanes); }
+    if (a.tpr <= 64) return;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u) { red[(a.wv * NR + u) * 2] = x[u]; red[(a.wv * NR + u) * 2 + 1] = y[u]; }
     }
-    const int lo = blockIdx.x * p.chunk, hi = min(lo + p.chunk, p.N);
-    for (int n0 = lo; n0 < hi; n0 += a.rpb) {                    // every thread of the workgroup makes the same number of rounds (barriers inside)
-        const bool ok = n0 + a.sub < hi;
-        const long row = (long)b * p.N + (ok ? n0 + a.sub : hi - 1);
-        float xv[VPT], hv[VPT];
-        ldv<TX, VEC>(static_cast<const TX*>(p.x) + row * C, a.t, tpr, C, xv);
-        ldv<TH, VEC>(static_cast<const TH*>(p.h) + row * C, a.t, tpr, C, hv);
-        if (p.gmode == 2) ldg<VEC>(p.gate, p.gdt, row, a.t, tpr, C, g);
-        float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
-        if (p.post) {
-            moments(hv, a.nval, a.nwave, p.post, p.eps1, invC, tpr, red[0], wv, m1, r1);
+    __syncthreads();
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) hv[j] = __builtin_fmaf((hv[j] - m1) * r1, w1[j], b1[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const float m = p.gmode == 2 ? hv[j] * g[j] : hv[j];
-            xv[j] = j < a.nval ? __builtin_fmaf(m, sc[j], xv[j]) : 0.f;
-        }
-        if (p.pre) {
-            moments(xv, a.nval, a.nwave, p.pre, p.eps2, invC, tpr, red[1], wv, m2, r2);
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) hv[j] = __builtin_fmaf((xv[j] - m2) * r2, w2[j], b2[j]);
-        }
-        if (ok) {
-            stv<TX, VEC>(static_cast<TX*>(p.r) + row * C, a.t, tpr, C, xv);
-            if (p.pre) stv<TH, VEC>(static_cast<TH*>(p.y) + row * C, a.t, tpr, C, hv);
-            if (a.t == 0 && p.stat) store4(p.stat + 4 * row, (f32x4){m1, r1, m2, r2});
-        }
-        if (tpr > 64) __syncthreads();               // the slots are free for the next row
+    for (int u = 0; u < NR; ++u) {
+        x[u] = y[u] = 0.f;
+        for (int i = 0; i < a.nw; ++i) { x[u] += red[((a.w0 + i) * NR + u) * 2]; y[u] += red[((a.w0 + i) * NR + u) * 2 + 1]; }
     }
 }
 
-template <typename TX, typename TH, bool VEC, int NT>
-__global__ __launch_bounds__(NT) void rn_bwd_kernel(RnP p, int tpr) {
-    __shared__ float red[2][16 * 2];
-    extern __shared__ __attribute__((aligned(16))) float fold[];                     // [rpb][tpr][8], only where a workgroup holds several rows
-    const int wv = threadIdx.x >> 6, C = p.C, b = blockIdx.y;
-    const RowThread a = row_thread<VEC>(tpr, C);
-    const float invC = 1.f / (float)C;
-    float w1[VPT], b1[VPT], w2[VPT], sc[VPT], g[VPT];
-    ldc<VEC>(p.w1, 1.f, a.t, tpr, C, w1);
-    ldc<VEC>(p.b1, 0.f, a.t, tpr, C, b1);
-    ldc<VEC>(p.w2, 1.f, a.t, tpr, C, w2);
-    ldc<VEC>(p.scale, 1.f, a.t, tpr, C, sc);
-    if (p.gmode == 1) ldg<VEC>(p.gate, p.gdt, b, a.t, tpr, C, g);
-    else {
+// mean and 1 / sqrt(variance + eps) (kind 1) or 0 and 1 / sqrt(mean square + eps) (kind 2) of NR rows
+template <int NR>
+__device__ __forceinline__ void moments(const f32x8 (&v)[NR], int kind, float eps, const RowThread& a, float* red, float (&mean)[NR], float (&rstd)[NR]) {
+    float s[NR], q[NR];
+    if (kind == 2) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) g[j] = 1.f;
+        for (int u = 0; u < NR; ++u) { s[u] = 0.f; q[u] = sum8(v[u] * v[u]); }
+        row_sum2<NR>(s, q, a, red);
+#pragma unroll
+        for (int u = 0; u < NR; ++u) { mean[u] = 0.f; rstd[u] = 1.f / sqrtf(q[u] * a.invC + eps); }
+        return;
     }
-    float acc[6][VPT];
+    const float inv = a.tpr <= 64 ? a.invC : a.invW;
 #pragma unroll
-    for (int i = 0; i < 6; ++i)
+    for (int u = 0; u < NR; ++u) {
+        s[u] = lanes_sum(sum8(v[u]), a.lanes);               // channels past C hold 0
+        const f32x8 d = (v[u] - s[u] * inv) * a.in;
+        q[u] = lanes_sum(sum8(d * d), a.lanes);
+    }
+    if (a.tpr > 64) {                                        // wavefronts of a row: second moments about their own means, joined about the row's
+        if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) acc[i][j] = 0.f;
+            for (int u = 0; u < NR; ++u) {
+                float* r = red + (a.wv * NR + u) * 3;
+                r[0] = s[u]; r[1] = q[u]; r[2] = a.nwave;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+            s[u] = q[u] = 0.f;
+            for (int i = 0; i < a.nw; ++i) s[u] += red[((a.w0 + i) * NR + u) * 3];
+            mean[u] = s[u] * a.invC;
+            for (int i = 0; i < a.nw; ++i) {
+                const float* r = red + ((a.w0 + i) * NR + u) * 3;
+                const float n = r[2], d = n > 0.f ? r[0] / n - mean[u] : 0.f;
+                q[u] += __builtin_fmaf(n * d, d, r[1]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < NR; ++u) mean[u] = s[u] * a.invC;
+    }
+#pragma unroll
+    for (int u = 0; u < NR; ++u) rstd[u] = 1.f / sqrtf(q[u] * a.invC + eps);
+}
+
+// grid (row chunks, B); a step takes NR rows a row-thread group: their loads are in flight together and they share the barriers
+template <typename TX, typename TH, bool VEC, int NT, int NR>
+__global__ __launch_bounds__(NT) void rn_fwd_kernel(RnP p, int tpr) {
+    __shared__ float red[2][2][NT / 64 * NR * 3];            // [step parity][norm]: a slot is written again two barriers later at the earliest
+    const int C = p.C, b = blockIdx.y;
+    const RowThread a = row_thread<VEC>(tpr, C);
+    const f32x8 w1 = ldc<VEC>(p.w1, 1.f, a.t, tpr, C), b1 = ldc<VEC>(p.b1, 0.f, a.t, tpr, C), w2 = ldc<VEC>(p.w2, 1.f, a.t, tpr, C),
+                b2 = ldc<VEC>(p.b2, 0.f, a.t, tpr, C);
+    f32x8 sc = ldc<VEC>(p.scale, 1.f, a.t, tpr, C);
+    if (p.gmode == 1) sc *= ldg<VEC>(p.gate, p.gdt, b, a.t, tpr, C);
     const int lo = blockIdx.x * p.chunk, hi = min(lo + p.chunk, p.N);
-    for (int n0 = lo; n0 < hi; n0 += a.rpb) {
-        const bool ok = n0 + a.sub < hi;
-        const long row = (long)b * p.N + (ok ? n0 + a.sub : hi - 1);
-        float xv[VPT], hv[VPT], dr[VPT], dy[VPT];
-        ldv<TX, VEC>(static_cast<const TX*>(p.x) + row * C, a.t, tpr, C, xv);
-        ldv<TH, VEC>(static_cast<const TH*>(p.h) + row * C, a.t, tpr, C, hv);
+    int par = 0;
+    Raw<TX, VEC> xn[NR];
+    Raw<TH, VEC> hn[NR];
+    auto fetch = [&](int n0) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) { dr[j] = 0.f; dy[j] = 0.f; }
-        if (ok && p.dr) ldv<TX, VEC>(static_cast<const TX*>(p.dr) + row * C, a.t, tpr, C, dr);
-        if (ok && p.dy) ldv<TH, VEC>(static_cast<const TH*>(p.dy) + row * C, a.t, tpr, C, dy);
-        if (p.gmode == 2) ldg<VEC>(p.gate, p.gdt, row, a.t, tpr, C, g);
-        const f32x4 st = load4(p.stat + 4 * row);
-        float u[VPT];
+        for (int u = 0; u < NR; ++u) {
+            const long at = ((long)b * p.N + min(n0 + u * a.rpb + a.sub, hi - 1)) * C;
+            hn[u].load(static_cast<const TH*>(p.h) + at, a.t, tpr, C);
+            xn[u].load(static_cast<const TX*>(p.x) + at, a.t, tpr, C);
+        }
+    };
+    if (lo < hi) fetch(lo);
+    for (int n0 = lo; n0 < hi; n0 += a.rpb * NR, par ^= 1) {             // every thread of the workgroup makes the same number of rounds (barriers inside)
+        bool ok[NR];
+        long row[NR];
+        f32x8 xv[NR], hv[NR], gv[NR];
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            hv[j] = (hv[j] - st[0]) * st[1];                          // h hat (h itself without a post norm: mean 0, rstd 1)
-            u[j] = __builtin_fmaf(hv[j], w1[j], b1[j]);
-            if (p.pre) {
-                const float rr = __builtin_fmaf(u[j] * g[j], sc[j], xv[j]);
-                xv[j] = (rr - st[2]) * st[3];                         // r hat
+        for (int u = 0; u < NR; ++u) {
+            const int n = n0 + u * a.rpb + a.sub;
+            ok[u] = n < hi;
+            row[u] = (long)b * p.N + (ok[u] ? n : hi - 1);
+            hv[u] = hn[u].get();
+            xv[u] = xn[u].get();
+            if (p.gmode == 2) gv[u] = ldg<VEC>(p.gate, p.gdt, row[u], a.t, tpr, C);
+        }
+        if (n0 + a.rpb * NR < hi) fetch(n0 + a.rpb * NR);
+        float m1[NR], r1[NR], m2[NR], r2[NR];
+#pragma unroll
+        for (int u = 0; u < NR; ++u) { m1[u] = m2[u] = 0.f; r1[u] = r2[u] = 1.f; }
+        if (p.post) {
+            moments<NR>(hv, p.post, p.eps1, a, red[par][0], m1, r1);
+#pragma unroll
+            for (int u = 0; u < NR; ++u) hv[u] = (hv[u] - m1[u]) * r1[u] * w1 + b1;
+        }
+#pragma unroll
+        for (int u = 0; u < NR; ++u) xv[u] = ((p.gmode == 2 ? hv[u] * gv[u] : hv[u]) * sc + xv[u]) * a.in;
+        if (p.pre) {
+            moments<NR>(xv, p.pre, p.eps2, a, red[par][1], m2, r2);
+#pragma unroll
+            for (int u = 0; u < NR; ++u) hv[u] = (xv[u] - m2[u]) * r2[u] * w2 + b2;
+        }
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+            if (!ok[u]) continue;
+            stv<TX, VEC>(static_cast<TX*>(p.r) + row[u] * C, a.t, tpr, C, xv[u]);
+            if (p.pre) stv<TH, VEC>(static_cast<TH*>(p.y) + row[u] * C, a.t, tpr, C, hv[u]);
+            if (a.t == 0 && p.stat) store4(p.stat + 4 * row[u], (f32x4){m1[u], r1[u], m2[u], r2[u]});
+        }
+    }
+}
+
+template <typename TX, typename TH, bool VEC, int NT, int NR>
+__global__ __launch_bounds__(NT) void rn_bwd_kernel(RnP p, int tpr) {
+    __shared__ float red[2][2][NT / 64 * NR * 2];
+    extern __shared__ __attribute__((aligned(16))) float fold[];                     // [rpb][tpr][8], only where a workgroup holds several rows
+    const int C = p.C, b = blockIdx.y;
+    const RowThread a = row_thread<VEC>(tpr, C);
+    const f32x8 w1 = ldc<VEC>(p.w1, 1.f, a.t, tpr, C), b1 = ldc<VEC>(p.b1, 0.f, a.t, tpr, C), w2 = ldc<VEC>(p.w2, 1.f, a.t, tpr, C),
+                sc = ldc<VEC>(p.scale, 1.f, a.t, tpr, C);
+    f32x8 g[NR], acc[6];
+#pragma unroll
+    for (int u = 0; u < NR; ++u) g[u] = p.gmode == 1 ? ldg<VEC>(p.gate, p.gdt, b, a.t, tpr, C) : all8(1.f);
+#pragma unroll
+    for (int i = 0; i < 6; ++i) acc[i] = all8(0.f);
+    const int lo = blockIdx.x * p.chunk, hi = min(lo + p.chunk, p.N);
+    int par = 0;
+    Raw<TX, VEC> xn[NR], drn[NR];
+    Raw<TH, VEC> hn[NR], dyn[NR];
+    f32x4 stn[NR];
+    auto fetch = [&](int n0) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+            const int n = n0 + u * a.rpb + a.sub;
+            const bool in = n < hi;
+            const long r = (long)b * p.N + (in ? n : hi - 1), at = r * C;
+            stn[u] = load4(p.stat + 4 * r);
+            hn[u].load(static_cast<const TH*>(p.h) + at, a.t, tpr, C);
+            xn[u].load(static_cast<const TX*>(p.x) + at, a.t, tpr, C);
+            drn[u].load(in && p.dr ? static_cast<const TX*>(p.dr) + at : nullptr, a.t, tpr, C);
+            dyn[u].load(in && p.dy ? static_cast<const TH*>(p.dy) + at : nullptr, a.t, tpr, C);
+        }
+    };
+    if (lo < hi) fetch(lo);
+    for (int n0 = lo; n0 < hi; n0 += a.rpb * NR, par ^= 1) {
+        bool ok[NR];
+        long row[NR];
+        f32x8 xv[NR], hv[NR], dr[NR], dy[NR], uu[NR];
+        f32x4 st[NR];
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+            const int n = n0 + u * a.rpb + a.sub;
+            ok[u] = n < hi;
+            row[u] = (long)b * p.N + (ok[u] ? n : hi - 1);
+            st[u] = stn[u];
+            hv[u] = hn[u].get();
+            xv[u] = xn[u].get();
+            dr[u] = drn[u].get();
+            dy[u] = dyn[u].get();
+            if (p.gmode == 2) g[u] = ldg<VEC>(p.gate, p.gdt, row[u], a.t, tpr, C);
+        }
+        if (n0 + a.rpb * NR < hi) fetch(n0 + a.rpb * NR);
+        float s1[NR], s2[NR];
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+            hv[u] = (hv[u] - st[u][0]) * st[u][1];                          // h hat (h itself without a post norm: mean 0, rstd 1)
+            uu[u] = hv[u] * w1 + b1;
+            if (p.pre) xv[u] = (uu[u] * g[u] * sc + xv[u] - st[u][2]) * st[u][3];       // r hat
+        }
+        if (p.pre && p.dy) {                                                // dr += d pre(r) / d r
+#pragma unroll
+            for (int u = 0; u < NR; ++u) {
+                acc[2] += dy[u] * xv[u];
+                acc[3] += dy[u];
+                dy[u] = dy[u] * w2 * a.in;
+                s1[u] = sum8(dy[u] * xv[u]);
+                s2[u] = sum8(dy[u]);
             }
-        }
-        if (p.pre && p.dy) {                                          // dr += d pre(r) / d r
-            float s1 = 0.f, s2 = 0.f;
+            row_sum2<NR>(s1, s2, a, red[par][0]);
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                acc[2][j] = __builtin_fmaf(dy[j], xv[j], acc[2][j]);
-                acc[3][j] += dy[j];
-                dy[j] *= w2[j];
-                if (j < a.nval) { s1 = __builtin_fmaf(dy[j], xv[j], s1); s2 += dy[j]; }
+            for (int u = 0; u < NR; ++u) dr[u] += (dy[u] - (p.pre == 1 ? s2[u] * a.invC : 0.f) - xv[u] * (s1[u] * a.invC)) * st[u][3];
+        }
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+            if (ok[u]) stv<TX, VEC>(static_cast<TX*>(p.dx) + row[u] * C, a.t, tpr, C, dr[u]);
+            else dr[u] = all8(0.f);
+            acc[4] += dr[u] * (uu[u] * g[u]);
+            const f32x8 dm = dr[u] * sc;
+            uu[u] *= dm;                                                    // gradient of the gate
+            acc[5] += uu[u];
+            dy[u] = dm * g[u];                                              // ... of post(h)
+            acc[0] += dy[u] * hv[u];
+            acc[1] += dy[u];
+            dy[u] = dy[u] * w1;
+            if (ok[u] && p.dgate_tok) {
+                if (p.gdt == PASSION_BF16) stv<bf16_t, VEC>(static_cast<bf16_t*>(p.dgate_tok) + row[u] * C, a.t, tpr, C, uu[u]);
+                else stv<float, VEC>(static_cast<float*>(p.dgate_tok) + row[u] * C, a.t, tpr, C, uu[u]);
             }
-            row_sum2(s1, s2, tpr, red[0], wv);
-            s1 *= invC;
-            s2 = p.pre == 1 ? s2 * invC : 0.f;
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) dr[j] += st[3] * (dy[j] - s2 - xv[j] * s1);
-        }
-        if (ok) stv<TX, VEC>(static_cast<TX*>(p.dx) + row * C, a.t, tpr, C, dr);
-        else {
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) dr[j] = 0.f;
-        }
-        float du[VPT];
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            acc[4][j] = __builtin_fmaf(dr[j], u[j] * g[j], acc[4][j]);
-            const float dm = dr[j] * sc[j];
-            u[j] *= dm;                                               // gradient of the gate
-            acc[5][j] += u[j];
-            du[j] = dm * g[j];
-            acc[0][j] = __builtin_fmaf(du[j], hv[j], acc[0][j]);
-            acc[1][j] += du[j];
-            du[j] *= w1[j];
-        }
-        if (ok && p.dgate_tok) {
-            if (p.gdt == PASSION_BF16) stv<bf16_t, VEC>(static_cast<bf16_t*>(p.dgate_tok) + row * C, a.t, tpr, C, u);
-            else stv<float, VEC>(static_cast<float*>(p.dgate_tok) + row * C, a.t, tpr, C, u);
         }
         if (p.post) {
-            float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-            for (int j = 0; j < VPT; ++j)
-                if (j < a.nval) { s1 = __builtin_fmaf(du[j], hv[j], s1); s2 += du[j]; }
-            row_sum2(s1, s2, tpr, red[1], wv);
-            s1 *= invC;
-            s2 = p.post == 1 ? s2 * invC : 0.f;
+            for (int u = 0; u < NR; ++u) {
+                const f32x8 d = dy[u] * a.in;
+                s1[u] = sum8(d * hv[u]);
+                s2[u] = sum8(d);
+            }
+            row_sum2<NR>(s1, s2, a, red[par][1]);
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) du[j] = st[1] * (du[j] - s2 - hv[j] * s1);
+            for (int u = 0; u < NR; ++u) dy[u] = (dy[u] - (p.post == 1 ? s2[u] * a.invC : 0.f) - hv[u] * (s1[u] * a.invC)) * st[u][1];
         }
-        if (ok) stv<TH, VEC>(static_cast<TH*>(p.dh) + row * C, a.t, tpr, C, du);
-        if (tpr > 64) __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NR; ++u)
+            if (ok[u]) stv<TH, VEC>(static_cast<TH*>(p.dh) + row[u] * C, a.t, tpr, C, dy[u]);
     }
     float* out = p.part + ((long)b * gridDim.x + blockIdx.x) * 6 * C;
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
+        if (!((p.wanted >> i) & 1)) continue;                         // uniform
         if (a.rpb > 1) {                                              // rows of the workgroup, in order
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) fold[(a.sub * tpr + a.t) * VPT + j] = acc[i][j];
+            for (int j = 0; j < VPT; ++j) fold[(j * a.rpb + a.sub) * tpr + a.t] = acc[i][j];
             __syncthreads();
-            if (a.sub == 0) {
-                for (int s = 1; s < a.rpb; ++s)
-#pragma unroll
-                    for (int j = 0; j < VPT; ++j) acc[i][j] += fold[(s * tpr + a.t) * VPT + j];
+            for (int e = threadIdx.x; e < VPT * tpr; e += NT) {
+                const int j = e / tpr, t = e % tpr, c = VEC ? 8 * t + j : j * tpr + t;
+                float s = 0.f;
+                for (int r = 0; r < a.rpb; ++r) s += fold[(j * a.rpb + r) * tpr + t];
+                if (c < C) out[(long)i * C + c] = s;
             }
-        }
-        if (a.sub == 0) stv<float, VEC>(out + (long)i * C, a.t, tpr, C, acc[i]);
+        } else stv<float, VEC>(out + (long)i * C, a.t, tpr, C, acc[i]);
     }
 }
 
-// column sums of the partials: slot 0 .. 4 over all workgroups, the gate's (slot 5) over those of its sample.  64 columns x 4 runs of
-// partials a workgroup, joined in order.  grid (ceil(C / 64), 5 + B)
+// column sums of the partials: slot 0 .. 4 over all workgroups, the gate's (slot 5) over those of its sample.  32 columns x 32 runs of
+// partials a workgroup, joined in order.  grid (ceil(C / 32), 5 + B)
 struct RnFold { const float* part; float* out[5]; void* dgate; int gdt, C, nblk, B; };
-__global__ __launch_bounds__(256) void rn_fold_kernel(RnFold f) {
-    __shared__ float red[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void rn_fold_kernel(RnFold f) {
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, run = threadIdx.x >> 5;
     const int what = blockIdx.y < 5 ? blockIdx.y : 5, b = blockIdx.y - 5;
     if (what < 5 ? !f.out[what] : !f.dgate) return;                   // uniform over the workgroup
     const long lo = what < 5 ? 0 : (long)b * f.nblk, n = what < 5 ? (long)f.B * f.nblk : f.nblk;
-    const long i0 = lo + n * run / 4, i1 = lo + n * (run + 1) / 4;
+    const long i0 = lo + n * run / 32, i1 = lo + n * (run + 1) / 32;
     float s = 0.f;
-    if (c < f.C)
-        for (long i = i0; i < i1; ++i) s += f.part[(i * 6 + what) * f.C + c];
-    red[run][threadIdx.x & 63] = s;
+    if (c < f.C) {
+        long i = i0;
+        for (; i + 4 <= i1; i += 4) {                                 // four loads in flight, added in order
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = f.part[((i + u) * 6 + what) * f.C + c];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s += v[u];
+        }
+        for (; i < i1; ++i) s += f.part[(i * 6 + what) * f.C + c];
+    }
+    red[run][lane] = s;
     __syncthreads();
     if (run == 0 && c < f.C) {
-        s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += red[i][lane];
         if (what < 5) f.out[what][c] = s;
         else if (f.gdt == PASSION_BF16) static_cast<bf16_t*>(f.dgate)[(long)b * f.C + c] = (bf16_t)s;
         else static_cast<float*>(f.dgate)[(long)b * f.C + c] = s;
@@ -358,11 +447,11 @@ int launch_nt(const RnP& p, int tpr, bool bwd, bool vec, hipStream_t st) {
     const dim3 grid((p.N + p.chunk - 1) / p.chunk, p.B);
     if (bwd) {
         const int bytes = NT > tpr ? NT * VPT * (int)sizeof(float) : 0;
-        if (vec) hipLaunchKernelGGL((rn_bwd_kernel<TX, TH, true, NT>), grid, dim3(NT), bytes, st, p, tpr);
-        else hipLaunchKernelGGL((rn_bwd_kernel<TX, TH, false, NT>), grid, dim3(NT), bytes, st, p, tpr);
+        if (vec) hipLaunchKernelGGL((rn_bwd_kernel<TX, TH, true, NT, 1>), grid, dim3(NT), bytes, st, p, tpr);
+        else hipLaunchKernelGGL((rn_bwd_kernel<TX, TH, false, NT, 1>), grid, dim3(NT), bytes, st, p, tpr);
     } else {
-        if (vec) hipLaunchKernelGGL((rn_fwd_kernel<TX, TH, true, NT>), grid, dim3(NT), 0, st, p, tpr);
-        else hipLaunchKernelGGL((rn_fwd_kernel<TX, TH, false, NT>), grid, dim3(NT), 0, st, p, tpr);
+        if (vec) hipLaunchKernelGGL((rn_fwd_kernel<TX, TH, true, NT, NT == 1024 ? 1 : 2>), grid, dim3(NT), 0, st, p, tpr);
+        else hipLaunchKernelGGL((rn_fwd_kernel<TX, TH, false, NT, 1>), grid, dim3(NT), 0, st, p, tpr);
     }
     LAUNCH_RET();
     return 0;
@@ -426,12 +515,15 @@ extern "C" int passion_residual_norm_bwd(const void* x, int x_dtype, const void*
     p.x = x; p.h = h; p.gate = gate; p.w1 = post ? w_post : nullptr; p.b1 = post == 1 ? b_post : nullptr; p.w2 = w_pre; p.scale = scale;
     p.stat = const_cast<float*>(stat); p.dr = dr; p.dy = pre ? dy : nullptr; p.dx = dx; p.dh = dh; p.dgate_tok = gate_mode == 2 ? dgate : nullptr;
     p.part = part; p.B = B; p.N = N; p.C = C; p.post = post; p.pre = pre; p.gmode = gate_mode; p.gdt = gate_dtype;
+    p.wanted = (dw_post ? 1 : 0) | (db_post ? 2 : 0) | (dw_pre ? 4 : 0) | (db_pre ? 8 : 0) | (dscale ? 16 : 0) | (gate_mode == 1 && dgate ? 32 : 0);
     const int nblk = bwd_blocks(B, N, C, p.chunk);
     hipStream_t st = (hipStream_t)stream;
     const int rc = dispatch(p, x_dtype, h_dtype, true, st);
     if (rc) return rc;
     RnFold f{part, {dw_post, db_post, dw_pre, db_pre, dscale}, gate_mode == 1 ? dgate : nullptr, gate_dtype, C, nblk, B};
-    hipLaunchKernelGGL(rn_fold_kernel, dim3((C + 63) / 64, 5 + (gate_mode == 1 && dgate ? B : 0)), dim3(256), 0, st, f);
-    LAUNCH_RET();
+    if (p.wanted) {
+        hipLaunchKernelGGL(rn_fold_kernel, dim3((C + 31) / 32, 5 + (gate_mode == 1 && dgate ? B : 0)), dim3(1024), 0, st, f);
+        LAUNCH_RET();
+    }
     return 0;
 }
