@@ -13,12 +13,13 @@ struct RelP {
     const float* e;                       // [H][nd] bias by offset, log2 units
     const void* table;                    // [nb][H], where few queries read it directly
     const int* buckets;                   // [nd]; NULL: an offset is its own bucket
-    float* slab;                          // the table's partial gradients, rows of slab_len; NULL: not wanted
+    float* slab;                          // the table's partial gradients (LINE: rows of slab_len, else the dense sums); NULL: not wanted
     long slab_len;
+    int QC, KC, parts;                    // dense sums: distinct query and key cells, parts of the passes
     float *po, *pm, *pl;                  // split forward: [nsplit][B][H][Nq](D), f32
     int B, Nq, Nk, H, Hkv, D;
     int gd, gh, gw, vol, nd, omax, q0, nb, tdt;
-    int bias, pack, nsplit;
+    int bias, pack, few, nsplit;          // few: few query rows (forward), the bias read straight from the table
     float c, scale;                       // c = scale * log2(e)
 };
 
@@ -30,6 +31,6 @@ __device__ __forceinline__ float rel_log2_bias(const void* table, int tdt, int b
     return t <= -1e30f ? -INFINITY : fminf(t * 1.4426950408889634f, 3.0e38f) + (t != t ? t : 0.f);
 }
 
-// what: 0 forward, 1 dQ + table partials, 2 dK, dV; nw: wavefronts a workgroup (1 or 4)
+// what: 0 forward, 1 dQ, 2 dK, dV (LINE: and the table's partials), 3 the dense sums of the table's gradient; nw: wavefronts a workgroup (1, 2 or 4)
 int rel_run_bf16(const RelP& p, int what, int nw, hipStream_t st);
 int rel_run_f32(const RelP& p, int what, int nw, hipStream_t st);

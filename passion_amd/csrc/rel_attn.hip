@@ -16,24 +16,22 @@
 
 namespace {
 
-constexpr int BOX_MAX = 4096;           // offsets whose table (and four histograms of it) fit LDS beside the tiles
+constexpr int BOX_MAX = 4096;           // offsets whose table fits LDS beside the tiles (16 KB)
 
-// e[h][o] = log2 units of the head's bias at offset o
-__global__ __launch_bounds__(256) void rel_expand_kernel(const void* table, int tdt, const int* buckets, int nb, int nd, int H, float* e) {
-    const int o = blockIdx.x * 256 + threadIdx.x;
-    if (o >= nd) return;
-    const int c = buckets ? buckets[o] : o;
-    for (int h = blockIdx.y; h < H; h += gridDim.y) e[(long)h * nd + o] = rel_log2_bias(table, tdt, c, nb, h, H);
-}
-
-__global__ __launch_bounds__(256) void rel_zero_kernel(float* p, long n) {
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.f;
-}
-
-// delta[b][h][q] = dout . out: 16 lanes a row
+// before the large kernels: workgroups [0, eb) form e[h][o] = log2 units of the head's bias at offset o, 256 / 8 offsets x 8 heads at a time; the others (backward)
+// delta[b][h][q] = dout . out, 16 lanes a row
 template <typename T>
-__global__ __launch_bounds__(256) void rel_delta_kernel(const T* o, const T* dout, float* delta, int B, int Nq, int H, int D) {
-    const long row = ((long)blockIdx.x * 256 + threadIdx.x) >> 4;             // (b Nq + q) H + h
+__global__ __launch_bounds__(256) void rel_pre_kernel(RelP p, float* e, int eb) {
+    if ((int)blockIdx.x < eb) {
+        const int o = blockIdx.x * 32 + (threadIdx.x & 31);
+        if (o >= p.nd) return;
+        const int c = p.buckets ? p.buckets[o] : o;
+        for (int h = threadIdx.x >> 5; h < p.H; h += 8) e[(long)h * p.nd + o] = rel_log2_bias(p.table, p.tdt, c, p.nb, h, p.H);
+        return;
+    }
+    const T *o = static_cast<const T*>(p.o), *dout = static_cast<const T*>(p.dout);
+    const int B = p.B, Nq = p.Nq, H = p.H, D = p.D;
+    const long row = ((long)(blockIdx.x - eb) * 256 + threadIdx.x) >> 4;             // (b Nq + q) H + h
     const int c = (threadIdx.x & 15) * 8;
     float s = 0.f;
     if (row < (long)B * Nq * H && c < D) {
@@ -47,7 +45,7 @@ __global__ __launch_bounds__(256) void rel_delta_kernel(const T* o, const T* dou
     s = group16_sum(s);
     if ((threadIdx.x & 15) == 0 && row < (long)B * Nq * H) {
         const long bq = row / H;
-        delta[((bq / Nq) * H + row % H) * Nq + bq % Nq] = s;
+        p.delta[((bq / Nq) * H + row % H) * Nq + bq % Nq] = s;
     }
 }
 
@@ -77,24 +75,86 @@ __global__ __launch_bounds__(256) void rel_combine_kernel(RelP p) {
     if (d == 0 && p.lse) p.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
-// G[h][o] = sum of the slab rows (b, tile) in order; four runs of rows a workgroup, joined in order.  line > 0: the rows are windows (row `tile`
-// begins at offset (gw - 1) + q_start + 32 tile - line + 1).  identity: written as the table's gradient at once
-struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, nd, tiles, line, base; };
-__global__ __launch_bounds__(256) void rel_fold_kernel(FoldP f) {
-    __shared__ float red[4][64];
-    const int o = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6, h = blockIdx.y;
-    const long n = (long)f.B * f.tiles, i0 = n * run / 4, i1 = n * (run + 1) / 4;
-    float s = 0.f;
-    if (o < f.nd)
-        for (long i = i0; i < i1; ++i) {
-            const int b = (int)(i / f.tiles), t = (int)(i % f.tiles);
-            const long u = f.line ? (long)o - f.base - 32L * t + f.line - 1 : o;
-            if (u >= 0 && u < f.len) s += f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + u];
+// ... of many splits (few rows): a workgroup a row, 8 groups of 32 lanes take every eighth split, joined in order
+template <typename T>
+__global__ __launch_bounds__(256) void rel_combine_row_kernel(RelP p) {
+    __shared__ float red[8][32 * 4 + 4];
+    const long rows = (long)p.B * p.H * p.Nq, row = blockIdx.x;
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, d = lane * 4;
+    float M = -INFINITY;
+    for (int s = lane; s < p.nsplit; s += 32) M = fmaxf(M, p.pm[s * rows + row]);
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = g; s < p.nsplit; s += 8) {
+        const float w = __builtin_amdgcn_exp2f(p.pm[s * rows + row] - ref);
+        L = __builtin_fmaf(w, p.pl[s * rows + row], L);
+        if (d < p.D) {
+            const f32x4 v = load4(p.po + (s * rows + row) * p.D + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = __builtin_fmaf(w, v[j], a[j]);
         }
-    red[run][threadIdx.x & 63] = s;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[g][d + j] = a[j];
+    if (lane == 0) red[g][128] = L;
+    __syncthreads();
+    if (g) return;
+    L = 0.f;
+    a = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        L += red[i][128];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] += red[i][d + j];
+    }
+    const float f = L == 0.f ? 0.f : 1.f / L;
+    const long bh = row / p.Nq, q = row % p.Nq, b = bh / p.H, h = bh % p.H;
+    if (d < p.D) store4(static_cast<T*>(p.out) + ((b * p.Nq + q) * p.H + h) * p.D + d, (f32x4){a[0] * f, a[1] * f, a[2] * f, a[3] * f});
+    if (d == 0 && p.lse) p.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+}
+
+// G[h][o]: sums by offset of the partials, 64 offsets x 16 runs of partials a workgroup, joined in order; written as the table's gradient at once where every offset is
+// its own bucket (dt).
+//   LINE: slab rows (b, key tile) of stride len, lim places each: row t holds offset o at place o - (gw - 1) - q_start + 31 + 32 t
+//   dense: M[z][h][a][c]: query cell a (place, coordinates uniform over the wavefront), key cell = its cell - offset where that lies on the grid
+struct FoldP { const float* slab; float* G; void* dt; long len, lim; int tdt, B, H, nd, tiles, base; int gd, gh, gw, vol, q0, QC, KC, ld, parts; };
+template <bool LINE_>
+__global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, o = blockIdx.x * 64 + lane, h = blockIdx.y;
+    float s = 0.f;
+    if constexpr (LINE_) {
+        const long n = (long)f.B * f.tiles;
+        const int i0 = (int)(n * run / 16), i1 = (int)(n * (run + 1) / 16);
+#pragma unroll 4
+        for (int i = i0; i < i1; ++i) {
+            const int b = i / f.tiles, t = i - b * f.tiles;
+            const long u = (long)o - f.base + 31 + 32L * t;
+            if (o < f.nd && u >= 0 && u < f.lim) s += f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + u];
+        }
+    } else {
+        const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
+        const int dx = o % sx - (f.gw - 1), dy = o / sx % sy - (f.gh - 1), dz = o / sx / sy - (f.gd - 1);
+        const int a0 = (int)((long)f.QC * run / 16), a1 = (int)((long)f.QC * (run + 1) / 16);
+        for (int z = 0; z < f.parts; ++z) {
+            const float* m = f.slab + ((long)z * f.H + h) * f.QC * (long)f.ld;
+#pragma unroll 4
+            for (int a = a0; a < a1; ++a) {
+                const int t = (int)(((long)f.q0 + a) % f.vol), qx = t % f.gw, qy = t / f.gw % f.gh, qz = t / f.gw / f.gh;
+                const int x = qx - dx, y = qy - dy, zz = qz - dz, c = (zz * f.gh + y) * f.gw + x;
+                if (o < f.nd && (unsigned)x < (unsigned)f.gw && (unsigned)y < (unsigned)f.gh && (unsigned)zz < (unsigned)f.gd && c < f.KC) s += m[(long)a * f.ld + c];
+            }
+        }
+    }
+    red[run][lane] = s;
     __syncthreads();
     if (run == 0 && o < f.nd) {
-        s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += red[i][lane];
         if (f.dt) {
             if (f.tdt == PASSION_BF16) static_cast<bf16_t*>(f.dt)[(long)o * f.H + h] = (bf16_t)s;
             else static_cast<float*>(f.dt)[(long)o * f.H + h] = s;
@@ -145,16 +205,21 @@ int bias_mode(const RelP& p) {
 // few query rows: all heads of a key / value head in one tile, the bias read straight from the table (an expansion of all offsets would cost more)
 bool few_rows(const RelP& p) { return (long)p.Nq * (p.H / p.Hkv) <= 32 && p.Nq <= 16; }
 
-// the forward's key ranges: enough wavefronts for two to four per SIMD ... of 1024 SIMDs, two blocks of keys each at least
+// the forward's key ranges.  Few rows: a block of keys a workgroup up to 2048 of them (all of a short cache in flight at once); else until there is a wavefront a SIMD,
+// two blocks each at least
 int pick_split(const RelP& p, int dtype) {
     const long tiles = (p.pack ? tiles32((long)p.Nq * (p.H / p.Hkv)) * p.Hkv : tiles32(p.Nq) * p.H) * p.B;
     const int nblk = (p.Nk + blk_of(dtype) - 1) / blk_of(dtype);
+    if (p.few) return (int)hmax(1, hmin(nblk, 2048 / tiles));
     int s = 1;
     while (tiles * s < 1024 && nblk / (2 * s) >= 2) s *= 2;
     return s;
 }
-// wavefronts a workgroup: 4 share the staged tiles where that leaves every CU a workgroup and the rows fill them
-int pick_waves(long rows32, long others) { return rows32 >= 4 && rows32 * others >= 1024 ? 4 : 1; }
+// wavefronts a workgroup: as many as leave every CU a workgroup; they share the staged tiles
+int pick_waves(long rows32, long others) {
+    const long waves = rows32 * others;
+    return rows32 >= 4 && waves >= 900 ? 4 : rows32 >= 2 && waves >= 384 ? 2 : 1;
+}
 
 int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start, const void* table, int tdt, const int* buckets, int nb,
           const uint8_t* mask, float scale) {
@@ -165,7 +230,7 @@ int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int 
         if (gd < 1 || gh < 1 || gw < 1 || (tdt != PASSION_F32 && tdt != PASSION_BF16) || nb < 1) return -1003;
         const int64_t a = 2LL * gd - 1, b = 2LL * gh - 1, c = 2LL * gw - 1;
         if (a > (1 << 30) || b > (1 << 30) || c > (1LL << 31) || a * b > (1 << 30) || a * b * c > (1LL << 30)) return -1003;
-        p.gd = gd; p.gh = gh; p.gw = gw; p.vol = gd * gh * gw; p.nd = (int)(a * b * c);
+        p.gd = gd; p.gh = gh; p.gw = gw; p.vol = (int)((int64_t)gd * gh * gw); p.nd = (int)(a * b * c);
         p.omax = ((gd - 1) * (2 * gh - 1) + gh - 1) * (2 * gw - 1) + gw - 1;
         if (!buckets && nb != p.nd) return -1003;
         p.table = table; p.buckets = buckets; p.nb = nb; p.tdt = tdt;
@@ -177,11 +242,17 @@ int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int 
     return 0;
 }
 
-// slab rows (per batch sample and head) and their length
-void slab_shape(const RelP& p, int dtype, int nw, long& tiles, long& len) {
-    if (p.bias == 1) { tiles = (p.Nq + 32 * nw - 1) / (32 * nw); len = p.nd; }
-    else if (p.bias == 2) { tiles = tiles32(p.Nq); len = (long)blk_of(dtype) * ((p.Nk + blk_of(dtype) - 1) / blk_of(dtype)) + 31; }
-    else { tiles = tiles32(p.Nq); len = p.nd; }
+// partials of the table's gradient, in floats; sets what the kernels need to know of them
+long slab_floats(RelP& p, int dtype) {
+    const long blk = blk_of(dtype);
+    if (p.bias == 2) {
+        p.slab_len = (p.Nq + blk - 1) / blk * blk + 64;
+        return p.B * p.H * tiles32(p.Nk) * p.slab_len;
+    }
+    p.QC = (int)hmin(p.Nq, p.vol); p.KC = (int)hmin(p.Nk, p.vol);
+    const long passes = (long)p.B * ((p.Nq + p.QC - 1) / p.QC) * ((p.Nk + p.KC - 1) / p.KC), nkb = (p.KC + blk - 1) / blk, waves = tiles32(p.QC) * nkb * p.H;
+    p.parts = (int)hmax(1, hmin(passes, 2048 / waves));            // about two wavefronts a SIMD
+    return p.parts * p.H * p.QC * nkb * blk;
 }
 
 int run(const RelP& p, int dtype, int what, int nw, hipStream_t st) { return dtype == PASSION_BF16 ? rel_run_bf16(p, what, nw, st) : rel_run_f32(p, what, nw, st); }
@@ -189,39 +260,39 @@ int run(const RelP& p, int dtype, int what, int nw, hipStream_t st) { return dty
 // layout of the workspaces, in floats
 struct Ws { long e, po, pm, pl, delta, slab, G, total; };
 Ws fwd_ws(RelP& p, int dtype) {
-    p.pack = few_rows(p) && p.H > p.Hkv;
-    if (p.bias && few_rows(p)) p.bias = 3;
+    p.few = few_rows(p);
+    p.pack = p.few && p.H > p.Hkv;
+    if (p.bias == 1 && p.few) p.bias = 3;
     p.nsplit = pick_split(p, dtype);
     const long rows = (long)p.B * p.H * p.Nq;
     Ws w{};
     long at = 0;
     auto take = [&](long n) { const long r = at; at += (n + 63) / 64 * 64; return r; };
-    w.e = take(p.bias && !few_rows(p) ? (long)p.H * p.nd : 0);
+    w.e = take(p.bias && !p.few ? (long)p.H * p.nd : 0);
     w.po = take(p.nsplit > 1 ? p.nsplit * rows * p.D : 0);
     w.pm = take(p.nsplit > 1 ? p.nsplit * rows : 0);
     w.pl = take(p.nsplit > 1 ? p.nsplit * rows : 0);
     w.total = at;
     return w;
 }
-Ws bwd_ws(RelP& p, int dtype, bool want_table, int nw) {
+Ws bwd_ws(RelP& p, int dtype, bool want_table) {
     Ws w{};
     long at = 0;
     auto take = [&](long n) { const long r = at; at += (n + 63) / 64 * 64; return r; };
     w.e = take(p.bias ? (long)p.H * p.nd : 0);
     w.delta = take((long)p.B * p.H * p.Nq);
     if (p.bias && want_table) {
-        long tiles, len;
-        slab_shape(p, dtype, nw, tiles, len);
-        w.slab = take((long)p.B * p.H * tiles * len);
+        w.slab = take(slab_floats(p, dtype));
         w.G = take(p.buckets ? (long)p.H * p.nd : 0);
     }
     w.total = at;
     return w;
 }
-int q_waves(const RelP& p) { return pick_waves(tiles32(p.Nq), (long)p.H * p.B); }
-
-int expand(RelP& p, float* e, hipStream_t st) {
-    hipLaunchKernelGGL(rel_expand_kernel, dim3((p.nd + 255) / 256, p.H < 8 ? p.H : 8), dim3(256), 0, st, p.table, p.tdt, p.buckets, p.nb, p.nd, p.H, e);
+int pre(RelP& p, int dtype, float* e, hipStream_t st) {
+    const int eb = e ? (p.nd + 31) / 32 : 0;
+    const long db = p.delta ? ((long)p.B * p.Nq * p.H * 16 + 255) / 256 : 0;
+    if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_pre_kernel<bf16_t>, dim3((unsigned)(eb + db)), dim3(256), 0, st, p, e, eb);
+    else hipLaunchKernelGGL(rel_pre_kernel<float>, dim3((unsigned)(eb + db)), dim3(256), 0, st, p, e, eb);
     LAUNCH_RET();
     p.e = e;
     return 0;
@@ -244,7 +315,7 @@ extern "C" int64_t passion_rel_attn_workspace_floats(int dtype, int backward, in
     static const int dummy = 0;
     const int rc = setup(p, dtype, B, Nq, Nk, H, Hkv, D, gd, gh, gw, q_start, has_table ? &dummy : nullptr, PASSION_F32, has_buckets ? &dummy : nullptr, nb, nullptr, 1.f);
     if (rc) return rc;
-    return backward ? bwd_ws(p, dtype, true, q_waves(p)).total : fwd_ws(p, dtype).total;
+    return backward ? bwd_ws(p, dtype, true).total : fwd_ws(p, dtype).total;
 }
 
 extern "C" int passion_rel_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype, int B,
@@ -260,13 +331,16 @@ extern "C" int passion_rel_attn_fwd(const void* q, const int64_t* q_strides, con
     hipStream_t st = (hipStream_t)stream;
     const Ws w = fwd_ws(p, dtype);
     if (w.total && !workspace) return -1003;
-    if (p.bias && !few_rows(p) && (rc = expand(p, workspace + w.e, st))) return rc;
+    if (p.bias && !p.few && (rc = pre(p, dtype, workspace + w.e, st))) return rc;
     p.po = workspace + w.po; p.pm = workspace + w.pm; p.pl = workspace + w.pl;
     const long rows32 = p.pack ? tiles32((long)p.Nq * (p.H / p.Hkv)) : tiles32(p.Nq);
     if ((rc = run(p, dtype, 0, pick_waves(rows32, (long)(p.pack ? p.Hkv : p.H) * p.B * p.nsplit), st))) return rc;
     if (p.nsplit > 1) {
         const long rows = (long)p.B * p.H * p.Nq;
-        if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_combine_kernel<bf16_t>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+        if (p.nsplit > 8) {
+            if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_combine_row_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, p);
+            else hipLaunchKernelGGL(rel_combine_row_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, p);
+        } else if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_combine_kernel<bf16_t>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
         else hipLaunchKernelGGL(rel_combine_kernel<float>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
         LAUNCH_RET();
     }
@@ -286,32 +360,20 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
     if ((rc = strides(p, dtype, q_strides, k_strides, v_strides))) return rc;
     p.q = q; p.k = k; p.v = v; p.o = out; p.dout = dout; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
     hipStream_t st = (hipStream_t)stream;
-    const int nw = q_waves(p);
-    const Ws w = bwd_ws(p, dtype, dtable != nullptr, nw);
-    if (p.bias && (rc = expand(p, workspace + w.e, st))) return rc;
+    const Ws w = bwd_ws(p, dtype, dtable != nullptr);
     p.delta = workspace + w.delta;
-    const long rows16 = (long)B * Nq * H * 16;
-    if (dtype == PASSION_BF16)
-        hipLaunchKernelGGL(rel_delta_kernel<bf16_t>, dim3((unsigned)((rows16 + 255) / 256)), dim3(256), 0, st, (const bf16_t*)out, (const bf16_t*)dout, p.delta, B, Nq, H, D);
-    else hipLaunchKernelGGL(rel_delta_kernel<float>, dim3((unsigned)((rows16 + 255) / 256)), dim3(256), 0, st, (const float*)out, (const float*)dout, p.delta, B, Nq, H, D);
-    LAUNCH_RET();
-    long tiles = 0, len = 0;
-    if (dtable) {
-        slab_shape(p, dtype, nw, tiles, len);
-        p.slab = workspace + w.slab;
-        p.slab_len = len;
-        if (p.bias == 3) {
-            hipLaunchKernelGGL(rel_zero_kernel, dim3(2048), dim3(256), 0, st, p.slab, (long)B * H * tiles * len);
-            LAUNCH_RET();
-        }
-    }
-    if ((rc = run(p, dtype, 1, nw, st))) return rc;
+    if ((rc = pre(p, dtype, p.bias ? workspace + w.e : nullptr, st))) return rc;
+    if (dtable) p.slab = workspace + w.slab;
+    if ((rc = run(p, dtype, 1, pick_waves(tiles32(Nq), (long)H * B), st))) return rc;
     if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B), st))) return rc;
     if (dtable) {
+        const long nkb = p.bias == 2 ? 0 : (p.KC + blk_of(dtype) - 1) / blk_of(dtype);
+        if (p.bias != 2 && (rc = run(p, dtype, 3, pick_waves(tiles32(p.QC), nkb * H * p.parts), st))) return rc;
         float* G = workspace + w.G;
-        const FoldP f{p.slab, G, buckets ? nullptr : dtable, len, table_dtype, B, H, p.nd, (int)tiles, p.bias == 2 ? blk_of(dtype) * ((Nk + blk_of(dtype) - 1) / blk_of(dtype)) : 0,
-                      p.gw - 1 + p.q0};
-        hipLaunchKernelGGL(rel_fold_kernel, dim3((p.nd + 63) / 64, H), dim3(256), 0, st, f);
+        const FoldP f{p.slab, G, buckets ? nullptr : dtable, p.slab_len, p.slab_len - 64 + 31, table_dtype, B, H, p.nd, (int)tiles32(Nk), p.gw - 1 + p.q0, p.gd, p.gh, p.gw, p.vol, p.q0, p.QC, p.KC,
+                      (int)(nkb * blk_of(dtype)), p.parts};
+        if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<true>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
+        else hipLaunchKernelGGL(rel_fold_kernel<false>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
         LAUNCH_RET();
         if (buckets) {
             const bool few = nb <= 256;

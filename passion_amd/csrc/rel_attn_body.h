@@ -12,9 +12,13 @@
 //   LINE   a 1D raster: the offsets of a (query tile, key block) pair are one window of 32 NW + BLK - 1 values, staged with the block, and the LDS
 //          address of a score is a lane constant plus an immediate;
 //   GATHER one global read a score (L1 / L2), any grid.
-// Gradient of the table: sums of dS by offset, without atomics between wavefronts.  Every wavefront of the query-major kernel owns a histogram
-// and adds its dS in program order: BOX the whole table in LDS, LINE a sliding window of BLK + 31 values (BLK leave it for good after a block),
-// GATHER a slab row in global memory.  Slab rows are folded in order afterwards.
+// Gradient of the table: sums of dS by offset, without atomics and in a fixed order.
+//   LINE: in the key-major kernel.  A wavefront's 32 keys x BLK queries of dS go through LDS as [key][query] and are read back along the diagonals: row kk,
+//         column (lane + kk) mod BLK, so a lane's values all belong to offset lane or lane - BLK, conflict-free.  Offsets that no later block of queries
+//         reaches (BLK a block, one aligned store) leave for a slab row of the key tile; the rest stay in a register.  (LDS float atomics into a window instead
+//         took 170 to 280 cycles an instruction: 3.2 ms where this kernel and its sums now take a third.)
+//   BOX, GATHER: a kernel of its own sums dS over batch and repeated cells for every pair of cells (a pair's bias is loaded once, its sum stays in a
+//         register), and the sums by offset follow from that dense matrix.
 #include "common.h"
 #include "passion_hip.h"
 #include "rel_attn.h"
@@ -30,6 +34,7 @@ constexpr float LAZY = 8.0f;           // log2 units by which a block must excee
 enum { NONE = 0, BOX = 1, LINE = 2, GATHER = 3 };
 
 template <typename T> constexpr int blk() { return sizeof(T) == 2 ? 64 : 32; }                       // rows staged a step
+// (registers: widths above 64 and f32 need the 512 of one wavefront a SIMD)
 template <typename T, int DP> constexpr int row_stride() { return DP * (int)sizeof(T) + 16; }        // row reads: 16 rows hit 16 bank groups
 // image that is only read transposed: bf16 wants 4 consecutive rows' 64 bytes in disjoint 16-bank windows (stride mod 256 = 64 or 192)
 template <typename T, int DP> constexpr int tr_stride() { return sizeof(T) == 4 ? DP * 4 + 16 : DP == 32 ? 64 : DP * 2 + 64; }
@@ -137,7 +142,7 @@ __device__ __forceinline__ uint64_t valid_keys(const RelP& p, int b, int key0, i
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// query-major: MODE 0 forward (out, lse or split partials), MODE 1 backward (dQ and the table's histogram).
+// query-major: MODE 0 forward (out, lse or split partials), MODE 1 backward (dQ; delta corrected in place).
 // grid (ceil(rows / (32 NW)) * nsplit, heads, B).  pack (forward, few queries): a workgroup's rows are the Nq queries of all the heads that
 // share a key / value head, so that K and V are read once for them
 template <typename T, int DP, int NW, int MODE, int BIAS>
@@ -145,7 +150,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
     constexpr int RS = row_stride<T, DP>(), VS = MODE == 0 ? tr_stride<T, DP>() : RS;
     constexpr int KIMG = BLKN * RS, VIMG = BLKN * VS, POS = BLKN * 4, WIN = (32 * NW + BLKN) * 4;
-    constexpr int BUF = KIMG + VIMG + (BIAS == LINE ? WIN : BIAS == NONE ? 0 : POS);
+    // few queries (LINE): a window a head of the tile, BLK + Nq values each
+    const int wrow = BLKN + p.Nq, BUF = KIMG + VIMG + (BIAS == LINE ? (p.few ? (p.pack ? p.H / p.Hkv : 1) * wrow * 4 + 15 & ~15 : WIN) : BIAS == NONE ? 0 : POS);
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
     const int b = blockIdx.z, rep = p.H / p.Hkv;
@@ -181,27 +187,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     if (MODE == 1 && qok) { lse2 = p.lse[lrow]; dlt = p.delta[lrow]; }
     const int aq = (BIAS == BOX || BIAS == GATHER) ? place(p, p.q0 + qi) + p.omax : 0;      // offset of a pair = aq - place(key)
 
-    // LDS behind the two buffers: BOX: the head's table, then the wavefronts' histograms; LINE backward: the sliding histograms
-    float* tab = reinterpret_cast<float*>(lds + 2 * BUF);
-    float* hist = BIAS == BOX ? tab + p.nd + wv * p.nd : tab + wv * (BLKN + 32);
-    float* ghist = nullptr;
-    if (BIAS == BOX) {
+    float* tab = reinterpret_cast<float*>(lds + 2 * BUF);                                  // BOX: the head's table behind the two buffers
+    if (BIAS == BOX)
         for (int i = tid; i < p.nd; i += NT) tab[i] = p.e[(long)blockIdx.y * p.nd + i];
-        if (MODE == 1 && p.slab) for (int i = lane; i < p.nd; i += 64) hist[i] = 0.f;
-    }
-    if (MODE == 1 && BIAS == LINE) {
-        for (int i = lane; i < BLKN + 32; i += 64) hist[i] = 0.f;
-    }
-    if (MODE == 1 && BIAS != NONE && BIAS != BOX) {
-        const int tiles = (p.Nq + 31) / 32;
-        ghist = p.slab + (((long)b * p.H + blockIdx.y) * tiles + min(tile * NW + wv, tiles - 1)) * p.slab_len;
-    }
     const bool wave_on = tile * NW + wv < (rows + 31) / 32;       // a wavefront without a row stages tiles and keeps out of the rest
 
     f32x16 o[ND];
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) o[dt] = zero16();
-    float l_run = 0.f, m_run = -INFINITY;
+    float l_run = 0.f, m_run = -INFINITY;               // backward: l_run sums dS
 
     Tile<T, DP, NT> kt_, vt_;
     uint64_t vnext = 0;
@@ -212,7 +206,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         kt_.fetch(kb_, p.ks[1], kb * BLKN, p.Nk, p.D, tid);
         vt_.fetch(vb_, p.vs[1], kb * BLKN, p.Nk, p.D, tid);
         vnext = valid_keys<BLKN>(p, b, kb * BLKN, lane);
-        if (BIAS == LINE) {
+        if (BIAS == LINE && p.few) {                       // straight into the next buffer (last read before the previous barrier), from the table itself
+            float* w = reinterpret_cast<float*>(lds + ((kb - kb0) & 1) * BUF + KIMG + VIMG);
+            const int first = p.q0 - (kb * BLKN + BLKN - 1) + p.gw - 1, heads = p.pack ? rep : 1;
+            for (int i = tid; i < wrow; i += NT) {
+                const int at = first + i;
+                const bool in = at >= 0 && at < p.nd;
+                const int c = in ? (p.buckets ? p.buckets[at] : at) : -1;
+                for (int g = 0; g < heads; ++g) w[g * wrow + i] = rel_log2_bias(p.table, p.tdt, c, p.nb, blockIdx.y * heads + g, p.H);
+            }
+        } else if (BIAS == LINE) {
             // window value w <-> offset of (query tile 0 of the workgroup, last key of the block) + w
             const int first = p.q0 + tile * NW * 32 - (kb * BLKN + BLKN - 1) + p.gw - 1;
 #pragma unroll
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     auto commit = [&](char* buf) {
         kt_.commit(buf, RS, tid, vnext);
         vt_.commit(buf + KIMG, VS, tid, vnext);
-        if (BIAS == LINE) {
+        if (BIAS == LINE && !p.few) {
 #pragma unroll
             for (int i = 0; i < NWIN; ++i)
                 if (i * NT + tid < 32 * NW + BLKN) reinterpret_cast<float*>(buf + KIMG + VIMG)[i * NT + tid] = win[i];
@@ -253,7 +256,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 for (int s = 0; s < NCH; ++s) st[kt] = dot<T>(row_frag<T>(kimg, RS, kt * 32, s, lane), qf[s], st[kt]);
             }
             // ---- scores in log2 units: scale * log2(e) * s + bias
-            const float* wl = reinterpret_cast<const float*>(vimg + VIMG) + (32 * wv + (lane & 31) + BLKN - 1 - 4 * h);
+            const float* wl = reinterpret_cast<const float*>(vimg + VIMG) + (p.few ? (p.pack ? rowc / p.Nq : 0) * wrow + qi : 32 * wv + (lane & 31)) + BLKN - 1 - 4 * h;
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -312,44 +315,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) tr_product<T, ND>(vimg, VS, kt * 32, st[kt], o, lane);
             } else {
+                f32x16 ds[KT];
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    f32x16 dp = zero16();
+                    ds[kt] = zero16();
 #pragma unroll
-                    for (int s = 0; s < NCH; ++s) dp = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], dp);
+                    for (int s = 0; s < NCH; ++s) ds[kt] = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], ds[kt]);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) st[kt][r] = __builtin_amdgcn_exp2f(st[kt][r] - lse2) * (dp[r] - dlt);
-                    if (BIAS != NONE && p.slab) {
-                        float* hl = hist + ((lane & 31) + BLKN - 1 - 4 * h);
-#pragma unroll
-                        for (int g4 = 0; g4 < 4; ++g4) {
-                            int4 kp;
-                            if (BIAS == BOX || BIAS == GATHER) kp = *reinterpret_cast<const int4*>(vimg + VIMG + (kt * 32 + 8 * g4 + 4 * h) * 4);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int r = 4 * g4 + j;
-                                const int o_ = aq - (j == 0 ? kp.x : j == 1 ? kp.y : j == 2 ? kp.z : kp.w);
-                                if (BIAS == LINE) __hip_atomic_fetch_add(hl - (kt * 32 + 8 * g4 + j), st[kt][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                                else if (BIAS == BOX) __hip_atomic_fetch_add(hist + o_, st[kt][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                                else unsafeAtomicAdd(ghist + o_, st[kt][r]);
-                            }
-                        }
+                    for (int r = 0; r < 16; ++r) {
+                        st[kt][r] = __builtin_amdgcn_exp2f(st[kt][r] - lse2);
+                        ds[kt][r] = st[kt][r] * (ds[kt][r] - dlt);
+                        l_run += ds[kt][r];
                     }
-                    tr_product<T, ND>(kimg, RS, kt * 32, st[kt], o, lane);
                 }
-            }
-        }
-        if (MODE == 1 && BIAS == LINE && p.slab && wave_on) {
-            // offsets that no later block reaches leave the window; 31 move on
-            const int up = BLKN * (nblk_all - 1 - kb);
-            const float mv = lane < 31 ? hist[lane] : 0.f;
-            if (lane < BLKN) ghist[up + 31 + lane] = hist[31 + lane];
-            if (kb == nblk_all - 1) {
-                if (lane < 31) ghist[lane] = mv;
-            } else {
-                __builtin_amdgcn_wave_barrier();
-                if (lane < BLKN) hist[lane] = 0.f;
-                if (lane < 31) hist[BLKN + lane] = mv;
+                // a row of dS sums to 0; what it sums to instead is the error of delta, which was formed from the rounded out.  One block of keys: taken off here
+                // (few keys: there it shows); else by the kernels that follow, through the corrected delta
+                if (nblk_all == 1) {
+                    const float off = half_sum(l_run);
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) ds[kt][r] = __builtin_fmaf(-off, st[kt][r], ds[kt][r]);
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) tr_product<T, ND>(kimg, RS, kt * 32, ds[kt], o, lane);
             }
         }
         if (kb + 1 < kb1) commit(lds + ((kb + 1 - kb0) & 1) * BUF);
@@ -397,16 +386,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                         store4(dst + d, (f32x4){o[dt][4 * g4] * p.scale, o[dt][4 * g4 + 1] * p.scale, o[dt][4 * g4 + 2] * p.scale, o[dt][4 * g4 + 3] * p.scale});
                 }
         }
-        if (BIAS == BOX && p.slab) {                 // the workgroup's histograms in wavefront order (the loop ended on a barrier)
-            float* dst = p.slab + (((long)b * p.H + blockIdx.y) * gridDim.x + tile) * p.slab_len;
-            const float* h0 = tab + p.nd;
-            for (int i = tid; i < p.nd; i += NT) {
-                float s = 0.f;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) s += h0[w * p.nd + i];
-                dst[i] = s;
-            }
-        }
+        const float off = half_sum(l_run);
+        if (qok && h == 0) p.delta[lrow] = dlt + off;
     }
 }
 
@@ -439,7 +420,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         }
     }
     const int ak = (BIAS == BOX || BIAS == GATHER) ? p.omax - place(p, keyc) : 0;
-    float* tab = reinterpret_cast<float*>(lds + 2 * BUF);
+    float* tab = reinterpret_cast<float*>(lds + 2 * BUF);               // BOX
+    // LINE: dS of this wavefront as [key][query], rows of BLK + 4 (b128 writes of 16 keys cover the banks once)
+    constexpr int SK = BLKN + 4;
+    float* skew = reinterpret_cast<float*>(lds + 2 * BUF) + wv * 32 * SK;
+    float now = 0.f, before = 0.f;                                      // running sums: offsets that began with this block of queries / with the one before
+    const bool sums = BIAS == LINE && p.slab;
+    const bool keys_all = __ballot(kok) == ~0ull;
+    const int ktile = blockIdx.x * NW + wv, ktiles = (p.Nk + 31) / 32;
     const bool any = __syncthreads_or(kok);                             // a workgroup whose keys are all masked has only zeros to store
 
     f32x16 dk[ND], dv[ND];
@@ -486,6 +474,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 if (i * NT + tid < 32 * NW + BLKN) side[2 * BLKN + i * NT + tid] = win[i];
         }
     };
+    if (!any && sums && ktile < ktiles)                                 // its slab rows are folded all the same
+        for (int g = 0; g < rep; ++g) {
+            float* row = p.slab + (((long)b * p.H + hk * rep + g) * ktiles + ktile) * p.slab_len;
+            for (int i = lane; i < nqb * BLKN + 31; i += 64) row[i] = 0.f;
+        }
     if (any) {
         fetch(0);
         commit(lds);
@@ -529,8 +522,40 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                         da[r] = pr;                                     // P   (a lane's columns are its own key's: a masked key's are not stored)
                     }
                 }
+                if (sums) {
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        f32x4 v = {sa[4 * g4], sa[4 * g4 + 1], sa[4 * g4 + 2], sa[4 * g4 + 3]};
+                        if (!keys_all) v = kok ? v : (f32x4){0.f, 0.f, 0.f, 0.f};       // (uniform test)
+                        *reinterpret_cast<f32x4*>(skew + (lane & 31) * SK + qt * 32 + 8 * g4 + 4 * h) = v;
+                    }
+                }
                 tr_product<T, ND>(dimg, RS, qt * 32, da, dv, lane);
                 tr_product<T, ND>(qimg, RS, qt * 32, sa, dk, lane);
+            }
+            if (sums) {
+                // column (lane + kk) mod BLK of row kk: query - key = lane, or lane - BLK once it has wrapped around (then it continues the block before)
+                const int l = lane & (BLKN - 1);
+                constexpr int ROWS = BLKN == 64 ? 32 : 16;                  // BLK = 32: the two halves of the wavefront take 16 keys each
+                const int kk0 = BLKN == 64 ? 0 : 16 * h;
+#pragma unroll
+                for (int t = 0; t < ROWS; ++t) {
+                    const int kk = kk0 + t;
+                    const float v = skew[kk * SK + ((l + kk) & (BLKN - 1))];
+                    const bool wrapped = l + kk >= BLKN;
+                    now += wrapped ? 0.f : v;
+                    before += wrapped ? v : 0.f;
+                }
+                const float a = BLKN == 64 ? now : half_sum(now), c = BLKN == 64 ? before : half_sum(before);
+                const bool whole = l + 31 < BLKN;                           // no key of the tile wraps: the offset ends with this block
+                if (ktile < ktiles) {
+                    float* row = p.slab + (((long)b * p.H + head) * ktiles + ktile) * p.slab_len + (it % nqb) * BLKN;
+                    if (lane < BLKN) row[whole ? l + 31 : l + 31 - BLKN] = whole ? a : c;
+                    if ((it + 1) % nqb == 0 && lane < BLKN && !whole) row[l + 31] = a;       // the head's last block: what would have gone on
+                }
+                const bool end = (it + 1) % nqb == 0;
+                before = (whole || end || (BLKN == 32 && h)) ? 0.f : a;
+                now = 0.f;
             }
             if (it + 1 < steps) commit(lds + ((it + 1) & 1) * BUF);
             __syncthreads();
@@ -556,6 +581,103 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------
+// dS summed over the batch and over repeated cells, for every pair of cells: M[z][h][a][c], a < QC = min(Nq, vol) the queries a, a + QC, ..., c < KC = min(Nk, vol)
+// the keys c, c + KC, ....  grid (query tiles of 32 NW x key blocks, H, parts z of the passes (batch, query copy, key copy)).  Tiles as in rel_q_kernel
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_d_kernel(RelP p) {
+    constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32;
+    constexpr int RS = row_stride<T, DP>(), IMG = BLKN * RS, BUF = 2 * IMG;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int nkb = (p.KC + BLKN - 1) / BLKN, head = blockIdx.y, hk = head / (p.H / p.Hkv);
+    const int a = ((blockIdx.x / nkb) * NW + wv) * 32 + (lane & 31), c0 = (blockIdx.x % nkb) * BLKN;
+    const int MQ = (p.Nq + p.QC - 1) / p.QC, MK = (p.Nk + p.KC - 1) / p.KC;
+    const long passes = (long)p.B * MQ * MK;
+    const int t0 = (int)(passes * blockIdx.z / gridDim.z), t1 = (int)(passes * (blockIdx.z + 1) / gridDim.z);
+
+    f32x16 acc[KT], bias[KT];
+    const int aq = place(p, p.q0 + min(a, p.QC - 1)) + p.omax;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        acc[kt] = zero16();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bias[kt][r] = p.e[(long)head * p.nd + aq - place(p, min(c0 + kt * 32 + (r & 3) + 8 * (r >> 2) + 4 * h, p.KC - 1))];
+    }
+    u32x4 qf[NCH], df[NCH];
+    float lse2 = INFINITY, dlt = 0.f;
+    Tile<T, DP, NT> kt_, vt_;
+    uint64_t vnext = 0, valid;
+    auto fetch = [&](int t) {
+        const int b = t / (MQ * MK), j0 = (t % MK) * p.KC + c0, n = min(p.Nk, (t % MK + 1) * p.KC);
+        kt_.fetch(static_cast<const T*>(p.k) + (long)b * p.ks[0] + (long)hk * p.ks[2], p.ks[1], j0, n, p.D, tid);
+        vt_.fetch(static_cast<const T*>(p.v) + (long)b * p.vs[0] + (long)hk * p.vs[2], p.vs[1], j0, n, p.D, tid);
+        const int key = j0 + lane;
+        vnext = __ballot(lane < BLKN && key < n && (!p.mask || p.mask[(long)b * p.Nk + key]));
+    };
+    if (t0 < t1) {
+        fetch(t0);
+        kt_.commit(lds, RS, tid, vnext);
+        vt_.commit(lds + IMG, RS, tid, vnext);
+    }
+    valid = vnext;
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const char* kimg = lds + ((t - t0) & 1) * BUF;
+        if (t + 1 < t1) fetch(t + 1);
+        if (t == t0 || t % MK == 0) {                              // the next (batch, query copy)
+            const int b = t / (MQ * MK), i = (t / MK) % MQ * p.QC + a;
+            const bool qok = a < p.QC && i < p.Nq;
+            const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)i * p.qs[1] + (long)head * p.qs[2]);
+            const char* dp = reinterpret_cast<const char*>(static_cast<const T*>(p.dout) + (((long)b * p.Nq + i) * p.H + head) * p.D);
+#pragma unroll
+            for (int s = 0; s < NCH; ++s) {
+                qf[s] = df[s] = (u32x4){0u, 0u, 0u, 0u};
+                if (qok && 32 * s + 16 * h < p.D * (int)sizeof(T)) {
+                    qf[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s + 16 * h);
+                    df[s] = *reinterpret_cast<const u32x4*>(dp + 32 * s + 16 * h);
+                }
+            }
+            const long lrow = ((long)b * p.H + head) * p.Nq + i;
+            lse2 = qok ? p.lse[lrow] : INFINITY;
+            dlt = qok ? p.delta[lrow] : 0.f;
+        }
+        if (valid) {
+            const uint64_t vh = valid >> (4 * h);
+            const bool full = valid == (BLKN == 64 ? ~0ull : 0xffffffffull);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                f32x16 st = zero16(), dp = zero16();
+#pragma unroll
+                for (int s = 0; s < NCH; ++s) {
+                    st = dot<T>(row_frag<T>(kimg, RS, kt * 32, s, lane), qf[s], st);
+                    dp = dot<T>(row_frag<T>(kimg + IMG, RS, kt * 32, s, lane), df[s], dp);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], p.c, bias[kt][r]) - lse2) * (dp[r] - dlt);
+                    if (!full) v = (vh >> (kt * 32 + (r & 3) + 8 * (r >> 2))) & 1 ? v : 0.f;
+                    acc[kt][r] += v;
+                }
+            }
+        }
+        if (t + 1 < t1) {
+            kt_.commit(lds + ((t + 1 - t0) & 1) * BUF, RS, tid, vnext);
+            vt_.commit(lds + ((t + 1 - t0) & 1) * BUF + IMG, RS, tid, vnext);
+        }
+        valid = vnext;
+        __syncthreads();
+    }
+    if (a < p.QC) {
+        float* dst = p.slab + (((long)blockIdx.z * p.H + head) * p.QC + a) * ((long)nkb * BLKN) + c0 + 4 * h;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4)
+                store4(dst + kt * 32 + 8 * g4, (f32x4){acc[kt][4 * g4], acc[kt][4 * g4 + 1], acc[kt][4 * g4 + 2], acc[kt][4 * g4 + 3]});
+    }
+}
+
 template <typename K> int grant_lds(K kern, int bytes) {
     if (bytes > 64 * 1024) HIP_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     return 0;
@@ -564,9 +686,8 @@ template <typename K> int grant_lds(K kern, int bytes) {
 template <typename T, int DP, int NW, int MODE, int BIAS>
 int launch_q(const RelP& p, hipStream_t st) {
     constexpr int BLKN = blk<T>(), RS = row_stride<T, DP>(), VS = MODE == 0 ? tr_stride<T, DP>() : RS;
-    int bytes = 2 * (BLKN * (RS + VS) + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
-    if (BIAS == BOX) bytes += p.nd * 4 * (MODE == 1 && p.slab ? 1 + NW : 1);
-    if (BIAS == LINE && MODE == 1) bytes += NW * (BLKN + 32) * 4;
+    int bytes = 2 * (BLKN * (RS + VS) + (BIAS == LINE ? (p.few ? (p.pack ? p.H / p.Hkv : 1) * (BLKN + p.Nq) * 4 + 15 & ~15 : (32 * NW + BLKN) * 4) : BIAS == NONE ? 0 : BLKN * 4));
+    if (BIAS == BOX) bytes += p.nd * 4;
     const int rc = grant_lds(rel_q_kernel<T, DP, NW, MODE, BIAS>, bytes);
     if (rc) return rc;
     const int rows = p.pack ? p.Nq * (p.H / p.Hkv) : p.Nq;
@@ -579,6 +700,7 @@ int launch_k(const RelP& p, hipStream_t st) {
     constexpr int BLKN = blk<T>(), RS = row_stride<T, DP>();
     int bytes = 2 * (2 * BLKN * RS + 2 * BLKN * 4 + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
     if (BIAS == BOX) bytes += p.nd * 4;
+    if (BIAS == LINE && p.slab) bytes += NW * 32 * (BLKN + 4) * 4;
     const int rc = grant_lds(rel_k_kernel<T, DP, NW, BIAS>, bytes);
     if (rc) return rc;
     hipLaunchKernelGGL((rel_k_kernel<T, DP, NW, BIAS>), dim3((p.Nk + 32 * NW - 1) / (32 * NW), p.Hkv, p.B), dim3(64 * NW), bytes, st, p);
@@ -587,7 +709,18 @@ int launch_k(const RelP& p, hipStream_t st) {
 }
 
 template <typename T, int DP, int NW>
+int launch_d(const RelP& p, hipStream_t st) {
+    constexpr int BLKN = blk<T>(), bytes = 4 * BLKN * row_stride<T, DP>();
+    const int rc = grant_lds(rel_d_kernel<T, DP, NW>, bytes);
+    if (rc) return rc;
+    hipLaunchKernelGGL((rel_d_kernel<T, DP, NW>), dim3((p.QC + 32 * NW - 1) / (32 * NW) * ((p.KC + BLKN - 1) / BLKN), p.H, p.parts), dim3(64 * NW), bytes, st, p);
+    LAUNCH_RET();
+    return 0;
+}
+
+template <typename T, int DP, int NW>
 int pick_bias(const RelP& p, int what, hipStream_t st) {
+    if (what == 3) return launch_d<T, DP, NW>(p, st);
 #define REL_ONE(BIAS) (what == 0 ? launch_q<T, DP, NW, 0, BIAS>(p, st) : what == 1 ? launch_q<T, DP, NW, 1, BIAS>(p, st) : launch_k<T, DP, NW, BIAS>(p, st))
     switch (p.bias) {
         case NONE: return REL_ONE(NONE);
@@ -598,6 +731,8 @@ int pick_bias(const RelP& p, int what, hipStream_t st) {
 #undef REL_ONE
 }
 template <typename T, int DP>
-int pick_nw(const RelP& p, int what, int nw, hipStream_t st) { return nw == 4 ? pick_bias<T, DP, 4>(p, what, st) : pick_bias<T, DP, 1>(p, what, st); }
+int pick_nw(const RelP& p, int what, int nw, hipStream_t st) {
+    return nw == 4 ? pick_bias<T, DP, 4>(p, what, st) : nw == 2 ? pick_bias<T, DP, 2>(p, what, st) : pick_bias<T, DP, 1>(p, what, st);
+}
 
 }  // namespace
