@@ -66,23 +66,22 @@ template <> __device__ __forceinline__ void vload<bf16_t>(const bf16_t* p, float
 template <typename T> __device__ __forceinline__ void vstore(T* p, const float* v);
 template <> __device__ __forceinline__ void vstore<float>(float* p, const float* v) { store4(p, (f32x4){v[0], v[1], v[2], v[3]}); }
 template <> __device__ __forceinline__ void vstore<bf16_t>(bf16_t* p, const float* v) {
-    float t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = v[j];
-    VecIO<bf16_t, 8>::store(p, t);
+    typedef float f8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    *reinterpret_cast<b8*>(p) = __builtin_convertvector((f8){v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}, b8);
 }
 
-// z values of N elements into the running pair
+// N logits into the running pair; m in the logits' units, l in units of exp2(c m).  A NaN reaches the sum, whatever the maximum makes of it
 template <int N> __device__ __forceinline__ void absorb(const float* v, float c, float& m, float& l) {
-    float x[N], mx = -INFINITY;
-    bool nan = false;
+    float mx = v[0];
 #pragma unroll
-    for (int j = 0; j < N; ++j) { x[j] = v[j] * c; mx = fmaxf(mx, x[j]); nan |= x[j] != x[j]; }
-    if (nan) { l = NAN; return; }                       // fmaxf drops a NaN: it must reach the sum
-    if (mx > m) { l *= exp2f(m - mx); m = mx; }         // m = -inf: l is 0
-    if (m == -INFINITY) return;
+    for (int j = 1; j < N; ++j) mx = fmaxf(mx, v[j]);
+    if (mx > m) { l *= __builtin_amdgcn_exp2f((m - mx) * c); m = mx; }         // m = -inf: l is 0
+    const float ref = m == -INFINITY ? 0.f : -m * c;
+    float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) l += __builtin_amdgcn_exp2f(x[j] - m);
+    for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], c, ref));
+    l += s;
 }
 
 // teacher of one row over the 64 lanes of a wavefront: reference and 1 / sum of its softmax (log2 units); false: no entry
@@ -112,17 +111,17 @@ __global__ __launch_bounds__(NT) void ds_fwd_row_kernel(DsP p) {
         if (tid < p.V - tail) { float v = to_f32(s[tail + tid]); absorb<1>(&v, p.c, m, l); }
         int i = tid;
         for (; i + 3 * NT < nvec; i += 4 * NT) {                       // four loads in flight
-            float v[4][VEC];
+            float v[4 * VEC];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) vload<T>(s + head + (long)(i + u * NT) * VEC, v[u]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) absorb<VEC>(v[u], p.c, m, l);
+            for (int u = 0; u < 4; ++u) vload<T>(s + head + (long)(i + u * NT) * VEC, v + u * VEC);
+            absorb<4 * VEC>(v, p.c, m, l);
         }
         for (; i < nvec; i += NT) {
             float v[VEC];
             vload<T>(s + head + (long)i * VEC, v);
             absorb<VEC>(v, p.c, m, l);
         }
+        m *= p.c;
         for (int o = 32; o > 0; o >>= 1) { const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64); join(m, l, m2, l2); }
         if (lane == 0) { red[0][wv] = m; red[1][wv] = l; }
         __syncthreads();

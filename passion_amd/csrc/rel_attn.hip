@@ -75,10 +75,10 @@ __global__ __launch_bounds__(256) void rel_combine_kernel(RelP p) {
     if (d == 0 && p.lse) p.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
-// ... of many splits (few rows): a workgroup a row, 8 groups of 32 lanes take every eighth split, joined in order
+// ... of many splits (few rows): a workgroup a row, 32 groups of 32 lanes take every 32nd split, joined in order
 template <typename T>
-__global__ __launch_bounds__(256) void rel_combine_row_kernel(RelP p) {
-    __shared__ float red[8][32 * 4 + 4];
+__global__ __launch_bounds__(1024) void rel_combine_row_kernel(RelP p) {
+    __shared__ float red[32][32 * 4 + 4];
     const long rows = (long)p.B * p.H * p.Nq, row = blockIdx.x;
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, d = lane * 4;
     float M = -INFINITY;
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void rel_combine_row_kernel(RelP p) {
     float L = 0.f;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = g; s < p.nsplit; s += 8) {
+    for (int s = g; s < p.nsplit; s += 32) {
         const float w = __builtin_amdgcn_exp2f(p.pm[s * rows + row] - ref);
         L = __builtin_fmaf(w, p.pl[s * rows + row], L);
         if (d < p.D) {
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void rel_combine_row_kernel(RelP p) {
     L = 0.f;
     a = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 32; ++i) {
         L += red[i][128];
 #pragma unroll
         for (int j = 0; j < 4; ++j) a[j] += red[i][d + j];
@@ -124,7 +124,7 @@ struct FoldP { const float* slab; float* G; void* dt; long len, lim; int tdt, B,
 template <bool LINE_>
 __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, o = blockIdx.x * 64 + lane, h = blockIdx.y;
+    const int lane = threadIdx.x & 63, run = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), o = blockIdx.x * 64 + lane, h = blockIdx.y;
     float s = 0.f;
     if constexpr (LINE_) {
         const long n = (long)f.B * f.tiles;
@@ -139,13 +139,21 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
         const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
         const int dx = o % sx - (f.gw - 1), dy = o / sx % sy - (f.gh - 1), dz = o / sx / sy - (f.gd - 1);
         const int a0 = (int)((long)f.QC * run / 16), a1 = (int)((long)f.QC * (run + 1) / 16);
-        for (int z = 0; z < f.parts; ++z) {
-            const float* m = f.slab + ((long)z * f.H + h) * f.QC * (long)f.ld;
-#pragma unroll 4
-            for (int a = a0; a < a1; ++a) {
-                const int t = (int)(((long)f.q0 + a) % f.vol), qx = t % f.gw, qy = t / f.gw % f.gh, qz = t / f.gw / f.gh;
-                const int x = qx - dx, y = qy - dy, zz = qz - dz, c = (zz * f.gh + y) * f.gw + x;
-                if (o < f.nd && (unsigned)x < (unsigned)f.gw && (unsigned)y < (unsigned)f.gh && (unsigned)zz < (unsigned)f.gd && c < f.KC) s += m[(long)a * f.ld + c];
+        const int t = (int)(((long)f.q0 + a0) % f.vol);
+        int qx = t % f.gw, qy = t / f.gw % f.gh, qz = t / f.gw / f.gh;                  // scalar, stepped with a
+        const int shift = (dz * f.gh + dy) * f.gw + dx;                                  // of the key cell's number
+        const long part = (long)f.H * f.QC * f.ld;
+        const float* m = f.slab + ((long)h * f.QC + a0) * f.ld;
+        for (int a = a0; a < a1; ++a, m += f.ld) {
+            const int c = (qz * f.gh + qy) * f.gw + qx - shift;
+            if (o < f.nd && (unsigned)(qx - dx) < (unsigned)f.gw && (unsigned)(qy - dy) < (unsigned)f.gh && (unsigned)(qz - dz) < (unsigned)f.gd && c < f.KC)
+                for (int z = 0; z < f.parts; ++z) s += m[z * part + c];
+            if (++qx == f.gw) {
+                qx = 0;
+                if (++qy == f.gh) {
+                    qy = 0;
+                    if (++qz == f.gd) qz = 0;
+                }
             }
         }
     }
@@ -337,9 +345,9 @@ extern "C" int passion_rel_attn_fwd(const void* q, const int64_t* q_strides, con
     if ((rc = run(p, dtype, 0, pick_waves(rows32, (long)(p.pack ? p.Hkv : p.H) * p.B * p.nsplit), st))) return rc;
     if (p.nsplit > 1) {
         const long rows = (long)p.B * p.H * p.Nq;
-        if (p.nsplit > 8) {
-            if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_combine_row_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, p);
-            else hipLaunchKernelGGL(rel_combine_row_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, p);
+        if (p.nsplit > 16) {
+            if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_combine_row_kernel<bf16_t>, dim3((unsigned)rows), dim3(1024), 0, st, p);
+            else hipLaunchKernelGGL(rel_combine_row_kernel<float>, dim3((unsigned)rows), dim3(1024), 0, st, p);
         } else if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_combine_kernel<bf16_t>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
         else hipLaunchKernelGGL(rel_combine_kernel<float>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
         LAUNCH_RET();
