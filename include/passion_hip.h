@@ -492,7 +492,7 @@ int passion_topk_distill_bwd(const void* logits, int dtype, const void* values, 
 /* ---- attention with a learned relative position bias ---------------------------------------
  * The token grid form of SelfAttention (reference code/models/mmformer.py:192-227, which has learned absolute positions instead).  q (and out, dout, dq):
  * [B][Nq][H][D]; k, v (and dk, dv): [B][Nk][Hkv][D], head h reads key / value head h / (H / Hkv).  q, k, v by element strides of (batch, token, head), last dimension
- * dense, 16-byte aligned rows (-1005); all else contiguous.  f32 or bf16; D a multiple of 8 up to 128; B, H <= 65535.
+ * dense, 16-byte aligned rows, tokens (and H D) less than 2^23 elements apart (-1005); all else contiguous.  f32 or bf16; D a multiple of 8 up to 128; B, H <= 65535.
  * Token t lies at cell t mod (gd gh gw) of a raster grid, query i is token q_start + i; the pair's offset is ((dz + gd - 1)(2 gh - 1) + dy + gh - 1)(2 gw - 1) + dx + gw - 1
  * with (dz, dy, dx) = cell of the query - cell of the key, its bias table[buckets[offset]][head] (buckets NULL: the offset itself, nb = number of offsets;
  * a bucket outside [0, nb): no bias; an entry at or below -1e30: the pair is excluded).  table: [nb][H] f32 or bf16, NULL: no bias.  mask: [B][Nk], 0 = key masked (its k and v are

@@ -118,9 +118,9 @@ __global__ __launch_bounds__(1024) void rel_combine_row_kernel(RelP p) {
 
 // G[h][o]: sums by offset of the partials, 64 offsets x 16 runs of partials a workgroup, joined in order; written as the table's gradient at once where every offset is
 // its own bucket (dt).
-//   LINE: slab rows (b, key tile) of stride len, lim places each: row t holds offset o at place o - (gw - 1) - q_start + 31 + 32 t
+//   LINE: slab rows (b, key tile) of len places: row t holds offset o at place o - (gw - 1) - q_start + 32 + 32 t
 //   dense: M[z][h][a][c]: query cell a (place, coordinates uniform over the wavefront), key cell = its cell - offset where that lies on the grid
-struct FoldP { const float* slab; float* G; void* dt; long len, lim; int tdt, B, H, nd, tiles, base; int gd, gh, gw, vol, q0, QC, KC, ld, parts; };
+struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, nd, tiles, base; int gd, gh, gw, vol, q0, QC, KC, ld, parts; };
 template <bool LINE_>
 __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     __shared__ float red[16][64];
@@ -132,8 +132,8 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
 #pragma unroll 4
         for (int i = i0; i < i1; ++i) {
             const int b = i / f.tiles, t = i - b * f.tiles;
-            const long u = (long)o - f.base + 31 + 32L * t;
-            if (o < f.nd && u >= 0 && u < f.lim) s += f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + u];
+            const long u = (long)o - f.base + 32 + 32L * t;
+            if (o < f.nd && u >= 0 && u < f.len) s += f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + u];
         }
     } else {
         const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
@@ -254,7 +254,7 @@ int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int 
 long slab_floats(RelP& p, int dtype) {
     const long blk = blk_of(dtype);
     if (p.bias == 2) {
-        p.slab_len = (p.Nq + blk - 1) / blk * blk + 64;
+        p.slab_len = (p.Nq + blk - 1) / blk * blk + 32;
         return p.B * p.H * tiles32(p.Nk) * p.slab_len;
     }
     p.QC = (int)hmin(p.Nq, p.vol); p.KC = (int)hmin(p.Nk, p.vol);
@@ -289,7 +289,7 @@ Ws bwd_ws(RelP& p, int dtype, bool want_table) {
     auto take = [&](long n) { const long r = at; at += (n + 63) / 64 * 64; return r; };
     w.e = take(p.bias ? (long)p.H * p.nd : 0);
     w.delta = take((long)p.B * p.H * p.Nq);
-    if (p.bias && want_table) {
+    if (p.bias == 2 || (p.bias && want_table)) {           // (1D: the key-major kernel forms its sums on the way)
         w.slab = take(slab_floats(p, dtype));
         w.G = take(p.buckets ? (long)p.H * p.nd : 0);
     }
@@ -312,6 +312,8 @@ int strides(RelP& p, int dtype, const int64_t* sq, const int64_t* sk, const int6
         if (sq[i] % unit || sk[i] % unit || sv[i] % unit) return -1005;
         p.qs[i] = sq[i]; p.ks[i] = sk[i]; p.vs[i] = sv[i];
     }
+    for (const int64_t s : {sq[1], sk[1], sv[1], (int64_t)p.H * p.D})           // 32-bit lane offsets over a block of 64 tokens
+        if (s < 0 || s >= (1 << 23)) return -1005;
     return 0;
 }
 
@@ -371,14 +373,14 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
     const Ws w = bwd_ws(p, dtype, dtable != nullptr);
     p.delta = workspace + w.delta;
     if ((rc = pre(p, dtype, p.bias ? workspace + w.e : nullptr, st))) return rc;
-    if (dtable) p.slab = workspace + w.slab;
+    p.slab = workspace + w.slab;
     if ((rc = run(p, dtype, 1, pick_waves(tiles32(Nq), (long)H * B), st))) return rc;
     if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B), st))) return rc;
     if (dtable) {
         const long nkb = p.bias == 2 ? 0 : (p.KC + blk_of(dtype) - 1) / blk_of(dtype);
         if (p.bias != 2 && (rc = run(p, dtype, 3, pick_waves(tiles32(p.QC), nkb * H * p.parts), st))) return rc;
         float* G = workspace + w.G;
-        const FoldP f{p.slab, G, buckets ? nullptr : dtable, p.slab_len, p.slab_len - 64 + 31, table_dtype, B, H, p.nd, (int)tiles32(Nk), p.gw - 1 + p.q0, p.gd, p.gh, p.gw, p.vol, p.q0, p.QC, p.KC,
+        const FoldP f{p.slab, G, buckets ? nullptr : dtable, p.slab_len, table_dtype, B, H, p.nd, (int)tiles32(Nk), p.gw - 1 + p.q0, p.gd, p.gh, p.gw, p.vol, p.q0, p.QC, p.KC,
                       (int)(nkb * blk_of(dtype)), p.parts};
         if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<true>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
         else hipLaunchKernelGGL(rel_fold_kernel<false>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);

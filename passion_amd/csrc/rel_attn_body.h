@@ -13,9 +13,9 @@
 //          address of a score is a lane constant plus an immediate;
 //   GATHER one global read a score (L1 / L2), any grid.
 // Gradient of the table: sums of dS by offset, without atomics and in a fixed order.
-//   LINE: in the key-major kernel.  A wavefront's 32 keys x BLK queries of dS go through LDS as [key][query] and are read back along the diagonals: row kk,
-//         column (lane + kk) mod BLK, so a lane's values all belong to offset lane or lane - BLK, conflict-free.  Offsets that no later block of queries
-//         reaches (BLK a block, one aligned store) leave for a slab row of the key tile; the rest stay in a register.  (LDS float atomics into a window instead
+//   LINE: in the key-major kernel.  A wavefront's 32 keys x 32 queries of dS go through LDS as [key][query] and are read back along the diagonals: row kk at
+//         column lane - 32 + kk (zeros on either side of a row), so a lane's values belong to one offset: an LDS read with an immediate address and an add each,
+//         conflict-free.  The 32 offsets that no later tile of queries reaches leave for a slab row of the key tile in one aligned store; the rest move on.  (LDS float atomics into a window instead
 //         took 170 to 280 cycles an instruction: 3.2 ms where this kernel and its sums now take a third.)
 //   BOX, GATHER: a kernel of its own sums dS over batch and repeated cells for every pair of cells (a pair's bias is loaded once, its sum stays in a
 //         register), and the sums by offset follow from that dense matrix.
@@ -99,27 +99,36 @@ __device__ __forceinline__ void tr_product(const char* img, int stride, int r0, 
     }
 }
 
-// a tile of BLK rows x DP columns in registers, NT threads; rows past n (or masked: keep[row] = 0) and columns past D are zero
+// a tile of BLK rows x DP columns in registers, NT threads, on its way to LDS.  Loads are unconditional (rows past `last` read row `last`, columns past D read
+// column 0) from a uniform base with 32-bit lane offsets; what is not there becomes 0 when it is stored
 template <typename T, int DP, int NT> struct Tile {
-    static constexpr int CPR = DP * (int)sizeof(T) / 16, N = blk<T>() * CPR / NT;
+    static constexpr int CPR = DP * (int)sizeof(T) / 16, N = blk<T>() * CPR / NT, STEP = NT / CPR;
     u32x4 r[N];
-    __device__ __forceinline__ void fetch(const T* base, long rowstride, int row0, int n, int D, int tid) {
+    __device__ __forceinline__ void fetch(const T* base, int stride, int last, int D, int tid) {      // stride in bytes (64 rows stay below 2^31: checked by the host)
+        const int row = tid / CPR, c = (tid % CPR) * 16;
+        const unsigned col = c < D * (int)sizeof(T) ? c : 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int ci = i * NT + tid, row = ci / CPR, c = ci % CPR;
-            r[i] = (u32x4){0u, 0u, 0u, 0u};
-            if (row0 + row < n && c * 16 < D * (int)sizeof(T))
-                r[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base + (long)(row0 + row) * rowstride) + c * 16);
+        for (int i = 0; i < N; ++i)
+            r[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + ((unsigned)min(row + i * STEP, last) * (unsigned)stride + col));
+    }
+    __device__ __forceinline__ void commit(char* img, int stride, int tid, uint64_t valid, int D) const {
+        const int row = tid / CPR, c = (tid % CPR) * 16;
+        if (valid == all_rows() && D == DP) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(img + (row + i * STEP) * stride + c) = r[i];
+        } else {
+            const bool in = c < D * (int)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool ok = in && ((valid >> (row + i * STEP)) & 1);
+                *reinterpret_cast<u32x4*>(img + (row + i * STEP) * stride + c) = ok ? r[i] : (u32x4){0u, 0u, 0u, 0u};
+            }
         }
     }
-    __device__ __forceinline__ void commit(char* img, int stride, int tid, uint64_t valid) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int ci = i * NT + tid, row = ci / CPR, c = ci % CPR;
-            *reinterpret_cast<u32x4*>(img + row * stride + c * 16) = (valid >> row) & 1 ? r[i] : (u32x4){0u, 0u, 0u, 0u};
-        }
-    }
+    static __device__ __forceinline__ constexpr uint64_t all_rows() { return blk<T>() == 64 ? ~0ull : 0xffffffffull; }
 };
+// bits of the first n rows of a block
+__device__ __forceinline__ uint64_t first_rows(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // place of token t in the box of offsets (before the constant that makes differences non-negative)
 __device__ __forceinline__ int place(const RelP& p, int t) {
@@ -133,20 +142,12 @@ __device__ __forceinline__ float gather_bias(const RelP& p, int head, int o) {
     return rel_log2_bias(p.table, p.tdt, p.buckets ? p.buckets[o] : o, p.nb, head, p.H);
 }
 
-// valid keys of a block of BLK, one bit each (every wavefront forms it for itself: lanes hold one key each)
-template <int BLKN>
-__device__ __forceinline__ uint64_t valid_keys(const RelP& p, int b, int key0, int lane) {
-    const int key = key0 + lane;
-    const bool ok = lane < BLKN && key < p.Nk && (!p.mask || p.mask[(long)b * p.Nk + key]);
-    return __ballot(ok);
-}
-
 // ---------------------------------------------------------------------------------------------------------------------------------
 // query-major: MODE 0 forward (out, lse or split partials), MODE 1 backward (dQ; delta corrected in place).
 // grid (ceil(rows / (32 NW)) * nsplit, heads, B).  pack (forward, few queries): a workgroup's rows are the Nq queries of all the heads that
 // share a key / value head, so that K and V are read once for them
 template <typename T, int DP, int NW, int MODE, int BIAS>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_q_kernel(RelP p) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 || (DP == 128 && NW == 1) ? 1 : 2))) void rel_q_kernel(RelP p) {
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
     constexpr int RS = row_stride<T, DP>(), VS = MODE == 0 ? tr_stride<T, DP>() : RS;
     constexpr int KIMG = BLKN * RS, VIMG = BLKN * VS, POS = BLKN * 4, WIN = (32 * NW + BLKN) * 4;
@@ -198,14 +199,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     float l_run = 0.f, m_run = -INFINITY;               // backward: l_run sums dS
 
     Tile<T, DP, NT> kt_, vt_;
-    uint64_t vnext = 0;
+    uint64_t valid = 0;
+    bool there = false;                                        // this lane's key of the block on its way takes part
     constexpr int NWIN = (32 * NW + BLKN + NT - 1) / NT;
     float win[BIAS == LINE ? NWIN : 1];
     int kpos = 0;
     auto fetch = [&](int kb) {
-        kt_.fetch(kb_, p.ks[1], kb * BLKN, p.Nk, p.D, tid);
-        vt_.fetch(vb_, p.vs[1], kb * BLKN, p.Nk, p.D, tid);
-        vnext = valid_keys<BLKN>(p, b, kb * BLKN, lane);
+        const int key0 = kb * BLKN, last = min(p.Nk - 1 - key0, BLKN - 1);
+        kt_.fetch(kb_ + key0 * p.ks[1], (int)(p.ks[1] * sizeof(T)), last, p.D, tid);
+        vt_.fetch(vb_ + key0 * p.vs[1], (int)(p.vs[1] * sizeof(T)), last, p.D, tid);
+        there = lane <= last;
+        if (p.mask) there = there && p.mask[(long)b * p.Nk + key0 + min(lane, last)];
         if (BIAS == LINE && p.few) {                       // straight into the next buffer (last read before the previous barrier), from the table itself
             float* w = reinterpret_cast<float*>(lds + ((kb - kb0) & 1) * BUF + KIMG + VIMG);
             const int first = p.q0 - (kb * BLKN + BLKN - 1) + p.gw - 1, heads = p.pack ? rep : 1;
@@ -227,8 +231,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         if ((BIAS == BOX || BIAS == GATHER) && tid < BLKN) kpos = place(p, min(kb * BLKN + tid, p.Nk - 1));
     };
     auto commit = [&](char* buf) {
-        kt_.commit(buf, RS, tid, vnext);
-        vt_.commit(buf + KIMG, VS, tid, vnext);
+        valid = __ballot(there);                               // lanes hold a key each (BLK = 32: the upper half none: last < 32)
+        kt_.commit(buf, RS, tid, valid, p.D);
+        vt_.commit(buf + KIMG, VS, tid, valid, p.D);
         if (BIAS == LINE && !p.few) {
 #pragma unroll
             for (int i = 0; i < NWIN; ++i)
@@ -236,17 +241,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         }
         if ((BIAS == BOX || BIAS == GATHER) && tid < BLKN) reinterpret_cast<int*>(buf + KIMG + VIMG)[tid] = kpos;
     };
-    if (kb0 < kb1) {
-        fetch(kb0);
-        commit(lds);
-    }
-    uint64_t valid = vnext;
-    __syncthreads();
-
-    for (int kb = kb0; kb < kb1; ++kb) {
+    auto step = [&](int kb) {
         const char* kimg = lds + ((kb - kb0) & 1) * BUF;
         const char* vimg = kimg + KIMG;
-        if (kb + 1 < kb1) fetch(kb + 1);
         if (valid && wave_on) {
             f32x16 st[KT];
 #pragma unroll
@@ -276,7 +273,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                         }
                     }
                 }
-            if (valid != (BLKN == 64 ? ~0ull : 0xffffffffull)) {
+            if (valid != Tile<T, DP, NT>::all_rows()) {
                 const uint64_t vh = valid >> (4 * h);
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
@@ -315,35 +312,47 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) tr_product<T, ND>(vimg, VS, kt * 32, st[kt], o, lane);
             } else {
-                f32x16 ds[KT];
+                // a row of dS sums to 0; what it sums to instead is the error of delta, which was formed from the rounded out.  One block of keys (few keys: there it
+                // shows): measured first and taken off; else by the kernels that follow, through the corrected delta
+                if (nblk_all == 1) {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        f32x16 dp = zero16();
+#pragma unroll
+                        for (int s = 0; s < NCH; ++s) dp = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], dp);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) l_run = __builtin_fmaf(__builtin_amdgcn_exp2f(st[kt][r] - lse2), dp[r] - dlt, l_run);
+                    }
+                    dlt += half_sum(l_run);
+                    l_run = 0.f;
+                }
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    ds[kt] = zero16();
+                    f32x16 dp = zero16();
 #pragma unroll
-                    for (int s = 0; s < NCH; ++s) ds[kt] = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], ds[kt]);
+                    for (int s = 0; s < NCH; ++s) dp = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], dp);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        st[kt][r] = __builtin_amdgcn_exp2f(st[kt][r] - lse2);
-                        ds[kt][r] = st[kt][r] * (ds[kt][r] - dlt);
-                        l_run += ds[kt][r];
+                        dp[r] = __builtin_amdgcn_exp2f(st[kt][r] - lse2) * (dp[r] - dlt);
+                        l_run += dp[r];
                     }
+                    tr_product<T, ND>(kimg, RS, kt * 32, dp, o, lane);
                 }
-                // a row of dS sums to 0; what it sums to instead is the error of delta, which was formed from the rounded out.  One block of keys: taken off here
-                // (few keys: there it shows); else by the kernels that follow, through the corrected delta
-                if (nblk_all == 1) {
-                    const float off = half_sum(l_run);
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) ds[kt][r] = __builtin_fmaf(-off, st[kt][r], ds[kt][r]);
-                }
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) tr_product<T, ND>(kimg, RS, kt * 32, ds[kt], o, lane);
             }
         }
-        if (kb + 1 < kb1) commit(lds + ((kb + 1 - kb0) & 1) * BUF);
-        valid = vnext;
+    };
+    // (the last block apart: a load that may or may not be waited for later costs a wait for everything at the loop's top)
+    if (kb0 < kb1) {
+        fetch(kb0);
+        commit(lds);
         __syncthreads();
+        for (int kb = kb0; kb + 1 < kb1; ++kb) {
+            fetch(kb + 1);
+            step(kb);
+            commit(lds + ((kb + 1 - kb0) & 1) * BUF);
+            __syncthreads();
+        }
+        step(kb1 - 1);
     }
 
     if (MODE == 0) {
@@ -421,12 +430,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     }
     const int ak = (BIAS == BOX || BIAS == GATHER) ? p.omax - place(p, keyc) : 0;
     float* tab = reinterpret_cast<float*>(lds + 2 * BUF);               // BOX
-    // LINE: dS of this wavefront as [key][query], rows of BLK + 4 (b128 writes of 16 keys cover the banks once)
-    constexpr int SK = BLKN + 4;
-    float* skew = reinterpret_cast<float*>(lds + 2 * BUF) + wv * 32 * SK;
-    float now = 0.f, before = 0.f;                                      // running sums: offsets that began with this block of queries / with the one before
-    const bool sums = BIAS == LINE && p.slab;
-    const bool keys_all = __ballot(kok) == ~0ull;
+    // LINE: dS of this wavefront, 32 keys x 32 queries as [key][query], rows of 36 zeros + 32 values (b128 writes of 16 keys cover the banks once; what is read
+    // before or behind a row's values is 0)
+    constexpr int SK = 68, SKEW = 32 * SK + 36;
+    float* skew = reinterpret_cast<float*>(lds + 2 * BUF) + wv * SKEW;
+    float run = 0.f;                                                    // running sum of offset (query tile) - (key tile) + lane - 32
+    if (BIAS == LINE)
+        for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
     const int ktile = blockIdx.x * NW + wv, ktiles = (p.Nk + 31) / 32;
     const bool any = __syncthreads_or(kok);                             // a workgroup whose keys are all masked has only zeros to store
 
@@ -440,9 +450,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     constexpr int NWIN = (32 * NW + BLKN + NT - 1) / NT;
     float win[BIAS == LINE ? NWIN : 1];
     auto fetch = [&](int it) {
-        const int head = hk * rep + it / nqb, q0 = (it % nqb) * BLKN;
-        qt_.fetch(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)head * p.qs[2], p.qs[1], q0, p.Nq, p.D, tid);
-        dt_.fetch(static_cast<const T*>(p.dout) + ((long)b * p.Nq * p.H + head) * p.D, (long)p.H * p.D, q0, p.Nq, p.D, tid);
+        const int head = hk * rep + it / nqb, q0 = (it % nqb) * BLKN, last = min(p.Nq - 1 - q0, BLKN - 1);
+        qt_.fetch(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)head * p.qs[2] + q0 * p.qs[1], (int)(p.qs[1] * sizeof(T)), last, p.D, tid);
+        dt_.fetch(static_cast<const T*>(p.dout) + (((long)b * p.Nq + q0) * p.H + head) * p.D, p.H * p.D * (int)sizeof(T), last, p.D, tid);
         if (tid < BLKN) {
             const bool ok = q0 + tid < p.Nq;
             const long lrow = ((long)b * p.H + head) * p.Nq + q0 + tid;
@@ -459,9 +469,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             }
         }
     };
-    auto commit = [&](char* buf) {
-        qt_.commit(buf, RS, tid, ~0ull);
-        dt_.commit(buf + IMG, RS, tid, ~0ull);
+    auto commit = [&](char* buf, int it) {
+        const uint64_t valid = first_rows(p.Nq - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows();
+        qt_.commit(buf, RS, tid, valid, p.D);
+        dt_.commit(buf + IMG, RS, tid, valid, p.D);
         float* side = reinterpret_cast<float*>(buf + 2 * IMG);
         if (tid < BLKN) {
             side[tid] = lr;
@@ -474,92 +485,91 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 if (i * NT + tid < 32 * NW + BLKN) side[2 * BLKN + i * NT + tid] = win[i];
         }
     };
-    if (!any && sums && ktile < ktiles)                                 // its slab rows are folded all the same
+    if (BIAS == LINE && !any && ktile < ktiles)                         // its slab rows are folded all the same
         for (int g = 0; g < rep; ++g) {
             float* row = p.slab + (((long)b * p.H + hk * rep + g) * ktiles + ktile) * p.slab_len;
-            for (int i = lane; i < nqb * BLKN + 31; i += 64) row[i] = 0.f;
+            for (int i = lane; i < p.slab_len; i += 64) row[i] = 0.f;
         }
-    if (any) {
-        fetch(0);
-        commit(lds);
-        for (int it = 0; it < steps; ++it) {
+    auto step = [&](int it) {
+        const int head = hk * rep + it / nqb;
+        const char* qimg = lds + (it & 1) * BUF;
+        const char* dimg = qimg + IMG;
+        const float* lsev = reinterpret_cast<const float*>(qimg + 2 * IMG);
+        const float* dltv = lsev + BLKN;
+        const float* wl = lsev + 2 * BLKN + (32 * NW - 1 - (wv * 32 + (lane & 31)) + 4 * h);
+        f32x16 sa[KT], da[KT];                                           // S and dP of the whole block first: the matrix pipe works on while the vector pipe starts
+#pragma unroll
+        for (int qt = 0; qt < KT; ++qt) {
+            sa[qt] = da[qt] = zero16();
+#pragma unroll
+            for (int s = 0; s < NCH; ++s) {
+                sa[qt] = dot<T>(row_frag<T>(qimg, RS, qt * 32, s, lane), kf[s], sa[qt]);
+                da[qt] = dot<T>(row_frag<T>(dimg, RS, qt * 32, s, lane), vf[s], da[qt]);
+            }
+        }
+#pragma unroll
+        for (int qt = 0; qt < KT; ++qt) {
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const int r0 = qt * 32 + 8 * g4 + 4 * h;
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(lsev + r0), d4 = *reinterpret_cast<const f32x4*>(dltv + r0);
+                int4 qp;
+                if (BIAS == BOX || BIAS == GATHER) qp = *reinterpret_cast<const int4*>(lsev + 2 * BLKN + r0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 4 * g4 + j;
+                    float x;
+                    if (BIAS == NONE) x = __builtin_fmaf(sa[qt][r], p.c, -l4[j]);
+                    else {
+                        const int o_ = ak + (j == 0 ? qp.x : j == 1 ? qp.y : j == 2 ? qp.z : qp.w);
+                        const float bias = BIAS == LINE ? wl[qt * 32 + 8 * g4 + j] : BIAS == BOX ? tab[o_] : gather_bias(p, head, o_);
+                        x = __builtin_fmaf(sa[qt][r], p.c, bias) - l4[j];
+                    }
+                    const float pr = __builtin_amdgcn_exp2f(x);
+                    sa[qt][r] = pr * (da[qt][r] - d4[j]);               // dS
+                    da[qt][r] = pr;                                     // P   (a lane's columns are its own key's: a masked key's are not stored)
+                }
+                if (BIAS == LINE) {
+                    const f32x4 v = {sa[qt][4 * g4], sa[qt][4 * g4 + 1], sa[qt][4 * g4 + 2], sa[qt][4 * g4 + 3]};
+                    *reinterpret_cast<f32x4*>(skew + (lane & 31) * SK + 36 + 8 * g4 + 4 * h) = kok ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
+                }
+            }
+            tr_product<T, ND>(dimg, RS, qt * 32, da[qt], dv, lane);
+            tr_product<T, ND>(qimg, RS, qt * 32, sa[qt], dk, lane);
+            if (BIAS == LINE) {
+                // along the diagonals: lane l takes query - key = l - 32 of every key kk.  The lower half's offsets end with this tile of queries, the upper half's
+                // are the lower half's of the next one
+#pragma unroll
+                for (int kk = 0; kk < 32; ++kk) run += skew[kk * (SK + 1) + 4 + lane];
+                const int q0 = (it % nqb) * BLKN + qt * 32;
+                float* row = p.slab + (((long)b * p.H + head) * ktiles + min(ktile, ktiles - 1)) * p.slab_len + q0;
+                const bool end = qt == KT - 1 && (it + 1) % nqb == 0;
+                if (ktile < ktiles && (lane < 32 || end)) row[lane] = run;
+                const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(run), 0u, false, false);
+                run = end ? 0.f : __uint_as_float(sw[1]);
+            }
+        }
+    };
+    auto table_of = [&](int it) {                                          // BOX: the next head's table (the step before ended on a barrier)
+        if (BIAS == BOX && it % nqb == 0) {
             const int head = hk * rep + it / nqb;
-            if (BIAS == BOX && it % nqb == 0)                              // the next head's table (the last step ended on a barrier)
-                for (int i = tid; i < p.nd; i += NT) tab[i] = p.e[(long)head * p.nd + i];
-            if (it == 0 || (BIAS == BOX && it % nqb == 0)) __syncthreads();
-            const char* qimg = lds + (it & 1) * BUF;
-            const char* dimg = qimg + IMG;
-            const float* lsev = reinterpret_cast<const float*>(qimg + 2 * IMG);
-            const float* dltv = lsev + BLKN;
-            const float* wl = lsev + 2 * BLKN + (32 * NW - 1 - (wv * 32 + (lane & 31)) + 4 * h);
-            if (it + 1 < steps) fetch(it + 1);
-#pragma unroll
-            for (int qt = 0; qt < KT; ++qt) {
-                f32x16 sa = zero16(), da = zero16();
-#pragma unroll
-                for (int s = 0; s < NCH; ++s) {
-                    sa = dot<T>(row_frag<T>(qimg, RS, qt * 32, s, lane), kf[s], sa);
-                    da = dot<T>(row_frag<T>(dimg, RS, qt * 32, s, lane), vf[s], da);
-                }
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) {
-                    const int r0 = qt * 32 + 8 * g4 + 4 * h;
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(lsev + r0), d4 = *reinterpret_cast<const f32x4*>(dltv + r0);
-                    int4 qp;
-                    if (BIAS == BOX || BIAS == GATHER) qp = *reinterpret_cast<const int4*>(lsev + 2 * BLKN + r0);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * g4 + j;
-                        float x;
-                        if (BIAS == NONE) x = sa[r] * p.c;
-                        else {
-                            const int o_ = ak + (j == 0 ? qp.x : j == 1 ? qp.y : j == 2 ? qp.z : qp.w);
-                            const float bias = BIAS == LINE ? wl[qt * 32 + 8 * g4 + j] : BIAS == BOX ? tab[o_] : gather_bias(p, head, o_);
-                            x = __builtin_fmaf(sa[r], p.c, bias);
-                        }
-                        const float pr = __builtin_amdgcn_exp2f(x - l4[j]);
-                        sa[r] = pr * (da[r] - d4[j]);                   // dS
-                        da[r] = pr;                                     // P   (a lane's columns are its own key's: a masked key's are not stored)
-                    }
-                }
-                if (sums) {
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4) {
-                        f32x4 v = {sa[4 * g4], sa[4 * g4 + 1], sa[4 * g4 + 2], sa[4 * g4 + 3]};
-                        if (!keys_all) v = kok ? v : (f32x4){0.f, 0.f, 0.f, 0.f};       // (uniform test)
-                        *reinterpret_cast<f32x4*>(skew + (lane & 31) * SK + qt * 32 + 8 * g4 + 4 * h) = v;
-                    }
-                }
-                tr_product<T, ND>(dimg, RS, qt * 32, da, dv, lane);
-                tr_product<T, ND>(qimg, RS, qt * 32, sa, dk, lane);
-            }
-            if (sums) {
-                // column (lane + kk) mod BLK of row kk: query - key = lane, or lane - BLK once it has wrapped around (then it continues the block before)
-                const int l = lane & (BLKN - 1);
-                constexpr int ROWS = BLKN == 64 ? 32 : 16;                  // BLK = 32: the two halves of the wavefront take 16 keys each
-                const int kk0 = BLKN == 64 ? 0 : 16 * h;
-#pragma unroll
-                for (int t = 0; t < ROWS; ++t) {
-                    const int kk = kk0 + t;
-                    const float v = skew[kk * SK + ((l + kk) & (BLKN - 1))];
-                    const bool wrapped = l + kk >= BLKN;
-                    now += wrapped ? 0.f : v;
-                    before += wrapped ? v : 0.f;
-                }
-                const float a = BLKN == 64 ? now : half_sum(now), c = BLKN == 64 ? before : half_sum(before);
-                const bool whole = l + 31 < BLKN;                           // no key of the tile wraps: the offset ends with this block
-                if (ktile < ktiles) {
-                    float* row = p.slab + (((long)b * p.H + head) * ktiles + ktile) * p.slab_len + (it % nqb) * BLKN;
-                    if (lane < BLKN) row[whole ? l + 31 : l + 31 - BLKN] = whole ? a : c;
-                    if ((it + 1) % nqb == 0 && lane < BLKN && !whole) row[l + 31] = a;       // the head's last block: what would have gone on
-                }
-                const bool end = (it + 1) % nqb == 0;
-                before = (whole || end || (BLKN == 32 && h)) ? 0.f : a;
-                now = 0.f;
-            }
-            if (it + 1 < steps) commit(lds + ((it + 1) & 1) * BUF);
+            for (int i = tid; i < p.nd; i += NT) tab[i] = p.e[(long)head * p.nd + i];
             __syncthreads();
         }
+    };
+    if (any) {
+        fetch(0);
+        commit(lds, 0);
+        __syncthreads();
+        for (int it = 0; it + 1 < steps; ++it) {
+            table_of(it);
+            fetch(it + 1);
+            step(it);
+            commit(lds + ((it + 1) & 1) * BUF, it + 1);
+            __syncthreads();
+        }
+        table_of(steps - 1);
+        step(steps - 1);
     }
     if (key < p.Nk) {
         const long at = (((long)b * p.Nk + key) * p.Hkv + hk) * p.D;
@@ -607,44 +617,43 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     u32x4 qf[NCH], df[NCH];
     float lse2 = INFINITY, dlt = 0.f;
     Tile<T, DP, NT> kt_, vt_;
-    uint64_t vnext = 0, valid;
+    uint64_t valid = 0;
+    bool there = false;
     auto fetch = [&](int t) {
-        const int b = t / (MQ * MK), j0 = (t % MK) * p.KC + c0, n = min(p.Nk, (t % MK + 1) * p.KC);
-        kt_.fetch(static_cast<const T*>(p.k) + (long)b * p.ks[0] + (long)hk * p.ks[2], p.ks[1], j0, n, p.D, tid);
-        vt_.fetch(static_cast<const T*>(p.v) + (long)b * p.vs[0] + (long)hk * p.vs[2], p.vs[1], j0, n, p.D, tid);
-        const int key = j0 + lane;
-        vnext = __ballot(lane < BLKN && key < n && (!p.mask || p.mask[(long)b * p.Nk + key]));
+        // (a copy of the cells may end before this block of them does: its rows are then the last token's, and none is valid)
+        const int b = t / (MQ * MK), j0 = min((t % MK) * p.KC + c0, p.Nk - 1), n = min(p.Nk, (t % MK + 1) * p.KC) - ((t % MK) * p.KC + c0), last = max(0, min(n, BLKN) - 1);
+        kt_.fetch(static_cast<const T*>(p.k) + (long)b * p.ks[0] + (long)hk * p.ks[2] + j0 * p.ks[1], (int)(p.ks[1] * sizeof(T)), last, p.D, tid);
+        vt_.fetch(static_cast<const T*>(p.v) + (long)b * p.vs[0] + (long)hk * p.vs[2] + j0 * p.vs[1], (int)(p.vs[1] * sizeof(T)), last, p.D, tid);
+        there = lane < min(n, BLKN);
+        if (p.mask) there = there && p.mask[(long)b * p.Nk + j0 + min(lane, last)];
     };
-    if (t0 < t1) {
-        fetch(t0);
-        kt_.commit(lds, RS, tid, vnext);
-        vt_.commit(lds + IMG, RS, tid, vnext);
-    }
-    valid = vnext;
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
+    auto commit = [&](char* buf) {
+        valid = __ballot(there);
+        kt_.commit(buf, RS, tid, valid, p.D);
+        vt_.commit(buf + IMG, RS, tid, valid, p.D);
+    };
+    auto step = [&](int t) {
         const char* kimg = lds + ((t - t0) & 1) * BUF;
-        if (t + 1 < t1) fetch(t + 1);
         if (t == t0 || t % MK == 0) {                              // the next (batch, query copy)
-            const int b = t / (MQ * MK), i = (t / MK) % MQ * p.QC + a;
+            const int b = t / (MQ * MK), i = (t / MK) % MQ * p.QC + a, ic = min(i, p.Nq - 1);
             const bool qok = a < p.QC && i < p.Nq;
-            const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)i * p.qs[1] + (long)head * p.qs[2]);
-            const char* dp = reinterpret_cast<const char*>(static_cast<const T*>(p.dout) + (((long)b * p.Nq + i) * p.H + head) * p.D);
+            const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)ic * p.qs[1] + (long)head * p.qs[2]);
+            const char* dp = reinterpret_cast<const char*>(static_cast<const T*>(p.dout) + (((long)b * p.Nq + ic) * p.H + head) * p.D);
 #pragma unroll
             for (int s = 0; s < NCH; ++s) {
-                qf[s] = df[s] = (u32x4){0u, 0u, 0u, 0u};
-                if (qok && 32 * s + 16 * h < p.D * (int)sizeof(T)) {
-                    qf[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s + 16 * h);
-                    df[s] = *reinterpret_cast<const u32x4*>(dp + 32 * s + 16 * h);
-                }
+                const bool in = 32 * s + 16 * h < p.D * (int)sizeof(T);
+                const int col = in ? 32 * s + 16 * h : 0;
+                const u32x4 u = *reinterpret_cast<const u32x4*>(qp + col), w = *reinterpret_cast<const u32x4*>(dp + col), zero = {0u, 0u, 0u, 0u};
+                qf[s] = qok && in ? u : zero;
+                df[s] = qok && in ? w : zero;
             }
-            const long lrow = ((long)b * p.H + head) * p.Nq + i;
+            const long lrow = ((long)b * p.H + head) * p.Nq + ic;
             lse2 = qok ? p.lse[lrow] : INFINITY;
             dlt = qok ? p.delta[lrow] : 0.f;
         }
         if (valid) {
             const uint64_t vh = valid >> (4 * h);
-            const bool full = valid == (BLKN == 64 ? ~0ull : 0xffffffffull);
+            const bool full = valid == Tile<T, DP, NT>::all_rows();
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 f32x16 st = zero16(), dp = zero16();
@@ -661,12 +670,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 }
             }
         }
-        if (t + 1 < t1) {
-            kt_.commit(lds + ((t + 1 - t0) & 1) * BUF, RS, tid, vnext);
-            vt_.commit(lds + ((t + 1 - t0) & 1) * BUF + IMG, RS, tid, vnext);
-        }
-        valid = vnext;
+    };
+    if (t0 < t1) {
+        fetch(t0);
+        commit(lds);
         __syncthreads();
+        for (int t = t0; t + 1 < t1; ++t) {
+            fetch(t + 1);
+            step(t);
+            commit(lds + ((t + 1 - t0) & 1) * BUF);
+            __syncthreads();
+        }
+        step(t1 - 1);
     }
     if (a < p.QC) {
         float* dst = p.slab + (((long)blockIdx.z * p.H + head) * p.QC + a) * ((long)nkb * BLKN) + c0 + 4 * h;
@@ -700,7 +715,7 @@ int launch_k(const RelP& p, hipStream_t st) {
     constexpr int BLKN = blk<T>(), RS = row_stride<T, DP>();
     int bytes = 2 * (2 * BLKN * RS + 2 * BLKN * 4 + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
     if (BIAS == BOX) bytes += p.nd * 4;
-    if (BIAS == LINE && p.slab) bytes += NW * 32 * (BLKN + 4) * 4;
+    if (BIAS == LINE) bytes += NW * (32 * 68 + 36) * 4;
     const int rc = grant_lds(rel_k_kernel<T, DP, NW, BIAS>, bytes);
     if (rc) return rc;
     hipLaunchKernelGGL((rel_k_kernel<T, DP, NW, BIAS>), dim3((p.Nk + 32 * NW - 1) / (32 * NW), p.Hkv, p.B), dim3(64 * NW), bytes, st, p);

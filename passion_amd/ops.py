@@ -1828,9 +1828,9 @@ def relative_buckets(grid, num_buckets, max_distance=128, device=None):
 
 
 def _rel_view(t):
-    """t as the kernels read it: dense last dimension, rows on 16-byte points; a copy where it is not"""
+    """t as the kernels read it: dense last dimension, rows on 16-byte points, tokens less than 2^23 elements apart; a copy where it is not"""
     a, b, c, d = t.stride()
-    if d != 1 or (a | b | c) % (16 // t.element_size()) or t.data_ptr() % 16:
+    if d != 1 or b >= 2 ** 23 or (a | b | c) % (16 // t.element_size()) or t.data_ptr() % 16:
         return _dense(t)
     return t
 
@@ -1852,7 +1852,7 @@ def rel_attention(q, k, v, table=None, grid=None, buckets=None, key_mask=None, s
         raise ValueError(f"rel_attention: dtypes {q.dtype}, {k.dtype}, {v.dtype}")
     if D < 8 or D > 128 or D % 8:
         raise ValueError(f"rel_attention: head width {D} (a multiple of 8 up to 128)")
-    if H < 1 or Hkv < 1 or H % Hkv or H > 65535 or B > 65535 or max(Nq, Nk) > 2 ** 30:
+    if H < 1 or Hkv < 1 or H % Hkv or H > 65535 or H * D >= 2 ** 23 or B > 65535 or max(Nq, Nk) > 2 ** 30:
         raise ValueError(f"rel_attention: {B} x {H} heads on {Hkv} key / value heads, {Nq} x {Nk} tokens")
     q_start = int(q_start)
     if not 0 <= q_start <= 2 ** 30:
