@@ -129,11 +129,14 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     if constexpr (LINE_) {
         const long n = (long)f.B * f.tiles;
         const int i0 = (int)(n * run / 16), i1 = (int)(n * (run + 1) / 16);
-#pragma unroll 4
+// (loads unconditional, eight in flight: a load under a condition is waited for before the next one)
+#pragma unroll 8
         for (int i = i0; i < i1; ++i) {
             const int b = i / f.tiles, t = i - b * f.tiles;
             const long u = (long)o - f.base + 32 + 32L * t;
-            if (o < f.nd && u >= 0 && u < f.len) s += f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + u];
+            const bool in = u >= 0 && u < f.len;
+            const float v = f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + (in ? u : 0)];
+            s += in ? v : 0.f;
         }
     } else {
         const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
@@ -144,16 +147,19 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
         const int shift = (dz * f.gh + dy) * f.gw + dx;                                  // of the key cell's number
         const long part = (long)f.H * f.QC * f.ld;
         const float* m = f.slab + ((long)h * f.QC + a0) * f.ld;
-        for (int a = a0; a < a1; ++a, m += f.ld) {
-            const int c = (qz * f.gh + qy) * f.gw + qx - shift;
-            if (o < f.nd && (unsigned)(qx - dx) < (unsigned)f.gw && (unsigned)(qy - dy) < (unsigned)f.gh && (unsigned)(qz - dz) < (unsigned)f.gd && c < f.KC)
-                for (int z = 0; z < f.parts; ++z) s += m[z * part + c];
-            if (++qx == f.gw) {
-                qx = 0;
-                if (++qy == f.gh) {
-                    qy = 0;
-                    if (++qz == f.gd) qz = 0;
-                }
+        for (int z = 0; z < f.parts; ++z) {
+            int x = qx, y = qy, w = qz;
+            const float* row = m + z * part;
+#pragma unroll 8
+            for (int a = a0; a < a1; ++a, row += f.ld) {
+                const int c = (w * f.gh + y) * f.gw + x - shift;
+                const bool in = (unsigned)(x - dx) < (unsigned)f.gw && (unsigned)(y - dy) < (unsigned)f.gh && (unsigned)(w - dz) < (unsigned)f.gd && c < f.KC;
+                const float v = row[in ? c : 0];
+                s += in ? v : 0.f;
+                const bool cx = x + 1 == f.gw, cy = cx && y + 1 == f.gh, cw = cy && w + 1 == f.gd;
+                x = cx ? 0 : x + 1;
+                y = cy ? 0 : cx ? y + 1 : y;
+                w = cw ? 0 : cy ? w + 1 : w;
             }
         }
     }
@@ -176,7 +182,11 @@ __global__ __launch_bounds__(256) void rel_bucket_few_kernel(const float* G, con
     __shared__ float red[4];
     const int c = blockIdx.x, h = blockIdx.y;
     float s = 0.f;
-    for (int o = threadIdx.x; o < nd; o += 256) s += buckets[o] == c ? G[(long)h * nd + o] : 0.f;
+#pragma unroll 8
+    for (int o = threadIdx.x; o < nd; o += 256) {
+        const float v = G[(long)h * nd + o];
+        s += buckets[o] == c ? v : 0.f;
+    }
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();

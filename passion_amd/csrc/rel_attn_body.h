@@ -34,10 +34,15 @@ constexpr float LAZY = 8.0f;           // log2 units by which a block must excee
 enum { NONE = 0, BOX = 1, LINE = 2, GATHER = 3 };
 
 template <typename T> constexpr int blk() { return sizeof(T) == 2 ? 64 : 32; }                       // rows staged a step
-// (registers: widths above 64 and f32 need the 512 of one wavefront a SIMD)
-template <typename T, int DP> constexpr int row_stride() { return DP * (int)sizeof(T) + 16; }        // row reads: 16 rows hit 16 bank groups
-// image that is only read transposed: bf16 wants 4 consecutive rows' 64 bytes in disjoint 16-bank windows (stride mod 256 = 64 or 192)
-template <typename T, int DP> constexpr int tr_stride() { return sizeof(T) == 4 ? DP * 4 + 16 : DP == 32 ? 64 : DP * 2 + 64; }
+
+// LDS images: rows of DP elements without padding, the 16-byte chunks of a row permuted by its number (chunk c of row r lies at place c ^ swz(r)), so that both ways of
+// reading are free of bank conflicts: 16 rows at one column (row fragments: 16 places), and 64 bytes of 4 consecutive rows (transposed fragments: 4 windows).  (Rows
+// padded by 16 bytes for the first way met 2- to 4-way conflicts the second way.)
+template <int BYTES> __device__ __forceinline__ int swz(int row) {
+    if constexpr (BYTES >= 256) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (BYTES == 128) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+}
 
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
@@ -65,39 +70,82 @@ template <typename T> __device__ __forceinline__ f32x16 dot(u32x4 a, u32x4 b, f3
         return acc;
     }
 }
-// row fragment: lane (row r0 + (l & 31), half l >> 5), 16-byte chunk ch
-template <typename T> __device__ __forceinline__ u32x4 row_frag(const char* img, int stride, int r0, int ch, int lane) {
-    return *reinterpret_cast<const u32x4*>(img + (r0 + (lane & 31)) * stride + 32 * ch + 16 * (lane >> 5));
-}
-// out[dt] += (image rows r0 .. r0 + 31, columns 32 dt ..)^T . acc, acc an accumulator tile whose rows are those image rows
-template <typename T, int ND>
-__device__ __forceinline__ void tr_product(const char* img, int stride, int r0, const f32x16& acc, f32x16 (&out)[ND], int lane) {
-    if constexpr (sizeof(T) == 2) {
-        const int n = lane & 15, g = lane >> 4, h = g >> 1, q4 = n >> 2, pq = n & 3;
-        const char* base = img + (r0 + 4 * h + q4) * stride + (16 * (g & 1) + 4 * pq) * 2;
+// out[dt] += (image rows r0 .. r0 + 31, columns 32 dt ..)^T . acc, acc an accumulator tile whose rows are those image rows (r0 a multiple of 32).  AHEAD: the image's
+// fragments are requested by load(), ahead of the arithmetic that forms acc; else by product() as it goes (kernels that have no registers left; f32)
+template <typename T, int DP, bool AHEAD> struct TrFrags {
+    static constexpr int ND = DP / 32, STRIDE = DP * (int)sizeof(T);
+    bf16x8 a[AHEAD ? 2 : 1][AHEAD ? ND : 1];
+    const char* base;
+    int q4, x;
+    __device__ __forceinline__ bf16x8 frag(int s, int dt, int lane) const {
+        s16x4 part[2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            bf16x8 b;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = (__bf16)acc[8 * s + j];
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) {
-                const char* p0 = base + 16 * s * stride + dt * 64;
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p0));
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p0 + 8 * stride));
-                const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, out[dt], 0, 0, 0);
-            }
+        for (int hi = 0; hi < 2; ++hi) {
+            // row 16 s + 8 hi + 4 h + q4, chunk 4 dt + x: its place from swz() of that row
+            const int grp = STRIDE == 256 ? dt ^ q4 : STRIDE == 128 ? dt ^ (q4 >> 1) : 0;
+            const char* p = base + (16 * s + 8 * hi) * STRIDE + (grp << 6) + ((x ^ (2 * hi)) << 4);
+            part[hi] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p));
         }
-    } else {
-        const char* base = img + (r0 + 4 * (lane >> 5)) * stride + (lane & 31) * 4;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt)
-                out[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(base + ((r & 3) + 8 * (r >> 2)) * stride + dt * 128), acc[r], out[dt], 0, 0, 0);
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
-}
+    __device__ __forceinline__ void load(const char* img, int r0, int lane) {
+        if constexpr (sizeof(T) == 2) {
+            const int n = lane & 15, g = lane >> 4, h = g >> 1, pq = n & 3;
+            q4 = n >> 2;
+            x = (2 * (g & 1) + (pq >> 1)) ^ h;
+            base = img + (r0 + 4 * h + q4) * STRIDE + (pq & 1) * 8;
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int dt = 0; dt < ND; ++dt) a[s][dt] = frag(s, dt, lane);
+            }
+        } else base = img + (r0 + 4 * (lane >> 5)) * STRIDE;
+    }
+    __device__ __forceinline__ void product(const f32x16& acc, f32x16 (&out)[ND], int lane) const {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                bf16x8 b;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[j] = (__bf16)acc[8 * s + j];
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) {
+                    bf16x8 f;
+                    if constexpr (AHEAD) f = a[s][dt];
+                    else f = frag(s, dt, lane);
+                    out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, b, out[dt], 0, 0, 0);
+                }
+            }
+        } else {
+            const int h = lane >> 5, col = lane & 31;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) {
+                    const int row = (r & 3) + 8 * (r >> 2) + 4 * h, c = 8 * dt + (col >> 2);
+                    const float v = *reinterpret_cast<const float*>(base + ((r & 3) + 8 * (r >> 2)) * STRIDE + ((c ^ swz<STRIDE>(row)) << 4) + (col & 3) * 4);
+                    out[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, acc[r], out[dt], 0, 0, 0);
+                }
+        }
+    }
+};
+// the row fragments of image rows r0 .. r0 + 31 (lane: row r0 + (l & 31), half l >> 5 of every 32 bytes)
+template <typename T, int DP> struct RowFrags {
+    static constexpr int STRIDE = DP * (int)sizeof(T), N = STRIDE / 32;
+    u32x4 a[N];
+    __device__ __forceinline__ void load(const char* img, int r0, int lane) {
+        const char* row = img + (r0 + (lane & 31)) * STRIDE;
+        const int at = ((lane >> 5) ^ swz<STRIDE>(lane & 31)) << 4;
+#pragma unroll
+        for (int s = 0; s < N; ++s) a[s] = *reinterpret_cast<const u32x4*>(row + ((32 * s) ^ at));
+    }
+    __device__ __forceinline__ f32x16 times(const u32x4 (&b)[N], f32x16 acc) const {
+#pragma unroll
+        for (int s = 0; s < N; ++s) acc = dot<T>(a[s], b[s], acc);
+        return acc;
+    }
+};
 
 // a tile of BLK rows x DP columns in registers, NT threads, on its way to LDS.  Loads are unconditional (rows past `last` read row `last`, columns past D read
 // column 0) from a uniform base with 32-bit lane offsets; what is not there becomes 0 when it is stored
@@ -111,18 +159,16 @@ template <typename T, int DP, int NT> struct Tile {
         for (int i = 0; i < N; ++i)
             r[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + ((unsigned)min(row + i * STEP, last) * (unsigned)stride + col));
     }
-    __device__ __forceinline__ void commit(char* img, int stride, int tid, uint64_t valid, int D) const {
-        const int row = tid / CPR, c = (tid % CPR) * 16;
-        if (valid == all_rows() && D == DP) {
+    __device__ __forceinline__ void commit(char* img, int tid, uint64_t valid, int D) const {
+        constexpr int STRIDE = DP * (int)sizeof(T);
+        const int row = tid / CPR, c = tid % CPR;
+        const bool whole = valid == all_rows() && D == DP, in = c * 16 < D * (int)sizeof(T);
 #pragma unroll
-            for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(img + (row + i * STEP) * stride + c) = r[i];
-        } else {
-            const bool in = c < D * (int)sizeof(T);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const bool ok = in && ((valid >> (row + i * STEP)) & 1);
-                *reinterpret_cast<u32x4*>(img + (row + i * STEP) * stride + c) = ok ? r[i] : (u32x4){0u, 0u, 0u, 0u};
-            }
+        for (int i = 0; i < N; ++i) {
+            const int at = row + i * STEP;
+            u32x4 v = r[i];
+            if (!whole) v = in && ((valid >> at) & 1) ? v : (u32x4){0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4*>(img + at * STRIDE + ((c ^ swz<STRIDE>(at)) << 4)) = v;
         }
     }
     static __device__ __forceinline__ constexpr uint64_t all_rows() { return blk<T>() == 64 ? ~0ull : 0xffffffffull; }
@@ -149,8 +195,8 @@ __device__ __forceinline__ float gather_bias(const RelP& p, int head, int o) {
 template <typename T, int DP, int NW, int MODE, int BIAS>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 || (DP == 128 && NW == 1) ? 1 : 2))) void rel_q_kernel(RelP p) {
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
-    constexpr int RS = row_stride<T, DP>(), VS = MODE == 0 ? tr_stride<T, DP>() : RS;
-    constexpr int KIMG = BLKN * RS, VIMG = BLKN * VS, POS = BLKN * 4, WIN = (32 * NW + BLKN) * 4;
+    constexpr int KIMG = BLKN * DP * (int)sizeof(T), VIMG = KIMG, POS = BLKN * 4, WIN = (32 * NW + BLKN) * 4;
+    constexpr bool AHEAD = sizeof(T) == 2 && DP <= 64;              // fragments requested ahead: where 256 registers hold them
     // few queries (LINE): a window a head of the tile, BLK + Nq values each
     const int wrow = BLKN + p.Nq, BUF = KIMG + VIMG + (BIAS == LINE ? (p.few ? (p.pack ? p.H / p.Hkv : 1) * wrow * 4 + 15 & ~15 : WIN) : BIAS == NONE ? 0 : POS);
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -169,7 +215,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
     const int kb0 = (int)((long)split * nblk_all / p.nsplit), kb1 = (int)((long)(split + 1) * nblk_all / p.nsplit);
     const long orow = ((long)b * p.Nq + qi) * p.H + head, lrow = ((long)b * p.H + head) * p.Nq + qi;
 
-    u32x4 qf[NCH], df[MODE == 1 ? NCH : 1];
+    u32x4 qf[NCH], df[NCH];
     {
         const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)qi * p.qs[1] + (long)head * p.qs[2]);
         const char* dp = MODE == 1 ? reinterpret_cast<const char*>(static_cast<const T*>(p.dout) + orow * p.D) : nullptr;
@@ -232,8 +278,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
     };
     auto commit = [&](char* buf) {
         valid = __ballot(there);                               // lanes hold a key each (BLK = 32: the upper half none: last < 32)
-        kt_.commit(buf, RS, tid, valid, p.D);
-        vt_.commit(buf + KIMG, VS, tid, valid, p.D);
+        kt_.commit(buf, tid, valid, p.D);
+        vt_.commit(buf + KIMG, tid, valid, p.D);
         if (BIAS == LINE && !p.few) {
 #pragma unroll
             for (int i = 0; i < NWIN; ++i)
@@ -245,43 +291,63 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         const char* kimg = lds + ((kb - kb0) & 1) * BUF;
         const char* vimg = kimg + KIMG;
         if (valid && wave_on) {
-            f32x16 st[KT];
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                st[kt] = zero16();
-#pragma unroll
-                for (int s = 0; s < NCH; ++s) st[kt] = dot<T>(row_frag<T>(kimg, RS, kt * 32, s, lane), qf[s], st[kt]);
-            }
-            // ---- scores in log2 units: scale * log2(e) * s + bias
+            // scores of 32 keys in log2 units: scale * log2(e) * s + bias, -inf where the key does not take part
             const float* wl = reinterpret_cast<const float*>(vimg + VIMG) + (p.few ? (p.pack ? rowc / p.Nq : 0) * wrow + qi : 32 * wv + (lane & 31)) + BLKN - 1 - 4 * h;
+            const bool full = valid == Tile<T, DP, NT>::all_rows();
+            const uint64_t vh = valid >> (4 * h);
+            auto bias_of = [&](int kt) {                        // requested together, ahead of the products where registers allow
+                f32x16 e = zero16();
+                if (BIAS == NONE) return e;
+                int4 kp[4];
+                if (BIAS == BOX || BIAS == GATHER) {
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+                    for (int g4 = 0; g4 < 4; ++g4) kp[g4] = *reinterpret_cast<const int4*>(vimg + VIMG + (kt * 32 + 8 * g4 + 4 * h) * 4);
+                }
 #pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) {
-                    int off[4];
-                    if (BIAS == BOX || BIAS == GATHER) {
-                        const int4 kp = *reinterpret_cast<const int4*>(vimg + VIMG + (kt * 32 + 8 * g4 + 4 * h) * 4);
-                        off[0] = aq - kp.x; off[1] = aq - kp.y; off[2] = aq - kp.z; off[3] = aq - kp.w;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * g4 + j;
-                        if (BIAS == NONE) st[kt][r] *= p.c;
-                        else {
-                            const float bias = BIAS == LINE ? wl[-(kt * 32 + 8 * g4 + j)] : BIAS == BOX ? tab[off[j]] : gather_bias(p, head, off[j]);
-                            st[kt][r] = __builtin_fmaf(st[kt][r], p.c, bias);
-                        }
+                for (int r = 0; r < 16; ++r) {
+                    const int g4 = r >> 2, j = r & 3;
+                    if (BIAS == LINE) e[r] = wl[-(kt * 32 + 8 * g4 + j)];
+                    else {
+                        const int off = aq - (j == 0 ? kp[g4].x : j == 1 ? kp[g4].y : j == 2 ? kp[g4].z : kp[g4].w);
+                        e[r] = BIAS == BOX ? tab[off] : gather_bias(p, head, off);
                     }
                 }
-            if (valid != Tile<T, DP, NT>::all_rows()) {
-                const uint64_t vh = valid >> (4 * h);
+                return e;
+            };
+            auto finish = [&](f32x16 st, f32x16 e, int kt) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int r = 0; r < 16; ++r) st[r] = BIAS == NONE ? st[r] * p.c : __builtin_fmaf(st[r], p.c, e[r]);
+                if (!full) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (!((vh >> (kt * 32 + (r & 3) + 8 * (r >> 2))) & 1)) st[kt][r] = -INFINITY;
-            }
+                        if (!((vh >> (kt * 32 + (r & 3) + 8 * (r >> 2))) & 1)) st[r] = -INFINITY;
+                }
+                return st;
+            };
             if (MODE == 0) {
+                f32x16 st[KT];
+                RowFrags<T, DP> kf[KT];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) kf[kt].load(kimg, kt * 32, lane);
+                f32x16 e[KT];
+                if (AHEAD) {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) e[kt] = bias_of(kt);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) st[kt] = kf[kt].times(qf, zero16());
+                TrFrags<T, DP, AHEAD> vf[KT];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) vf[kt].load(vimg, kt * 32, lane);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    if (!AHEAD) {
+                        e[kt] = bias_of(kt);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    st[kt] = finish(st[kt], e[kt], kt);
+                }
                 float mx = -INFINITY;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
@@ -310,33 +376,53 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
                     }
                 l_run += psum;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) tr_product<T, ND>(vimg, VS, kt * 32, st[kt], o, lane);
+                for (int kt = 0; kt < KT; ++kt) vf[kt].product(st[kt], o, lane);
             } else {
                 // a row of dS sums to 0; what it sums to instead is the error of delta, which was formed from the rounded out.  One block of keys (few keys: there it
                 // shows): measured first and taken off; else by the kernels that follow, through the corrected delta
+                // scores and dP - delta (delta is where the product starts from)
+                auto tile = [&](int kt, f32x16& st, f32x16& dp) {
+                    RowFrags<T, DP> kf, vf;
+                    kf.load(kimg, kt * 32, lane);
+                    vf.load(vimg, kt * 32, lane);
+                    f32x16 e;
+                    if (AHEAD) {
+                        e = bias_of(kt);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[r] = -dlt;
+                    st = kf.times(qf, zero16());
+                    dp = vf.times(df, dp);
+                    if (!AHEAD) {
+                        e = bias_of(kt);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    st = finish(st, e, kt);
+                };
                 if (nblk_all == 1) {
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt) {
-                        f32x16 dp = zero16();
+                        f32x16 st, dp;
+                        tile(kt, st, dp);
 #pragma unroll
-                        for (int s = 0; s < NCH; ++s) dp = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], dp);
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) l_run = __builtin_fmaf(__builtin_amdgcn_exp2f(st[kt][r] - lse2), dp[r] - dlt, l_run);
+                        for (int r = 0; r < 16; ++r) l_run = __builtin_fmaf(__builtin_amdgcn_exp2f(st[r] - lse2), dp[r], l_run);
                     }
                     dlt += half_sum(l_run);
                     l_run = 0.f;
                 }
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    f32x16 dp = zero16();
-#pragma unroll
-                    for (int s = 0; s < NCH; ++s) dp = dot<T>(row_frag<T>(vimg, RS, kt * 32, s, lane), df[s], dp);
+                    f32x16 st, dp;
+                    tile(kt, st, dp);
+                    TrFrags<T, DP, AHEAD> kt2;
+                    kt2.load(kimg, kt * 32, lane);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        dp[r] = __builtin_amdgcn_exp2f(st[kt][r] - lse2) * (dp[r] - dlt);
+                        dp[r] *= __builtin_amdgcn_exp2f(st[r] - lse2);
                         l_run += dp[r];
                     }
-                    tr_product<T, ND>(kimg, RS, kt * 32, dp, o, lane);
+                    kt2.product(dp, o, lane);
                 }
             }
         }
@@ -406,8 +492,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
 template <typename T, int DP, int NW, int BIAS>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_k_kernel(RelP p) {
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
-    constexpr int RS = row_stride<T, DP>(), IMG = BLKN * RS, WIN = (32 * NW + BLKN) * 4;
+    constexpr int IMG = BLKN * DP * (int)sizeof(T), WIN = (32 * NW + BLKN) * 4;
     constexpr int BUF = 2 * IMG + 2 * BLKN * 4 + (BIAS == LINE ? WIN : BIAS == NONE ? 0 : BLKN * 4);
+    constexpr bool AHEAD = sizeof(T) == 2 && DP != 64;               // (width 64: two wavefronts a SIMD leave no registers for it)
     extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][Q image | dO image | lse | delta | window or places], BOX: the table
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
     const int hk = blockIdx.y, b = blockIdx.z, rep = p.H / p.Hkv;
@@ -457,7 +544,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             const bool ok = q0 + tid < p.Nq;
             const long lrow = ((long)b * p.H + head) * p.Nq + q0 + tid;
             lr = ok ? p.lse[lrow] : INFINITY;                           // queries past the end: p = 0
-            tr = ok ? p.delta[lrow] : 0.f;
+            tr = ok ? -p.delta[lrow] : 0.f;
             if (BIAS == BOX || BIAS == GATHER) qpos = place(p, p.q0 + min(q0 + tid, p.Nq - 1));
         }
         if (BIAS == LINE) {
@@ -471,8 +558,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     };
     auto commit = [&](char* buf, int it) {
         const uint64_t valid = first_rows(p.Nq - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows();
-        qt_.commit(buf, RS, tid, valid, p.D);
-        dt_.commit(buf + IMG, RS, tid, valid, p.D);
+        qt_.commit(buf, tid, valid, p.D);
+        dt_.commit(buf + IMG, tid, valid, p.D);
         float* side = reinterpret_cast<float*>(buf + 2 * IMG);
         if (tid < BLKN) {
             side[tid] = lr;
@@ -497,50 +584,72 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         const float* lsev = reinterpret_cast<const float*>(qimg + 2 * IMG);
         const float* dltv = lsev + BLKN;
         const float* wl = lsev + 2 * BLKN + (32 * NW - 1 - (wv * 32 + (lane & 31)) + 4 * h);
-        f32x16 sa[KT], da[KT];                                           // S and dP of the whole block first: the matrix pipe works on while the vector pipe starts
+        f32x16 sa[KT], da[KT];                                           // S and dP - delta of the whole block first: the matrix pipe works on while the vector pipe starts
 #pragma unroll
         for (int qt = 0; qt < KT; ++qt) {
-            sa[qt] = da[qt] = zero16();
+            RowFrags<T, DP> qa, oa;
+            qa.load(qimg, qt * 32, lane);
+            oa.load(dimg, qt * 32, lane);
 #pragma unroll
-            for (int s = 0; s < NCH; ++s) {
-                sa[qt] = dot<T>(row_frag<T>(qimg, RS, qt * 32, s, lane), kf[s], sa[qt]);
-                da[qt] = dot<T>(row_frag<T>(dimg, RS, qt * 32, s, lane), vf[s], da[qt]);
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(dltv + qt * 32 + 8 * g4 + 4 * h);       // -delta
+#pragma unroll
+                for (int j = 0; j < 4; ++j) da[qt][4 * g4 + j] = d4[j];
             }
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+            sa[qt] = qa.times(kf, zero16());
+            da[qt] = oa.times(vf, da[qt]);
         }
 #pragma unroll
         for (int qt = 0; qt < KT; ++qt) {
+            TrFrags<T, DP, AHEAD> td, tq;
+            td.load(dimg, qt * 32, lane);
+            tq.load(qimg, qt * 32, lane);
+            // what the 16 scores of a lane need from LDS, requested together (a read at a time would be waited for at a time)
+            f32x16 e = zero16(), l = zero16();
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int r0 = qt * 32 + 8 * g4 + 4 * h;
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(lsev + r0), d4 = *reinterpret_cast<const f32x4*>(dltv + r0);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(lsev + r0);
                 int4 qp;
                 if (BIAS == BOX || BIAS == GATHER) qp = *reinterpret_cast<const int4*>(lsev + 2 * BLKN + r0);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = 4 * g4 + j;
-                    float x;
-                    if (BIAS == NONE) x = __builtin_fmaf(sa[qt][r], p.c, -l4[j]);
-                    else {
-                        const int o_ = ak + (j == 0 ? qp.x : j == 1 ? qp.y : j == 2 ? qp.z : qp.w);
-                        const float bias = BIAS == LINE ? wl[qt * 32 + 8 * g4 + j] : BIAS == BOX ? tab[o_] : gather_bias(p, head, o_);
-                        x = __builtin_fmaf(sa[qt][r], p.c, bias) - l4[j];
-                    }
-                    const float pr = __builtin_amdgcn_exp2f(x);
-                    sa[qt][r] = pr * (da[qt][r] - d4[j]);               // dS
-                    da[qt][r] = pr;                                     // P   (a lane's columns are its own key's: a masked key's are not stored)
+                    l[r] = l4[j];
+                    if (BIAS == NONE) continue;
+                    const int o_ = ak + (j == 0 ? qp.x : j == 1 ? qp.y : j == 2 ? qp.z : qp.w);
+                    e[r] = BIAS == LINE ? wl[qt * 32 + 8 * g4 + j] : BIAS == BOX ? tab[o_] : gather_bias(p, head, o_);
                 }
-                if (BIAS == LINE) {
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float x = BIAS == NONE ? __builtin_fmaf(sa[qt][r], p.c, -l[r]) : __builtin_fmaf(sa[qt][r], p.c, e[r]) - l[r];
+                const float pr = __builtin_amdgcn_exp2f(x);
+                sa[qt][r] = pr * da[qt][r];                             // dS
+                da[qt][r] = pr;                                         // P   (a lane's columns are its own key's: a masked key's are not stored)
+            }
+            if (BIAS == LINE) {
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
                     const f32x4 v = {sa[qt][4 * g4], sa[qt][4 * g4 + 1], sa[qt][4 * g4 + 2], sa[qt][4 * g4 + 3]};
                     *reinterpret_cast<f32x4*>(skew + (lane & 31) * SK + 36 + 8 * g4 + 4 * h) = kok ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
                 }
             }
-            tr_product<T, ND>(dimg, RS, qt * 32, da[qt], dv, lane);
-            tr_product<T, ND>(qimg, RS, qt * 32, sa[qt], dk, lane);
+            float diag[BIAS == LINE ? 32 : 1];
             if (BIAS == LINE) {
                 // along the diagonals: lane l takes query - key = l - 32 of every key kk.  The lower half's offsets end with this tile of queries, the upper half's
                 // are the lower half's of the next one
 #pragma unroll
-                for (int kk = 0; kk < 32; ++kk) run += skew[kk * (SK + 1) + 4 + lane];
+                for (int kk = 0; kk < 32; ++kk) diag[kk] = skew[kk * (SK + 1) + 4 + lane];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            td.product(da[qt], dv, lane);
+            tq.product(sa[qt], dk, lane);
+            if (BIAS == LINE) {
+#pragma unroll
+                for (int kk = 0; kk < 32; ++kk) run += diag[kk];
                 const int q0 = (it % nqb) * BLKN + qt * 32;
                 float* row = p.slab + (((long)b * p.H + head) * ktiles + min(ktile, ktiles - 1)) * p.slab_len + q0;
                 const bool end = qt == KT - 1 && (it + 1) % nqb == 0;
@@ -597,7 +706,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_d_kernel(RelP p) {
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32;
-    constexpr int RS = row_stride<T, DP>(), IMG = BLKN * RS, BUF = 2 * IMG;
+    constexpr int IMG = BLKN * DP * (int)sizeof(T), BUF = 2 * IMG;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
     const int nkb = (p.KC + BLKN - 1) / BLKN, head = blockIdx.y, hk = head / (p.H / p.Hkv);
@@ -629,8 +738,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     };
     auto commit = [&](char* buf) {
         valid = __ballot(there);
-        kt_.commit(buf, RS, tid, valid, p.D);
-        vt_.commit(buf + IMG, RS, tid, valid, p.D);
+        kt_.commit(buf, tid, valid, p.D);
+        vt_.commit(buf + IMG, tid, valid, p.D);
     };
     auto step = [&](int t) {
         const char* kimg = lds + ((t - t0) & 1) * BUF;
@@ -656,15 +765,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             const bool full = valid == Tile<T, DP, NT>::all_rows();
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                f32x16 st = zero16(), dp = zero16();
+                RowFrags<T, DP> kf, vf;
+                kf.load(kimg, kt * 32, lane);
+                vf.load(kimg + IMG, kt * 32, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                f32x16 st = zero16(), dp;
 #pragma unroll
-                for (int s = 0; s < NCH; ++s) {
-                    st = dot<T>(row_frag<T>(kimg, RS, kt * 32, s, lane), qf[s], st);
-                    dp = dot<T>(row_frag<T>(kimg + IMG, RS, kt * 32, s, lane), df[s], dp);
-                }
+                for (int r = 0; r < 16; ++r) dp[r] = -dlt;
+                st = kf.times(qf, st);
+                dp = vf.times(df, dp);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], p.c, bias[kt][r]) - lse2) * (dp[r] - dlt);
+                    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], p.c, bias[kt][r]) - lse2) * dp[r];
                     if (!full) v = (vh >> (kt * 32 + (r & 3) + 8 * (r >> 2))) & 1 ? v : 0.f;
                     acc[kt][r] += v;
                 }
@@ -700,8 +812,8 @@ template <typename K> int grant_lds(K kern, int bytes) {
 
 template <typename T, int DP, int NW, int MODE, int BIAS>
 int launch_q(const RelP& p, hipStream_t st) {
-    constexpr int BLKN = blk<T>(), RS = row_stride<T, DP>(), VS = MODE == 0 ? tr_stride<T, DP>() : RS;
-    int bytes = 2 * (BLKN * (RS + VS) + (BIAS == LINE ? (p.few ? (p.pack ? p.H / p.Hkv : 1) * (BLKN + p.Nq) * 4 + 15 & ~15 : (32 * NW + BLKN) * 4) : BIAS == NONE ? 0 : BLKN * 4));
+    constexpr int BLKN = blk<T>();
+    int bytes = 2 * (2 * BLKN * DP * (int)sizeof(T) + (BIAS == LINE ? (p.few ? (p.pack ? p.H / p.Hkv : 1) * (BLKN + p.Nq) * 4 + 15 & ~15 : (32 * NW + BLKN) * 4) : BIAS == NONE ? 0 : BLKN * 4));
     if (BIAS == BOX) bytes += p.nd * 4;
     const int rc = grant_lds(rel_q_kernel<T, DP, NW, MODE, BIAS>, bytes);
     if (rc) return rc;
@@ -712,8 +824,8 @@ int launch_q(const RelP& p, hipStream_t st) {
 }
 template <typename T, int DP, int NW, int BIAS>
 int launch_k(const RelP& p, hipStream_t st) {
-    constexpr int BLKN = blk<T>(), RS = row_stride<T, DP>();
-    int bytes = 2 * (2 * BLKN * RS + 2 * BLKN * 4 + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
+    constexpr int BLKN = blk<T>();
+    int bytes = 2 * (2 * BLKN * DP * (int)sizeof(T) + 2 * BLKN * 4 + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
     if (BIAS == BOX) bytes += p.nd * 4;
     if (BIAS == LINE) bytes += NW * (32 * 68 + 36) * 4;
     const int rc = grant_lds(rel_k_kernel<T, DP, NW, BIAS>, bytes);
@@ -725,7 +837,7 @@ int launch_k(const RelP& p, hipStream_t st) {
 
 template <typename T, int DP, int NW>
 int launch_d(const RelP& p, hipStream_t st) {
-    constexpr int BLKN = blk<T>(), bytes = 4 * BLKN * row_stride<T, DP>();
+    constexpr int BLKN = blk<T>(), bytes = 4 * BLKN * DP * (int)sizeof(T);
     const int rc = grant_lds(rel_d_kernel<T, DP, NW>, bytes);
     if (rc) return rc;
     hipLaunchKernelGGL((rel_d_kernel<T, DP, NW>), dim3((p.QC + 32 * NW - 1) / (32 * NW) * ((p.KC + BLKN - 1) / BLKN), p.H, p.parts), dim3(64 * NW), bytes, st, p);
