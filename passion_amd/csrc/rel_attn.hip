@@ -141,7 +141,14 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     } else {
         const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
         const int dx = o % sx - (f.gw - 1), dy = o / sx % sy - (f.gh - 1), dz = o / sx / sy - (f.gd - 1);
-        const int a0 = (int)((long)f.QC * run / 16), a1 = (int)((long)f.QC * (run + 1) / 16);
+        // query cells from the grid's start on: only the planes that some offset of the workgroup reaches
+        int lo = 0, hi = f.QC;
+        if (f.q0 % f.vol == 0) {
+            const int first = blockIdx.x * 64 / sx / sy - (f.gd - 1), last = min(blockIdx.x * 64 + 63, f.nd - 1) / sx / sy - (f.gd - 1);
+            lo = min(f.QC, max(0, first) * f.gh * f.gw);
+            hi = max(lo, min(f.QC, (min(0, last) + f.gd) * f.gh * f.gw));
+        }
+        const int a0 = lo + (int)((long)(hi - lo) * run / 16), a1 = lo + (int)((long)(hi - lo) * (run + 1) / 16);
         const int t = (int)(((long)f.q0 + a0) % f.vol);
         int qx = t % f.gw, qy = t / f.gw % f.gh, qz = t / f.gw / f.gh;                  // scalar, stepped with a
         const int shift = (dz * f.gh + dy) * f.gw + dx;                                  // of the key cell's number

@@ -245,15 +245,21 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
     float l_run = 0.f, m_run = -INFINITY;               // backward: l_run sums dS
 
     Tile<T, DP, NT> kt_, vt_;
-    uint64_t valid = 0;
+    uint64_t valid = 0, vnext = 0;
     bool there = false;                                        // this lane's key of the block on its way takes part
     constexpr int NWIN = (32 * NW + BLKN + NT - 1) / NT;
     float win[BIAS == LINE ? NWIN : 1];
     int kpos = 0;
+    // (width 128: the value tile follows the key tile through the same registers, half a step later)
+    constexpr bool HALVES = sizeof(T) == 2 && DP == 128;
+    auto fetch_v = [&](int kb) {
+        const int key0 = kb * BLKN, last = min(p.Nk - 1 - key0, BLKN - 1);
+        vt_.fetch(vb_ + key0 * p.vs[1], (int)(p.vs[1] * sizeof(T)), last, p.D, tid);
+    };
     auto fetch = [&](int kb) {
         const int key0 = kb * BLKN, last = min(p.Nk - 1 - key0, BLKN - 1);
         kt_.fetch(kb_ + key0 * p.ks[1], (int)(p.ks[1] * sizeof(T)), last, p.D, tid);
-        vt_.fetch(vb_ + key0 * p.vs[1], (int)(p.vs[1] * sizeof(T)), last, p.D, tid);
+        if (!HALVES) fetch_v(kb);
         there = lane <= last;
         if (p.mask) there = there && p.mask[(long)b * p.Nk + key0 + min(lane, last)];
         if (BIAS == LINE && p.few) {                       // straight into the next buffer (last read before the previous barrier), from the table itself
@@ -276,10 +282,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         }
         if ((BIAS == BOX || BIAS == GATHER) && tid < BLKN) kpos = place(p, min(kb * BLKN + tid, p.Nk - 1));
     };
+    auto commit_k = [&](char* buf) {
+        vnext = __ballot(there);                               // lanes hold a key each (BLK = 32: the upper half none: last < 32)
+        kt_.commit(buf, tid, vnext, p.D);
+    };
     auto commit = [&](char* buf) {
-        valid = __ballot(there);                               // lanes hold a key each (BLK = 32: the upper half none: last < 32)
-        kt_.commit(buf, tid, valid, p.D);
-        vt_.commit(buf + KIMG, tid, valid, p.D);
+        if (!HALVES) commit_k(buf);
+        vt_.commit(buf + KIMG, tid, vnext, p.D);
         if (BIAS == LINE && !p.few) {
 #pragma unroll
             for (int i = 0; i < NWIN; ++i)
@@ -287,10 +296,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         }
         if ((BIAS == BOX || BIAS == GATHER) && tid < BLKN) reinterpret_cast<int*>(buf + KIMG + VIMG)[tid] = kpos;
     };
-    auto step = [&](int kb) {
+    auto step = [&](int kb, auto between) {
         const char* kimg = lds + ((kb - kb0) & 1) * BUF;
         const char* vimg = kimg + KIMG;
-        if (valid && wave_on) {
+        if (!(valid && wave_on)) between();
+        else {
             // scores of 32 keys in log2 units: scale * log2(e) * s + bias, -inf where the key does not take part
             const float* wl = reinterpret_cast<const float*>(vimg + VIMG) + (p.few ? (p.pack ? rowc / p.Nq : 0) * wrow + qi : 32 * wv + (lane & 31)) + BLKN - 1 - 4 * h;
             const bool full = valid == Tile<T, DP, NT>::all_rows();
@@ -337,6 +347,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
                 }
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) st[kt] = kf[kt].times(qf, zero16());
+                between();
                 TrFrags<T, DP, AHEAD> vf[KT];
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) vf[kt].load(vimg, kt * 32, lane);
@@ -384,21 +395,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
                 auto tile = [&](int kt, f32x16& st, f32x16& dp) {
                     RowFrags<T, DP> kf, vf;
                     kf.load(kimg, kt * 32, lane);
-                    vf.load(vimg, kt * 32, lane);
-                    f32x16 e;
                     if (AHEAD) {
-                        e = bias_of(kt);
+                        vf.load(vimg, kt * 32, lane);
+                        const f32x16 e = bias_of(kt);
                         __builtin_amdgcn_sched_barrier(0);
-                    }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) dp[r] = -dlt;
-                    st = kf.times(qf, zero16());
-                    dp = vf.times(df, dp);
-                    if (!AHEAD) {
-                        e = bias_of(kt);
+                        for (int r = 0; r < 16; ++r) dp[r] = -dlt;
+                        st = kf.times(qf, zero16());
+                        dp = vf.times(df, dp);
+                        st = finish(st, e, kt);
+                    } else {                                    // (apart, so that no more than one product's fragments are held)
+                        st = kf.times(qf, zero16());
                         __builtin_amdgcn_sched_barrier(0);
+                        vf.load(vimg, kt * 32, lane);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) dp[r] = -dlt;
+                        dp = vf.times(df, dp);
+                        __builtin_amdgcn_sched_barrier(0);
+                        st = finish(st, bias_of(kt), kt);
                     }
-                    st = finish(st, e, kt);
                 };
                 if (nblk_all == 1) {
 #pragma unroll
@@ -423,6 +438,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
                         l_run += dp[r];
                     }
                     kt2.product(dp, o, lane);
+                    if (kt == 0) between();
                 }
             }
         }
@@ -430,15 +446,21 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
     // (the last block apart: a load that may or may not be waited for later costs a wait for everything at the loop's top)
     if (kb0 < kb1) {
         fetch(kb0);
+        if (HALVES) { commit_k(lds); fetch_v(kb0); }
         commit(lds);
+        valid = vnext;
         __syncthreads();
         for (int kb = kb0; kb + 1 < kb1; ++kb) {
+            char* next = lds + ((kb + 1 - kb0) & 1) * BUF;
             fetch(kb + 1);
-            step(kb);
-            commit(lds + ((kb + 1 - kb0) & 1) * BUF);
+            step(kb, [&] {
+                if (HALVES) { commit_k(next); fetch_v(kb + 1); }
+            });
+            commit(next);
+            valid = vnext;
             __syncthreads();
         }
-        step(kb1 - 1);
+        step(kb1 - 1, [] {});
     }
 
     if (MODE == 0) {
@@ -536,10 +558,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     int qpos = 0;
     constexpr int NWIN = (32 * NW + BLKN + NT - 1) / NT;
     float win[BIAS == LINE ? NWIN : 1];
+    constexpr bool HALVES = sizeof(T) == 2 && DP == 128;               // as in rel_q_kernel
+    auto fetch_d = [&](int it) {
+        const int head = hk * rep + it / nqb, q0 = (it % nqb) * BLKN, last = min(p.Nq - 1 - q0, BLKN - 1);
+        dt_.fetch(static_cast<const T*>(p.dout) + (((long)b * p.Nq + q0) * p.H + head) * p.D, p.H * p.D * (int)sizeof(T), last, p.D, tid);
+    };
     auto fetch = [&](int it) {
         const int head = hk * rep + it / nqb, q0 = (it % nqb) * BLKN, last = min(p.Nq - 1 - q0, BLKN - 1);
         qt_.fetch(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)head * p.qs[2] + q0 * p.qs[1], (int)(p.qs[1] * sizeof(T)), last, p.D, tid);
-        dt_.fetch(static_cast<const T*>(p.dout) + (((long)b * p.Nq + q0) * p.H + head) * p.D, p.H * p.D * (int)sizeof(T), last, p.D, tid);
+        if (!HALVES) fetch_d(it);
         if (tid < BLKN) {
             const bool ok = q0 + tid < p.Nq;
             const long lrow = ((long)b * p.H + head) * p.Nq + q0 + tid;
@@ -556,10 +583,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             }
         }
     };
+    auto commit_q = [&](char* buf, int it) { qt_.commit(buf, tid, first_rows(p.Nq - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows(), p.D); };
     auto commit = [&](char* buf, int it) {
-        const uint64_t valid = first_rows(p.Nq - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows();
-        qt_.commit(buf, tid, valid, p.D);
-        dt_.commit(buf + IMG, tid, valid, p.D);
+        if (!HALVES) commit_q(buf, it);
+        dt_.commit(buf + IMG, tid, first_rows(p.Nq - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows(), p.D);
         float* side = reinterpret_cast<float*>(buf + 2 * IMG);
         if (tid < BLKN) {
             side[tid] = lr;
@@ -577,7 +604,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             float* row = p.slab + (((long)b * p.H + hk * rep + g) * ktiles + ktile) * p.slab_len;
             for (int i = lane; i < p.slab_len; i += 64) row[i] = 0.f;
         }
-    auto step = [&](int it) {
+    auto step = [&](int it, auto between) {
         const int head = hk * rep + it / nqb;
         const char* qimg = lds + (it & 1) * BUF;
         const char* dimg = qimg + IMG;
@@ -657,6 +684,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(run), 0u, false, false);
                 run = end ? 0.f : __uint_as_float(sw[1]);
             }
+            if (qt == 0) between();
         }
     };
     auto table_of = [&](int it) {                                          // BOX: the next head's table (the step before ended on a barrier)
@@ -668,17 +696,21 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     };
     if (any) {
         fetch(0);
+        if (HALVES) { commit_q(lds, 0); fetch_d(0); }
         commit(lds, 0);
         __syncthreads();
         for (int it = 0; it + 1 < steps; ++it) {
+            char* next = lds + ((it + 1) & 1) * BUF;
             table_of(it);
             fetch(it + 1);
-            step(it);
-            commit(lds + ((it + 1) & 1) * BUF, it + 1);
+            step(it, [&] {
+                if (HALVES) { commit_q(next, it + 1); fetch_d(it + 1); }
+            });
+            commit(next, it + 1);
             __syncthreads();
         }
         table_of(steps - 1);
-        step(steps - 1);
+        step(steps - 1, [] {});
     }
     if (key < p.Nk) {
         const long at = (((long)b * p.Nk + key) * p.Hkv + hk) * p.D;
