@@ -119,7 +119,7 @@ __global__ __launch_bounds__(1024) void rel_combine_row_kernel(RelP p) {
 // G[h][o]: sums by offset of the partials, 64 offsets x 16 runs of partials a workgroup, joined in order; written as the table's gradient at once where every offset is
 // its own bucket (dt).
 //   LINE: slab rows (b, key tile) of len places: row t holds offset o at place o - (gw - 1) - q_start + 32 + 32 t
-//   dense: M[z][h][a][c]: query cell a (place, coordinates uniform over the wavefront), key cell = its cell - offset where that lies on the grid
+//   dense: M[z][h][a][c]: the pairs of a query cell a and the key cell = its cell - offset, where both lie on the grid
 struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, nd, tiles, base; int gd, gh, gw, vol, q0, QC, KC, ld, parts; };
 template <bool LINE_>
 __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
@@ -141,34 +141,27 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     } else {
         const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
         const int dx = o % sx - (f.gw - 1), dy = o / sx % sy - (f.gh - 1), dz = o / sx / sy - (f.gd - 1);
-        // query cells from the grid's start on: only the planes that some offset of the workgroup reaches
-        int lo = 0, hi = f.QC;
-        if (f.q0 % f.vol == 0) {
-            const int first = blockIdx.x * 64 / sx / sy - (f.gd - 1), last = min(blockIdx.x * 64 + 63, f.nd - 1) / sx / sy - (f.gd - 1);
-            lo = min(f.QC, max(0, first) * f.gh * f.gw);
-            hi = max(lo, min(f.QC, (min(0, last) + f.gd) * f.gh * f.gw));
-        }
-        const int a0 = lo + (int)((long)(hi - lo) * run / 16), a1 = lo + (int)((long)(hi - lo) * (run + 1) / 16);
-        const int t = (int)(((long)f.q0 + a0) % f.vol);
-        int qx = t % f.gw, qy = t / f.gw % f.gh, qz = t / f.gw / f.gh;                  // scalar, stepped with a
-        const int shift = (dz * f.gh + dy) * f.gw + dx;                                  // of the key cell's number
+        // units of 8 cells along x of the rows (z, y) that have a partner; the query's cell counts from q_start (the raster may begin inside the grid)
+        const int nz = f.gd - abs(dz), ny = f.gh - abs(dy), z0 = max(0, dz), y0 = max(0, dy), XC = (f.gw + 7) / 8;
+        const int shift = (dz * f.gh + dy) * f.gw + dx, n = o < f.nd ? nz * ny * XC : 0, first = f.q0 % f.vol;
         const long part = (long)f.H * f.QC * f.ld;
-        const float* m = f.slab + ((long)h * f.QC + a0) * f.ld;
-        for (int z = 0; z < f.parts; ++z) {
-            int x = qx, y = qy, w = qz;
-            const float* row = m + z * part;
-#pragma unroll 8
-            for (int a = a0; a < a1; ++a, row += f.ld) {
-                const int c = (w * f.gh + y) * f.gw + x - shift;
-                const bool in = (unsigned)(x - dx) < (unsigned)f.gw && (unsigned)(y - dy) < (unsigned)f.gh && (unsigned)(w - dz) < (unsigned)f.gd && c < f.KC;
-                const float v = row[in ? c : 0];
-                s += in ? v : 0.f;
-                const bool cx = x + 1 == f.gw, cy = cx && y + 1 == f.gh, cw = cy && w + 1 == f.gd;
-                x = cx ? 0 : x + 1;
-                y = cy ? 0 : cx ? y + 1 : y;
-                w = cw ? 0 : cy ? w + 1 : w;
+        const float* m = f.slab + (long)h * f.QC * f.ld;
+        for (int z = 0; z < f.parts; ++z, m += part)
+            for (int u = run; __any(u < n); u += 16) {
+                const int row = u / XC, x8 = (u - row * XC) * 8, rz = row / ny, ry = row - rz * ny, cell = ((z0 + rz) * f.gh + y0 + ry) * f.gw + x8;
+                float v[8];
+                bool in[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int x = x8 + i, c = cell + i - shift;
+                    int a = cell + i - first;
+                    a = a < 0 ? a + f.vol : a;
+                    in[i] = u < n && x < f.gw && (unsigned)(x - dx) < (unsigned)f.gw && a < f.QC && c < f.KC;
+                    v[i] = m[in[i] ? (long)a * f.ld + c : 0];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += in[i] ? v[i] : 0.f;
             }
-        }
     }
     red[run][lane] = s;
     __syncthreads();
