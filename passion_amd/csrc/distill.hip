@@ -104,6 +104,15 @@ __global__ __launch_bounds__(NT) void ds_fwd_row_kernel(DsP p) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     for (long row = blockIdx.x; row < p.R; row += gridDim.x) {
         const T* s = static_cast<const T*>(p.s) + row * p.V;
+        // K <= 64: the first wavefront asks for the teacher's entries and the student's logits at them before the row, and uses them behind it
+        const bool early = p.K <= 64 && wv == 0 && lane < p.K;
+        int at0 = -1;
+        float tv0 = 0.f, z0 = 0.f;
+        if (early) {
+            at0 = tidx(p, row * p.K + lane);
+            tv0 = tval(p, row * p.K + lane);
+            z0 = to_f32(s[max(at0, 0)]);
+        }
         const int head = (int)min((long)p.V, (long)(((16 - ((uintptr_t)s & 15)) & 15) / sizeof(T)));
         const int nvec = (p.V - head) / VEC, tail = head + nvec * VEC;
         float m = -INFINITY, l = 0.f;
@@ -129,21 +138,33 @@ __global__ __launch_bounds__(NT) void ds_fwd_row_kernel(DsP p) {
             m = red[0][0]; l = red[1][0];
             for (int w = 1; w < NT / 64; ++w) join(m, l, red[0][w], red[1][w]);
             const float lse = m + log2f(l);
-            float tm, inv = 0.f, acc = 0.f;
-            const bool live = teacher(p, row, lane, tm, inv);
-            if (live) {
-                const float lt = -log2f(inv);
-                for (int k = lane; k < p.K; k += 64) {
-                    const int at = tidx(p, row * p.K + k);
-                    if (at < 0) continue;
-                    const float d = tval(p, row * p.K + k) * p.c - tm, pk = exp2f(d) * inv;
-                    if (pk != 0.f) acc += pk * ((d - lt) - (to_f32(s[at]) * p.c - lse));
+            float acc = 0.f;
+            bool live;
+            if (p.K <= 64) {
+                const float t = at0 >= 0 ? tv0 * p.c : -INFINITY;
+                float tm = t;
+                for (int o = 32; o > 0; o >>= 1) { const float u = __shfl_xor(tm, o, 64); tm = u > tm || u != u ? u : tm; }
+                live = tm != -INFINITY;
+                const float e = live && at0 >= 0 ? exp2f(t - tm) : 0.f, sum = lanes_sum(e, 64), pk = e / sum;
+                if (e != 0.f) acc = pk * ((t - tm - log2f(sum)) - (z0 * p.c - lse));
+                acc = lanes_sum(acc, 64);
+            } else {
+                float tm, inv = 0.f;
+                live = teacher(p, row, lane, tm, inv);
+                if (live) {
+                    const float lt = -log2f(inv);
+                    for (int k = lane; k < p.K; k += 64) {
+                        const int at = tidx(p, row * p.K + k);
+                        if (at < 0) continue;
+                        const float d = tval(p, row * p.K + k) * p.c - tm, pk = exp2f(d) * inv;
+                        if (pk != 0.f) acc += pk * ((d - lt) - (to_f32(s[at]) * p.c - lse));
+                    }
+                    acc = wave_sum(acc);
                 }
-                acc = wave_sum(acc);
             }
             if (lane == 0) {
                 p.loss[row] = live ? p.T * p.T * LN2 * acc : 0.f;
-                if (p.lse) p.lse[row] = lse;
+                if (p.lse) p.lse[row] = live ? lse : INFINITY;           // +inf marks a row without a teacher (a finite or NaN sum never gives it)
             }
         }
         __syncthreads();
@@ -155,24 +176,20 @@ __global__ __launch_bounds__(NT) void ds_bwd_row_kernel(DsP p) {
     constexpr int VEC = 16 / sizeof(T);
     __shared__ float pk[MAX_K];
     __shared__ int at[MAX_K];
-    __shared__ int live_s;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     for (long row = blockIdx.x; row < p.R; row += gridDim.x) {
         const T* s = static_cast<const T*>(p.s) + row * p.V;
         T* o = static_cast<T*>(p.ds) + row * p.V;
-        if (wv == 0) {
-            float tm, inv = 0.f;
-            const bool live = teacher(p, row, lane, tm, inv);
-            if (lane == 0) live_s = live;
-            if (live)
-                for (int k = lane; k < p.K; k += 64) {
-                    at[k] = tidx(p, row * p.K + k);
-                    pk[k] = at[k] < 0 ? 0.f : exp2f(tval(p, row * p.K + k) * p.c - tm) * inv;
-                }
-        }
-        __syncthreads();
-        const bool live = live_s;
         const float lse = p.lse[row], f = p.g[row] * p.T;
+        const bool live = lse != INFINITY;
+        if (live && wv == NT / 64 - 1) {                 // the last wavefront, while the others stream the row; read behind the barrier below
+            float tm, inv = 0.f;
+            teacher(p, row, lane, tm, inv);
+            for (int k = lane; k < p.K; k += 64) {
+                at[k] = tidx(p, row * p.K + k);
+                pk[k] = at[k] < 0 ? 0.f : exp2f(tval(p, row * p.K + k) * p.c - tm) * inv;
+            }
+        }
         // the student's and the gradient's rows start at the same offset from a 16-byte point (both bases are aligned)
         const int head = (int)min((long)p.V, (long)(((16 - ((uintptr_t)s & 15)) & 15) / sizeof(T)));
         const int nvec = (p.V - head) / VEC, tail = head + nvec * VEC;

@@ -11,7 +11,7 @@ import torch
 
 from .. import ops
 
-__all__ = ["softmax_weighted_loss_bs", "dice_loss_bs", "temp_kl_loss_bs", "prototype_passion_loss_bs"]
+__all__ = ["softmax_weighted_loss_bs", "dice_loss_bs", "temp_kl_loss_bs", "topk_distill_loss_bs", "prototype_passion_loss_bs"]
 
 
 def _factor(up_op):
@@ -82,6 +82,14 @@ def temp_kl_loss_bs(logit_s, logit_t, target=None, num_cls=4, temp=1.0, up_op=No
     k = _factor(up_op)
     ls, lt = _NcdhwToCl.apply(logit_s.float()), ops.to_channels_last(logit_t.detach().float())
     return kl_cl(ls, ops.softmax_classes(lt, 1.0 / temp), temp, k)
+
+
+def topk_distill_loss_bs(logit_s, top_values, top_index, temp=1.0):
+    """temp_kl_loss_bs (no upsampling) against a teacher of whom only the top K logits per voxel were kept: student logits (B,C,D,H,W), top_values and
+    top_index (B,K,D,H,W) as torch.topk(teacher, K, dim=1) gives them; voxels without a teacher: index -1 throughout.  -> (B,1), mean over classes and
+    voxels as there (K = C: the same loss up to its clamps)"""
+    rows = ops.topk_distill(_NcdhwToCl.apply(logit_s.float()), top_values.detach().movedim(1, -1), top_index.movedim(1, -1), temp)
+    return rows.flatten(1).mean(1, keepdim=True) / logit_s.shape[1]
 
 
 def prototype_passion_loss_bs(feature_s, feature_t, target, logit_s=None, logit_t=None, num_cls=4, temp=1.0,
