@@ -19,7 +19,7 @@ struct RelP {
     float *po, *pm, *pl;                  // split forward: [nsplit][B][H][Nq](D), f32
     int B, Nq, Nk, H, Hkv, D;
     int gd, gh, gw, vol, nd, omax, q0, nb, tdt;
-    int bias, pack, few, nsplit;          // few: few query rows (forward), the bias read straight from the table
+    int bias, pack, few, nsplit, ksplit;  // few: few query rows (forward), the bias read straight from the table; nsplit: parts of the keys (forward, dQ); ksplit: of the queries (dK, dV)
     float c, scale;                       // c = scale * log2(e)
 };
 

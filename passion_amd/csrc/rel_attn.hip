@@ -116,27 +116,55 @@ __global__ __launch_bounds__(1024) void rel_combine_row_kernel(RelP p) {
     if (d == 0 && p.lse) p.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
+// sum of the n parts of dQ, dK or dV, in their order: 32 lanes a row, 4 columns a lane.  Nq > 0: rows (b H + h) Nq + q, and delta takes its correction, the sum of pm;
+// else rows as in out
+template <typename T>
+__global__ __launch_bounds__(256) void rel_join_kernel(const float* part, int n, long rows, int D, float scale, T* out, int Nq, int H, const float* pm, float* delta) {
+    const long row = (long)blockIdx.x * 8 + threadIdx.x / 32;
+    const int d = (threadIdx.x & 31) * 4;
+    if (row >= rows) return;
+    if (d < D) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < n; ++s) a += load4(part + (s * rows + row) * D + d);
+        long to = row;
+        if (Nq) {
+            const long bh = row / Nq, q = row % Nq, b = bh / H, h = bh % H;
+            to = (b * Nq + q) * H + h;
+        }
+        store4(out + to * D + d, (f32x4){a[0] * scale, a[1] * scale, a[2] * scale, a[3] * scale});
+    }
+    if (Nq && d == 0) {
+        float off = 0.f;
+        for (int s = 0; s < n; ++s) off += pm[s * rows + row];
+        delta[row] += off;
+    }
+}
+
 // G[h][o]: sums by offset of the partials, 64 offsets x 16 runs of partials a workgroup, joined in order; written as the table's gradient at once where every offset is
 // its own bucket (dt).
-//   LINE: slab rows (b, key tile) of len places: row t holds offset o at place o - (gw - 1) - q_start + 32 + 32 t
+//   LINE: slab rows (b, key tile, part of the queries) of len places: row t of the part that begins at query q holds offset o at place
+//         o - (gw - 1) - q_start + 32 + 32 t - q
 //   dense: M[z][h][a][c]: the pairs of a query cell a and the key cell = its cell - offset, where both lie on the grid
-struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, nd, tiles, base; int gd, gh, gw, vol, q0, QC, KC, ld, parts; };
+struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, nd, tiles, base; int gd, gh, gw, vol, q0, QC, KC, ld, parts, ksplit, klog, nqb, blk; };
 template <bool LINE_>
 __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, run = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), o = blockIdx.x * 64 + lane, h = blockIdx.y;
     float s = 0.f;
     if constexpr (LINE_) {
-        const long n = (long)f.B * f.tiles;
-        const int i0 = (int)(n * run / 16), i1 = (int)(n * (run + 1) / 16);
+        // the key tiles that may hold one of the workgroup's offsets, W of them from ta on, for every batch entry and part
+        const int W = (int)(f.len / 32) + 3, n = f.B * f.ksplit * W, i0 = (int)((long)n * run / 16), i1 = (int)((long)n * (run + 1) / 16);
+        int bp = i0 / W, j = i0 - bp * W;
 // (loads unconditional, eight in flight: a load under a condition is waited for before the next one)
 #pragma unroll 8
         for (int i = i0; i < i1; ++i) {
-            const int b = i / f.tiles, t = i - b * f.tiles;
-            const long u = (long)o - f.base + 32 + 32L * t;
-            const bool in = u >= 0 && u < f.len;
-            const float v = f.slab[(((long)b * f.H + h) * f.tiles + t) * f.len + (in ? u : 0)];
+            const int part = bp & (f.ksplit - 1), b = bp >> f.klog;
+            const int q0 = (int)((unsigned)(part * f.nqb) >> f.klog), q1 = (int)((unsigned)((part + 1) * f.nqb) >> f.klog);       // (in blocks)
+            const int from = f.base - 32 + q0 * f.blk, ta = (from - (int)blockIdx.x * 64 - 63 + 31) >> 5, t = ta + j, u = o - from + 32 * t;
+            const bool in = (unsigned)t < (unsigned)f.tiles && (unsigned)u < (unsigned)((q1 - q0) * f.blk + 32);
+            const float v = f.slab[in ? ((((long)b * f.H + h) * f.tiles + t) * f.ksplit + part) * f.len + u : 0];
             s += in ? v : 0.f;
+            if (++j == W) { j = 0; ++bp; }
         }
     } else {
         const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
@@ -230,7 +258,15 @@ int pick_split(const RelP& p, int dtype) {
     const int nblk = (p.Nk + blk_of(dtype) - 1) / blk_of(dtype);
     if (p.few) return (int)hmax(1, hmin(nblk, 2048 / tiles));
     int s = 1;
-    while (tiles * s < 1024 && nblk / (2 * s) >= 2) s *= 2;
+    while (tiles * s < 768 && nblk / (2 * s) >= 2) s *= 2;
+    return s;
+}
+// the backward's: parts (a power of two) of at least 128 of the n tokens that a wavefront walks, until there is a wavefront on three of four SIMDs.
+// Forward + backward, us, whole / in parts: 185 x 1626 tokens, 2 heads of 128, f32 555 / 220; 2 x 2774^2, 2 heads of 64 on one, f32 1495 / 571; 2258^2, 2 heads of 128 on
+// one, bf16 779 / 165; 2048^2 over 8^3 cells, 8 heads of 64, bf16 241 / 187.  Up to a wavefront on every SIMD the last is as fast, the second takes 647
+int pick_split_bwd(long tiles, int n) {
+    int s = 1;
+    while (tiles * s < 768 && n / (2 * s) >= 128) s *= 2;
     return s;
 }
 // wavefronts a workgroup: as many as leave every CU a workgroup; they share the staged tiles
@@ -255,7 +291,7 @@ int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int 
     }
     p.B = B; p.Nq = Nq; p.Nk = Nk; p.H = H; p.Hkv = Hkv; p.D = D; p.q0 = q_start; p.mask = mask;
     p.scale = scale; p.c = scale * 1.4426950408889634f;
-    p.nsplit = 1;
+    p.nsplit = p.ksplit = 1;
     p.bias = bias_mode(p);
     return 0;
 }
@@ -264,8 +300,9 @@ int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int 
 long slab_floats(RelP& p, int dtype) {
     const long blk = blk_of(dtype);
     if (p.bias == 2) {
-        p.slab_len = (p.Nq + blk - 1) / blk * blk + 32;
-        return p.B * p.H * tiles32(p.Nk) * p.slab_len;
+        const long nqb = (p.Nq + blk - 1) / blk;
+        p.slab_len = (nqb + p.ksplit - 1) / p.ksplit * blk + 32;
+        return p.B * p.H * tiles32(p.Nk) * p.ksplit * p.slab_len;
     }
     p.QC = (int)hmin(p.Nq, p.vol); p.KC = (int)hmin(p.Nk, p.vol);
     const long passes = (long)p.B * ((p.Nq + p.QC - 1) / p.QC) * ((p.Nk + p.KC - 1) / p.KC), nkb = (p.KC + blk - 1) / blk, waves = tiles32(p.QC) * nkb * p.H;
@@ -299,6 +336,11 @@ Ws bwd_ws(RelP& p, int dtype, bool want_table) {
     auto take = [&](long n) { const long r = at; at += (n + 63) / 64 * 64; return r; };
     w.e = take(p.bias ? (long)p.H * p.nd : 0);
     w.delta = take((long)p.B * p.H * p.Nq);
+    p.nsplit = pick_split_bwd(tiles32(p.Nq) * p.H * p.B, p.Nk);
+    p.ksplit = pick_split_bwd(tiles32(p.Nk) * p.Hkv * p.B, p.Nq);
+    const long rows = (long)p.B * p.H * p.Nq, krows = (long)p.B * p.Nk * p.Hkv;
+    w.po = take(hmax(p.nsplit > 1 ? p.nsplit * rows * p.D : 0, p.ksplit > 1 ? 2 * p.ksplit * krows * p.D : 0));       // dQ's parts, then those of dK and dV
+    w.pm = take(p.nsplit > 1 ? p.nsplit * rows : 0);
     if (p.bias == 2 || (p.bias && want_table)) {           // (1D: the key-major kernel forms its sums on the way)
         w.slab = take(slab_floats(p, dtype));
         w.G = take(p.buckets ? (long)p.H * p.nd : 0);
@@ -313,6 +355,13 @@ int pre(RelP& p, int dtype, float* e, hipStream_t st) {
     else hipLaunchKernelGGL(rel_pre_kernel<float>, dim3((unsigned)(eb + db)), dim3(256), 0, st, p, e, eb);
     LAUNCH_RET();
     p.e = e;
+    return 0;
+}
+int join(int dtype, const float* part, int n, long rows, int D, float scale, void* out, int Nq, int H, const float* pm, float* delta, hipStream_t st) {
+    const dim3 grid((unsigned)((rows + 7) / 8));
+    if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_join_kernel<bf16_t>, grid, dim3(256), 0, st, part, n, rows, D, scale, static_cast<bf16_t*>(out), Nq, H, pm, delta);
+    else hipLaunchKernelGGL(rel_join_kernel<float>, grid, dim3(256), 0, st, part, n, rows, D, scale, static_cast<float*>(out), Nq, H, pm, delta);
+    LAUNCH_RET();
     return 0;
 }
 bool misaligned(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0; }
@@ -384,14 +433,22 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
     p.delta = workspace + w.delta;
     if ((rc = pre(p, dtype, p.bias ? workspace + w.e : nullptr, st))) return rc;
     p.slab = workspace + w.slab;
-    if ((rc = run(p, dtype, 1, pick_waves(tiles32(Nq), (long)H * B), st))) return rc;
-    if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B), st))) return rc;
+    p.po = workspace + w.po;
+    p.pm = workspace + w.pm;
+    if ((rc = run(p, dtype, 1, pick_waves(tiles32(Nq), (long)H * B * p.nsplit), st))) return rc;
+    const long rows = (long)B * H * Nq, krows = (long)B * Nk * Hkv;
+    if (p.nsplit > 1 && (rc = join(dtype, p.po, p.nsplit, rows, D, scale, dq, Nq, H, p.pm, p.delta, st))) return rc;
+    if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B * p.ksplit), st))) return rc;
+    if (p.ksplit > 1) {
+        if ((rc = join(dtype, p.po, p.ksplit, krows, D, scale, dk, 0, 0, nullptr, nullptr, st))) return rc;
+        if ((rc = join(dtype, p.po + p.ksplit * krows * D, p.ksplit, krows, D, 1.f, dv, 0, 0, nullptr, nullptr, st))) return rc;
+    }
     if (dtable) {
         const long nkb = p.bias == 2 ? 0 : (p.KC + blk_of(dtype) - 1) / blk_of(dtype);
         if (p.bias != 2 && (rc = run(p, dtype, 3, pick_waves(tiles32(p.QC), nkb * H * p.parts), st))) return rc;
         float* G = workspace + w.G;
         const FoldP f{p.slab, G, buckets ? nullptr : dtable, p.slab_len, table_dtype, B, H, p.nd, (int)tiles32(Nk), p.gw - 1 + p.q0, p.gd, p.gh, p.gw, p.vol, p.q0, p.QC, p.KC,
-                      (int)(nkb * blk_of(dtype)), p.parts};
+                      (int)(nkb * blk_of(dtype)), p.parts, p.ksplit, __builtin_ctz(p.ksplit), (Nq + blk_of(dtype) - 1) / blk_of(dtype), blk_of(dtype)};
         if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<true>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
         else hipLaunchKernelGGL(rel_fold_kernel<false>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
         LAUNCH_RET();

@@ -498,6 +498,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
                 }
             if (h == 0 && p.lse) p.lse[lrow] = l == 0.f ? INFINITY : m_run + __builtin_amdgcn_logf(l);
         }
+    } else if (p.nsplit > 1) {                                                    // joined afterwards, delta's correction with it
+        const float off = half_sum(l_run);
+        if (qok) {
+            const long at = (long)split * p.B * p.H * p.Nq + lrow;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int d = dt * 32 + 8 * g4 + 4 * h;
+                    if (d < p.D) store4(p.po + at * p.D + d, (f32x4){o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]});
+                }
+            if (h == 0) p.pm[at] = off;
+        }
     } else {
         if (qok) {
             T* dst = static_cast<T*>(p.dq) + orow * p.D;
@@ -516,8 +529,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// key-major backward: dK, dV.  grid (ceil(Nk / (32 NW)), Hkv, B); a wavefront owns 32 keys and walks the queries of all the heads that share its
-// key / value head, BLK at a time: their gradients sum in registers
+// key-major backward: dK, dV.  grid (ceil(Nk / (32 NW)) * ksplit, Hkv, B); a wavefront owns 32 keys and walks the queries (of its part, where they are split) of all
+// the heads that share its key / value head, BLK at a time: their gradients sum in registers
 template <typename T, int DP, int NW, int BIAS>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_k_kernel(RelP p) {
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
@@ -527,9 +540,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][Q image | dO image | lse | delta | window or places], BOX: the table
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
     const int hk = blockIdx.y, b = blockIdx.z, rep = p.H / p.Hkv;
-    const int k0 = blockIdx.x * NW * 32, key = k0 + wv * 32 + (lane & 31), keyc = min(key, p.Nk - 1);
+    const int split = blockIdx.x % p.ksplit, kt0 = blockIdx.x / p.ksplit * NW, k0 = kt0 * 32, key = k0 + wv * 32 + (lane & 31), keyc = min(key, p.Nk - 1);
     const bool kok = key < p.Nk && (!p.mask || p.mask[(long)b * p.Nk + keyc]);
-    const int nqb = (p.Nq + BLKN - 1) / BLKN, steps = nqb * rep;
+    const int nqb_all = (p.Nq + BLKN - 1) / BLKN, qb0 = (int)((long)split * nqb_all / p.ksplit), nqb = (int)((long)(split + 1) * nqb_all / p.ksplit) - qb0, steps = nqb * rep;
+    const int qs0 = qb0 * BLKN;                                          // the part's first query
 
     u32x4 kf[NCH], vf[NCH];
     {
@@ -553,7 +567,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     float run = 0.f;                                                    // running sum of offset (query tile) - (key tile) + lane - 32
     if (BIAS == LINE)
         for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
-    const int ktile = blockIdx.x * NW + wv, ktiles = (p.Nk + 31) / 32;
+    const int ktile = kt0 + wv, ktiles = (p.Nk + 31) / 32;
     const bool any = __syncthreads_or(kok);                             // a workgroup whose keys are all masked has only zeros to store
 
     f32x16 dk[ND], dv[ND];
@@ -567,11 +581,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     float win[BIAS == LINE ? NWIN : 1];
     constexpr bool HALVES = sizeof(T) == 2 && DP == 128;               // as in rel_q_kernel
     auto fetch_d = [&](int it) {
-        const int head = hk * rep + it / nqb, q0 = (it % nqb) * BLKN, last = min(p.Nq - 1 - q0, BLKN - 1);
+        const int head = hk * rep + it / nqb, q0 = qs0 + (it % nqb) * BLKN, last = min(p.Nq - 1 - q0, BLKN - 1);
         dt_.fetch(static_cast<const T*>(p.dout) + (((long)b * p.Nq + q0) * p.H + head) * p.D, p.H * p.D * (int)sizeof(T), last, p.D, tid);
     };
     auto fetch = [&](int it) {
-        const int head = hk * rep + it / nqb, q0 = (it % nqb) * BLKN, last = min(p.Nq - 1 - q0, BLKN - 1);
+        const int head = hk * rep + it / nqb, q0 = qs0 + (it % nqb) * BLKN, last = min(p.Nq - 1 - q0, BLKN - 1);
         qt_.fetch(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)head * p.qs[2] + q0 * p.qs[1], (int)(p.qs[1] * sizeof(T)), last, p.D, tid);
         if (!HALVES) fetch_d(it);
         if (tid < BLKN) {
@@ -590,10 +604,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             }
         }
     };
-    auto commit_q = [&](char* buf, int it) { qt_.commit(buf, tid, first_rows(p.Nq - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows(), p.D); };
+    auto commit_q = [&](char* buf, int it) { qt_.commit(buf, tid, first_rows(p.Nq - qs0 - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows(), p.D); };
     auto commit = [&](char* buf, int it) {
         if (!HALVES) commit_q(buf, it);
-        dt_.commit(buf + IMG, tid, first_rows(p.Nq - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows(), p.D);
+        dt_.commit(buf + IMG, tid, first_rows(p.Nq - qs0 - (it % nqb) * BLKN) & Tile<T, DP, NT>::all_rows(), p.D);
         float* side = reinterpret_cast<float*>(buf + 2 * IMG);
         if (tid < BLKN) {
             side[tid] = lr;
@@ -608,7 +622,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     };
     if (BIAS == LINE && !any && ktile < ktiles)                         // its slab rows are folded all the same
         for (int g = 0; g < rep; ++g) {
-            float* row = p.slab + (((long)b * p.H + hk * rep + g) * ktiles + ktile) * p.slab_len;
+            float* row = p.slab + ((((long)b * p.H + hk * rep + g) * ktiles + ktile) * p.ksplit + split) * p.slab_len;
             for (int i = lane; i < p.slab_len; i += 64) row[i] = 0.f;
         }
     auto step = [&](int it, auto between) {
@@ -684,8 +698,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             if (BIAS == LINE) {
 #pragma unroll
                 for (int kk = 0; kk < 32; ++kk) run += diag[kk];
-                const int q0 = (it % nqb) * BLKN + qt * 32;
-                float* row = p.slab + (((long)b * p.H + head) * ktiles + min(ktile, ktiles - 1)) * p.slab_len + q0;
+                float* row = p.slab + ((((long)b * p.H + head) * ktiles + min(ktile, ktiles - 1)) * p.ksplit + split) * p.slab_len + (it % nqb) * BLKN + qt * 32;
                 const bool end = qt == KT - 1 && (it + 1) % nqb == 0;
                 if (ktile < ktiles && (lane < 32 || end)) row[lane] = run;
                 const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(run), 0u, false, false);
@@ -721,7 +734,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     }
     if (key < p.Nk) {
         const long at = (((long)b * p.Nk + key) * p.Hkv + hk) * p.D;
-        const float f = kok ? p.scale : 0.f, g = kok ? 1.f : 0.f;
+        const float f = p.ksplit > 1 ? 1.f : p.scale;
+        const long part = (long)p.B * p.Nk * p.Hkv * p.D;
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -731,7 +745,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 f32x4 a = {0.f, 0.f, 0.f, 0.f}, c = a;
                 if (kok) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) { a[j] = dk[dt][4 * g4 + j] * f; c[j] = dv[dt][4 * g4 + j] * g; }
+                    for (int j = 0; j < 4; ++j) { a[j] = dk[dt][4 * g4 + j] * f; c[j] = dv[dt][4 * g4 + j]; }
+                }
+                if (p.ksplit > 1) {
+                    store4(p.po + split * part + at + d, a);
+                    store4(p.po + (p.ksplit + split) * part + at + d, c);
+                    continue;
                 }
                 store4(static_cast<T*>(p.dk) + at + d, a);
                 store4(static_cast<T*>(p.dv) + at + d, c);
@@ -869,7 +888,7 @@ int launch_k(const RelP& p, hipStream_t st) {
     if (BIAS == LINE) bytes += NW * (32 * 68 + 36) * 4;
     const int rc = grant_lds(rel_k_kernel<T, DP, NW, BIAS>, bytes);
     if (rc) return rc;
-    hipLaunchKernelGGL((rel_k_kernel<T, DP, NW, BIAS>), dim3((p.Nk + 32 * NW - 1) / (32 * NW), p.Hkv, p.B), dim3(64 * NW), bytes, st, p);
+    hipLaunchKernelGGL((rel_k_kernel<T, DP, NW, BIAS>), dim3((p.Nk + 32 * NW - 1) / (32 * NW) * p.ksplit, p.Hkv, p.B), dim3(64 * NW), bytes, st, p);
     LAUNCH_RET();
     return 0;
 }

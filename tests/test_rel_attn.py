@@ -169,6 +169,17 @@ def test_few_queries(Nq, Nk, heads, Hkv, B, dt):
 
 
 @pytest.mark.gpu
+@BOTH
+@pytest.mark.parametrize("grid,B,Nq,Nk,heads,Hkv,D,nb,q0,mask", [((1700,), 1, 200, 1500, 2, 2, 128, 8, 190, None), ((1700,), 1, 1500, 200, 2, 1, 64, None, 0, None),
+                                                                   ((1100,), 2, 1100, 700, 2, 1, 40, 32, 0, "runs"), ((1300,), 1, 1300, 1300, 1, 1, 64, None, 0, "runs"),
+                                                                   ((300,), 3, 290, 257, 1, 1, 16, 12, 10, "empty"), ((10, 10, 10), 1, 1000, 1000, 2, 1, 96, None, 0, "runs"),
+                                                                   ((40, 40), 1, 700, 1500, 1, 1, 32, 12, 0, "random"), (None, 1, 900, 1100, 2, 1, 72, None, 0, "runs")])
+def test_few_tiles_of_long_rows(grid, B, Nq, Nk, heads, Hkv, D, nb, q0, mask, dt):
+    """the backward in parts of the keys (dQ) and of the queries (dK, dV, the table's gradient), the parts of unequal lengths, some without a valid key"""
+    _check(_make(B, Nq, Nk, heads, Hkv, D, dt, grid, nb, q0, mask))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("grid,B,heads,Hkv,D", [((7, 10, 8), 1, 8, 4, 128), ((7, 10, 8), 1, 8, 4, 96), ((6, 9, 10), 1, 8, 4, 96), ((7, 9, 9), 1, 8, 4, 128), ((560,), 4, 8, 8, 64),
                                                  ((560,), 4, 8, 2, 64), ((2, 14, 20), 3, 8, 8, 64), ((6, 10, 12), 1, 12, 12, 112)])
 def test_ragged_last_block_in_every_workgroup(grid, B, heads, Hkv, D):
