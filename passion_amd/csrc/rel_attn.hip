@@ -8,8 +8,13 @@
 //     delta_i = dout_i . out_i,  dS = p (dout v^T - delta),  dq = scale dS k,  dk = scale dS^T q,  dv = p^T dout,  dtable[c] = sum over pairs of bucket c of dS
 // The reference's SelfAttention (code/models/mmformer.py:192-227) has learned absolute positions instead; its tokens are such a grid.
 //
-// Two backward kernels as in flash_attn.hip: query-major (dq and the table's sums) and key-major (dk, dv: the heads that share a key / value head
-// sum in registers); both free of atomics between wavefronts.
+// Two backward kernels as in flash_attn.hip: query-major (dq) and key-major (dk, dv: the heads that share a key / value head sum in registers), and the table's sums
+// (rel_attn_body.h); all free of atomics.
+//
+// Bound: long sequences by the matrix pipe and the vector arithmetic per score (exponential, bias, conversions), one token by the latency of a chain of loads.  Measured, bf16:
+//   8000 x 8000 tokens, 8 heads of 128 on 4, 1D table: forward 331 us (396 TF), dq 546 (360 TF), dk / dv / diagonal sums 810 (324 TF), fold 44;
+//   4 x 2048 x 2048, 8 heads of 64, 8^3 cells, 30 % of the keys masked: forward 75, dq 85, dk / dv 93, the table's dense sums 84, fold 17 us;
+//   4 x 1 x 6000, 8 heads of 64 on 2: 10 + 6 us (12.4 MB of cache).
 #include "common.h"
 #include "passion_hip.h"
 #include "rel_attn.h"
@@ -269,10 +274,11 @@ int pick_split_bwd(long tiles, int n) {
     while (tiles * s < 768 && n / (2 * s) >= 128) s *= 2;
     return s;
 }
-// wavefronts a workgroup: as many as leave every CU a workgroup; they share the staged tiles
-int pick_waves(long rows32, long others) {
+// wavefronts a workgroup: as many as leave every CU a workgroup; they share the staged tiles.  Key-major with heads over 64 wide: LDS and registers hold one workgroup a CU,
+// and a workgroup more than there are CUs is a second round: four as soon as two would begin one (1077^2, 8 heads of 96 on 2, f32, 544 wavefronts: forward + backward 804 us by two, 481 by four)
+int pick_waves(long rows32, long others, bool alone = false) {
     const long waves = rows32 * others;
-    return rows32 >= 4 && waves >= 900 ? 4 : rows32 >= 2 && waves >= 384 ? 2 : 1;
+    return rows32 >= 4 && waves > (alone ? 512 : 899) ? 4 : rows32 >= 2 && waves > (alone ? 256 : 383) ? 2 : 1;
 }
 
 int setup(RelP& p, int dtype, int B, int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start, const void* table, int tdt, const int* buckets, int nb,
@@ -302,12 +308,12 @@ long slab_floats(RelP& p, int dtype) {
     if (p.bias == 2) {
         const long nqb = (p.Nq + blk - 1) / blk;
         p.slab_len = (nqb + p.ksplit - 1) / p.ksplit * blk + 32;
-        return p.B * p.H * tiles32(p.Nk) * p.ksplit * p.slab_len;
+        return (long)p.B * p.H * tiles32(p.Nk) * p.ksplit * p.slab_len;
     }
     p.QC = (int)hmin(p.Nq, p.vol); p.KC = (int)hmin(p.Nk, p.vol);
     const long passes = (long)p.B * ((p.Nq + p.QC - 1) / p.QC) * ((p.Nk + p.KC - 1) / p.KC), nkb = (p.KC + blk - 1) / blk, waves = tiles32(p.QC) * nkb * p.H;
     p.parts = (int)hmax(1, hmin(passes, 2048 / waves));            // about two wavefronts a SIMD
-    return p.parts * p.H * p.QC * nkb * blk;
+    return (long)p.parts * p.H * p.QC * nkb * blk;
 }
 
 int run(const RelP& p, int dtype, int what, int nw, hipStream_t st) { return dtype == PASSION_BF16 ? rel_run_bf16(p, what, nw, st) : rel_run_f32(p, what, nw, st); }
@@ -438,7 +444,7 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
     if ((rc = run(p, dtype, 1, pick_waves(tiles32(Nq), (long)H * B * p.nsplit), st))) return rc;
     const long rows = (long)B * H * Nq, krows = (long)B * Nk * Hkv;
     if (p.nsplit > 1 && (rc = join(dtype, p.po, p.nsplit, rows, D, scale, dq, Nq, H, p.pm, p.delta, st))) return rc;
-    if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B * p.ksplit), st))) return rc;
+    if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B * p.ksplit, D > 64), st))) return rc;
     if (p.ksplit > 1) {
         if ((rc = join(dtype, p.po, p.ksplit, krows, D, scale, dk, 0, 0, nullptr, nullptr, st))) return rc;
         if ((rc = join(dtype, p.po + p.ksplit * krows * D, p.ksplit, krows, D, 1.f, dv, 0, 0, nullptr, nullptr, st))) return rc;

@@ -448,3 +448,12 @@ def test_c_entry_refuses_on_the_host():
     size = lambda *a: lib.passion_rel_attn_workspace_floats(*a)
     assert size(0, 0, 1, 4, 4, 2, 2, 12, 1, 1, 4, 0, 1, 0, 7) == -1003
     assert size(1, 1, 1, 400, 400, 2, 2, 64, 1, 1, 400, 0, 1, 0, 799) > 0
+
+
+def test_workspace_sizes_past_32_bits():
+    """the partials of the table's gradient, counted on the host: products of batch, heads and lengths past 2^31"""
+    from passion_amd import _lib
+    size = lambda B, N, M, H, grid: _lib.load().passion_rel_attn_workspace_floats(1, 1, B, N, M, H, H, 8, *grid, 0, 1, 0, math.prod(2 * g - 1 for g in grid))
+    assert size(40000, 33, 33, 60000, (1, 1, 40)) >= 40000 * 60000 * 2 * (64 + 32)                    # 1D: batch x heads x key tiles x (queries in blocks + 32)
+    assert size(1, 1 << 22, 1 << 22, 1024, (4, 1, 1 << 20)) >= 1024 << 44                               # dense: heads x query cells x key cells
+    assert size(1, 1 << 22, 10, 1024, (4, 1, 1 << 20)) >= (1024 << 22) * 64
