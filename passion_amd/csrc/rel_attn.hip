@@ -12,7 +12,7 @@
 // (rel_attn_body.h); all free of atomics.
 //
 // Bound: long sequences by the matrix pipe and the vector arithmetic per score (exponential, bias, conversions), one token by the latency of a chain of loads.  Measured, bf16:
-//   8000 x 8000 tokens, 8 heads of 128 on 4, 1D table: forward 331 us (396 TF), dq 546 (360 TF), dk / dv / diagonal sums 810 (324 TF), fold 44;
+//   8000 x 8000 tokens, 8 heads of 128 on 4, 1D table: forward 331 us (792 TF), dq 546 (720 TF), dk / dv / diagonal sums 810 (647 TF), fold 44;
 //   4 x 2048 x 2048, 8 heads of 64, 8^3 cells, 30 % of the keys masked: forward 75, dq 85, dk / dv 93, the table's dense sums 84, fold 17 us;
 //   4 x 1 x 6000, 8 heads of 64 on 2: 10 + 6 us (12.4 MB of cache).
 #include "common.h"
@@ -121,10 +121,11 @@ __global__ __launch_bounds__(1024) void rel_combine_row_kernel(RelP p) {
     if (d == 0 && p.lse) p.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
-// sum of the n parts of dQ, dK or dV, in their order: 32 lanes a row, 4 columns a lane.  Nq > 0: rows (b H + h) Nq + q, and delta takes its correction, the sum of pm;
-// else rows as in out
+// sum of the n parts of dQ, or of dK and dV (grid y), in their order: 32 lanes a row, 4 columns a lane.  Nq > 0: rows (b H + h) Nq + q, and delta takes its correction, the
+// sum of pm; else rows as in out and out2 (unscaled)
 template <typename T>
-__global__ __launch_bounds__(256) void rel_join_kernel(const float* part, int n, long rows, int D, float scale, T* out, int Nq, int H, const float* pm, float* delta) {
+__global__ __launch_bounds__(256) void rel_join_kernel(const float* part, int n, long rows, int D, float scale, T* out, T* out2, int Nq, int H, const float* pm, float* delta) {
+    if (blockIdx.y) { part += n * rows * D; out = out2; scale = 1.f; }
     const long row = (long)blockIdx.x * 8 + threadIdx.x / 32;
     const int d = (threadIdx.x & 31) * 4;
     if (row >= rows) return;
@@ -363,10 +364,10 @@ int pre(RelP& p, int dtype, float* e, hipStream_t st) {
     p.e = e;
     return 0;
 }
-int join(int dtype, const float* part, int n, long rows, int D, float scale, void* out, int Nq, int H, const float* pm, float* delta, hipStream_t st) {
-    const dim3 grid((unsigned)((rows + 7) / 8));
-    if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_join_kernel<bf16_t>, grid, dim3(256), 0, st, part, n, rows, D, scale, static_cast<bf16_t*>(out), Nq, H, pm, delta);
-    else hipLaunchKernelGGL(rel_join_kernel<float>, grid, dim3(256), 0, st, part, n, rows, D, scale, static_cast<float*>(out), Nq, H, pm, delta);
+int join(int dtype, const float* part, int n, long rows, int D, float scale, void* out, void* out2, int Nq, int H, const float* pm, float* delta, hipStream_t st) {
+    const dim3 grid((unsigned)((rows + 7) / 8), out2 ? 2 : 1);
+    if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_join_kernel<bf16_t>, grid, dim3(256), 0, st, part, n, rows, D, scale, static_cast<bf16_t*>(out), static_cast<bf16_t*>(out2), Nq, H, pm, delta);
+    else hipLaunchKernelGGL(rel_join_kernel<float>, grid, dim3(256), 0, st, part, n, rows, D, scale, static_cast<float*>(out), static_cast<float*>(out2), Nq, H, pm, delta);
     LAUNCH_RET();
     return 0;
 }
@@ -443,12 +444,9 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
     p.pm = workspace + w.pm;
     if ((rc = run(p, dtype, 1, pick_waves(tiles32(Nq), (long)H * B * p.nsplit), st))) return rc;
     const long rows = (long)B * H * Nq, krows = (long)B * Nk * Hkv;
-    if (p.nsplit > 1 && (rc = join(dtype, p.po, p.nsplit, rows, D, scale, dq, Nq, H, p.pm, p.delta, st))) return rc;
+    if (p.nsplit > 1 && (rc = join(dtype, p.po, p.nsplit, rows, D, scale, dq, nullptr, Nq, H, p.pm, p.delta, st))) return rc;
     if ((rc = run(p, dtype, 2, pick_waves(tiles32(Nk), (long)Hkv * B * p.ksplit, D > 64), st))) return rc;
-    if (p.ksplit > 1) {
-        if ((rc = join(dtype, p.po, p.ksplit, krows, D, scale, dk, 0, 0, nullptr, nullptr, st))) return rc;
-        if ((rc = join(dtype, p.po + p.ksplit * krows * D, p.ksplit, krows, D, 1.f, dv, 0, 0, nullptr, nullptr, st))) return rc;
-    }
+    if (p.ksplit > 1 && (rc = join(dtype, p.po, p.ksplit, krows, D, scale, dk, dv, 0, 0, nullptr, nullptr, st))) return rc;
     if (dtable) {
         const long nkb = p.bias == 2 ? 0 : (p.KC + blk_of(dtype) - 1) / blk_of(dtype);
         if (p.bias != 2 && (rc = run(p, dtype, 3, pick_waves(tiles32(p.QC), nkb * H * p.parts), st))) return rc;
