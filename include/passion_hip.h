@@ -481,7 +481,8 @@ int passion_residual_norm_bwd(const void* x, int x_dtype, const void* h, int h_d
  * The form of temp_kl_loss_bs (reference code/utils/criterions.py:92-103) that keeps K of the teacher's V logits a row:
  * loss[r] = T^2 sum_k p_k (log p_k - log softmax(logits / T)[index_k]), p = softmax(values / T) over the row's entries with 0 <= index < V.  A row without
  * such an entry (or whose values are all -inf): loss 0, gradient 0.  logits [R][V] f32 / bf16, values [R][K] f32 / bf16, index [R][K] int32 or int64
- * (index64); K <= passion_topk_distill_max_k().  lse: f32 [R], kept by the forward for the backward (NULL: loss only).
+ * (index64); K <= passion_topk_distill_max_k().  lse: f32 [R][2], the row's largest logit and log2 of its sum of exp((logit - largest) / T), kept by the
+ * forward for the backward (NULL: loss only).  Logits may hold -inf and their type's lowest value.
  * Backward: dlogits = dloss[r] * d loss[r] / d logits, of logits' dtype; V > 512: both 16-byte aligned (-1005). */
 int passion_topk_distill_max_k(void);
 int passion_topk_distill_fwd(const void* logits, int dtype, const void* values, int values_dtype, const void* index, int index64, int64_t R, int V, int K,

@@ -12,7 +12,8 @@
 //    writer each): the bulk of the row needs no comparison with the indices.
 //  * V <= 512: G lanes a row (a power of two), the row in registers, 256 / G rows a workgroup -- the voxel classes of this framework (V = 4: one
 //    lane, one 16-byte load a row).
-// Sums and exponentials are f32; the gradient rounds once.
+// Sums and exponentials are f32; the gradient rounds once.  Exponents are differences of logits times log2(e) / T, and a row's largest logit and the log of its sum stay
+// apart: masked classes may hold their type's lowest value (log2(e) / T times that is past the type's range below T = 1.44), and a large common offset costs no bits.
 // 4096 x 50000 bf16, K = 32: forward 119 us (3.45 TB/s: what a read-only pass reaches on this card), backward 157 (5.2 TB/s of reads and writes).
 #include "common.h"
 #include "passion_hip.h"
@@ -26,7 +27,7 @@ struct DsP {
     const void* s;            // [R][V] student logits
     const void* tv;           // [R][K] teacher logits
     const void* idx;          // [R][K] int32 / int64
-    float* lse;               // [R] log2 of sum exp(s / T)  (+inf marks a row without a teacher)
+    float* lse;               // [R][2] m = the largest logit, log2 of sum exp((s - m) / T)  (+inf marks a row without a teacher)
     float* loss;              // [R]
     const float* g;           // [R]
     void* ds;
@@ -44,11 +45,11 @@ __device__ __forceinline__ int tidx(const DsP& p, long i) {
     return v >= 0 && v < p.V ? (int)v : -1;
 }
 
-// running (reference, sum of exp2(z - reference)); -inf references carry an empty sum
-__device__ __forceinline__ void join(float& m, float& l, float m2, float l2) {
+// running (reference, sum of exp2(c (s - reference))), s and the reference in the logits' units; -inf references carry an empty sum
+__device__ __forceinline__ void join(float& m, float& l, float m2, float l2, float c) {
     const float M = fmaxf(m, m2);
     const float a = M == -INFINITY ? 0.f : M;
-    l = l * exp2f(m - a) + l2 * exp2f(m2 - a);
+    l = l * exp2f((m - a) * c) + l2 * exp2f((m2 - a) * c);
     m = M;
 }
 
@@ -72,27 +73,27 @@ template <> __device__ __forceinline__ void vstore<bf16_t>(bf16_t* p, const floa
     *reinterpret_cast<b8*>(p) = __builtin_convertvector((f8){v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}, b8);
 }
 
-// N logits into the running pair; m in the logits' units, l in units of exp2(c m).  A NaN reaches the sum, whatever the maximum makes of it
+// N logits into the running pair.  A NaN reaches the sum, whatever the maximum makes of it
 template <int N> __device__ __forceinline__ void absorb(const float* v, float c, float& m, float& l) {
     float mx = v[0];
 #pragma unroll
     for (int j = 1; j < N; ++j) mx = fmaxf(mx, v[j]);
     if (mx > m) { l *= __builtin_amdgcn_exp2f((m - mx) * c); m = mx; }         // m = -inf: l is 0
-    const float ref = m == -INFINITY ? 0.f : -m * c;
+    const float ref = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], c, ref));
+    for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f((v[j] - ref) * c);
     l += s;
 }
 
-// teacher of one row over the 64 lanes of a wavefront: reference and 1 / sum of its softmax (log2 units); false: no entry
+// teacher of one row over the 64 lanes of a wavefront: largest logit and 1 / sum of its softmax; false: no entry
 __device__ __forceinline__ bool teacher(const DsP& p, long row, int lane, float& m, float& inv) {
     m = -INFINITY;
-    for (int k = lane; k < p.K; k += 64) if (tidx(p, row * p.K + k) >= 0) { const float t = tval(p, row * p.K + k) * p.c; m = t > m || t != t ? t : m; }
+    for (int k = lane; k < p.K; k += 64) if (tidx(p, row * p.K + k) >= 0) { const float t = tval(p, row * p.K + k); m = t > m || t != t ? t : m; }
     for (int o = 32; o > 0; o >>= 1) { const float t = __shfl_xor(m, o, 64); m = t > m || t != t ? t : m; }
     if (m == -INFINITY) return false;
     float l = 0.f;
-    for (int k = lane; k < p.K; k += 64) if (tidx(p, row * p.K + k) >= 0) l += exp2f(tval(p, row * p.K + k) * p.c - m);
+    for (int k = lane; k < p.K; k += 64) if (tidx(p, row * p.K + k) >= 0) l += exp2f((tval(p, row * p.K + k) - m) * p.c);
     l = wave_sum(l);
     inv = 1.f / l;
     return true;
@@ -131,23 +132,22 @@ __global__ __launch_bounds__(NT) void ds_fwd_row_kernel(DsP p) {
             vload<T>(s + head + (long)i * VEC, v);
             absorb<VEC>(v, p.c, m, l);
         }
-        m *= p.c;
-        for (int o = 32; o > 0; o >>= 1) { const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64); join(m, l, m2, l2); }
+        for (int o = 32; o > 0; o >>= 1) { const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64); join(m, l, m2, l2, p.c); }
         if (lane == 0) { red[0][wv] = m; red[1][wv] = l; }
         __syncthreads();
         if (wv == 0) {
             m = red[0][0]; l = red[1][0];
-            for (int w = 1; w < NT / 64; ++w) join(m, l, red[0][w], red[1][w]);
-            const float lse = m + log2f(l);
+            for (int w = 1; w < NT / 64; ++w) join(m, l, red[0][w], red[1][w], p.c);
+            const float ls = log2f(l);
             float acc = 0.f;
             bool live;
             if (p.K <= 64) {
-                const float t = at0 >= 0 ? tv0 * p.c : -INFINITY;
+                const float t = at0 >= 0 ? tv0 : -INFINITY;
                 float tm = t;
                 for (int o = 32; o > 0; o >>= 1) { const float u = __shfl_xor(tm, o, 64); tm = u > tm || u != u ? u : tm; }
                 live = tm != -INFINITY;
-                const float e = live && at0 >= 0 ? exp2f(t - tm) : 0.f, sum = lanes_sum(e, 64), pk = e / sum;
-                if (e != 0.f) acc = pk * ((t - tm - log2f(sum)) - (z0 * p.c - lse));
+                const float d = (t - tm) * p.c, e = live && at0 >= 0 ? exp2f(d) : 0.f, sum = lanes_sum(e, 64), pk = e / sum;
+                if (e != 0.f) acc = pk * ((d - log2f(sum)) - ((z0 - m) * p.c - ls));
                 acc = lanes_sum(acc, 64);
             } else {
                 float tm, inv = 0.f;
@@ -157,15 +157,18 @@ __global__ __launch_bounds__(NT) void ds_fwd_row_kernel(DsP p) {
                     for (int k = lane; k < p.K; k += 64) {
                         const int at = tidx(p, row * p.K + k);
                         if (at < 0) continue;
-                        const float d = tval(p, row * p.K + k) * p.c - tm, pk = exp2f(d) * inv;
-                        if (pk != 0.f) acc += pk * ((d - lt) - (to_f32(s[at]) * p.c - lse));
+                        const float d = (tval(p, row * p.K + k) - tm) * p.c, pk = exp2f(d) * inv;
+                        if (pk != 0.f) acc += pk * ((d - lt) - ((to_f32(s[at]) - m) * p.c - ls));
                     }
                     acc = wave_sum(acc);
                 }
             }
             if (lane == 0) {
                 p.loss[row] = live ? p.T * p.T * LN2 * acc : 0.f;
-                if (p.lse) p.lse[row] = live ? lse : INFINITY;           // +inf marks a row without a teacher (a finite or NaN sum never gives it)
+                if (p.lse) {
+                    p.lse[2 * row] = m;
+                    p.lse[2 * row + 1] = live ? ls : INFINITY;           // +inf marks a row without a teacher (a finite or NaN sum never gives it)
+                }
             }
         }
         __syncthreads();
@@ -181,22 +184,23 @@ __global__ __launch_bounds__(NT) void ds_bwd_row_kernel(DsP p) {
     for (long row = blockIdx.x; row < p.R; row += gridDim.x) {
         const T* s = static_cast<const T*>(p.s) + row * p.V;
         T* o = static_cast<T*>(p.ds) + row * p.V;
-        const float lse = p.lse[row], f = p.g[row] * p.T;
-        const bool live = lse != INFINITY;
+        const float m = p.lse[2 * row], ls = p.lse[2 * row + 1], f = p.g[row] * p.T;
+        const bool live = ls != INFINITY;
+        auto grad = [&](float z) { return f * __builtin_amdgcn_exp2f(__builtin_fmaf(z - m, p.c, -ls)); };        // f q
         if (live && wv == NT / 64 - 1) {                 // the last wavefront, while the others stream the row; read behind the barrier below
             float tm, inv = 0.f;
             teacher(p, row, lane, tm, inv);
             for (int k = lane; k < p.K; k += 64) {
                 at[k] = tidx(p, row * p.K + k);
-                pk[k] = at[k] < 0 ? 0.f : exp2f(tval(p, row * p.K + k) * p.c - tm) * inv;
+                pk[k] = at[k] < 0 ? 0.f : exp2f((tval(p, row * p.K + k) - tm) * p.c) * inv;
             }
         }
         // the student's and the gradient's rows start at the same offset from a 16-byte point (both bases are aligned)
         const int head = (int)min((long)p.V, (long)(((16 - ((uintptr_t)s & 15)) & 15) / sizeof(T)));
         const int nvec = (p.V - head) / VEC, tail = head + nvec * VEC;
         if (live) {
-            if (tid < head) o[tid] = from_f32<T>(f * __builtin_amdgcn_exp2f(to_f32(s[tid]) * p.c - lse));
-            if (tid < p.V - tail) o[tail + tid] = from_f32<T>(f * __builtin_amdgcn_exp2f(to_f32(s[tail + tid]) * p.c - lse));
+            if (tid < head) o[tid] = from_f32<T>(grad(to_f32(s[tid])));
+            if (tid < p.V - tail) o[tail + tid] = from_f32<T>(grad(to_f32(s[tail + tid])));
             int i = tid;
             for (; i + 3 * NT < nvec; i += 4 * NT) {
                 float v[4][VEC];
@@ -205,7 +209,7 @@ __global__ __launch_bounds__(NT) void ds_bwd_row_kernel(DsP p) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[u][j] = f * __builtin_amdgcn_exp2f(v[u][j] * p.c - lse);
+                    for (int j = 0; j < VEC; ++j) v[u][j] = grad(v[u][j]);
                     vstore<T>(o + head + (long)(i + u * NT) * VEC, v[u]);
                 }
             }
@@ -213,7 +217,7 @@ __global__ __launch_bounds__(NT) void ds_bwd_row_kernel(DsP p) {
                 float v[VEC];
                 vload<T>(s + head + (long)i * VEC, v);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = f * __builtin_amdgcn_exp2f(v[j] * p.c - lse);
+                for (int j = 0; j < VEC; ++j) v[j] = grad(v[j]);
                 vstore<T>(o + head + (long)i * VEC, v);
             }
             stores_done();                               // the row is written before the named classes are written again
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(NT) void ds_bwd_row_kernel(DsP p) {
                 bool first = true;
                 for (int j = 0; j < p.K; ++j)
                     if (at[j] == a) { sum += pk[j]; first &= j >= k; }
-                if (first) o[a] = from_f32<T>(f * (__builtin_amdgcn_exp2f(to_f32(s[a]) * p.c - lse) - sum));
+                if (first) o[a] = from_f32<T>(f * (__builtin_amdgcn_exp2f(__builtin_fmaf(to_f32(s[a]) - m, p.c, -ls)) - sum));
             }
         __syncthreads();
     }
@@ -257,50 +261,48 @@ __global__ __launch_bounds__(256) void ds_small_kernel(DsP p, int G) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = a[j];
             }
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) x[j] *= p.c;
         } else {
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) { const int c = VEC ? t * VPT + j : j * G + t; x[j] = c < p.V ? to_f32(s[c]) * p.c : -INFINITY; }
+            for (int j = 0; j < VPT; ++j) { const int c = VEC ? t * VPT + j : j * G + t; x[j] = c < p.V ? to_f32(s[c]) : -INFINITY; }
         }
-        // teacher (log2 units)
+        // teacher
         float tm = -INFINITY;
-        for (int k = t; k < p.K; k += G) if (tidx(p, row * p.K + k) >= 0) { const float v = tval(p, row * p.K + k) * p.c; tm = v > tm || v != v ? v : tm; }
+        for (int k = t; k < p.K; k += G) if (tidx(p, row * p.K + k) >= 0) { const float v = tval(p, row * p.K + k); tm = v > tm || v != v ? v : tm; }
         for (int o = G >> 1; o > 0; o >>= 1) { const float v = __shfl_xor(tm, o, 64); tm = v > tm || v != v ? v : tm; }
         const bool live = tm != -INFINITY;
         float tl = 0.f;
-        if (live) for (int k = t; k < p.K; k += G) if (tidx(p, row * p.K + k) >= 0) tl += exp2f(tval(p, row * p.K + k) * p.c - tm);
+        if (live) for (int k = t; k < p.K; k += G) if (tidx(p, row * p.K + k) >= 0) tl += exp2f((tval(p, row * p.K + k) - tm) * p.c);
         for (int o = G >> 1; o > 0; o >>= 1) tl += __shfl_xor(tl, o, 64);
         const float inv = 1.f / tl;
         if constexpr (!BWD) {
             float m = -INFINITY, l = 0.f;
-            absorb<VPT>(x, 1.f, m, l);
-            for (int o = G >> 1; o > 0; o >>= 1) { const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64); join(m, l, m2, l2); }
-            const float lse = m + log2f(l);
+            absorb<VPT>(x, p.c, m, l);
+            for (int o = G >> 1; o > 0; o >>= 1) { const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64); join(m, l, m2, l2, p.c); }
+            const float ls = log2f(l);
             float acc = 0.f;
             if (live) {
                 const float lt = log2f(tl);
                 for (int k = t; k < p.K; k += G) {
                     const int a = tidx(p, row * p.K + k);
                     if (a < 0) continue;
-                    const float d = tval(p, row * p.K + k) * p.c - tm, pk = exp2f(d) * inv;
-                    if (pk != 0.f) acc += pk * ((d - lt) - (to_f32(s[a]) * p.c - lse));
+                    const float d = (tval(p, row * p.K + k) - tm) * p.c, pk = exp2f(d) * inv;
+                    if (pk != 0.f) acc += pk * ((d - lt) - ((to_f32(s[a]) - m) * p.c - ls));
                 }
             }
             for (int o = G >> 1; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
             if (ok && t == 0) {
                 p.loss[row] = live ? p.T * p.T * LN2 * acc : 0.f;
-                if (p.lse) p.lse[row] = lse;
+                if (p.lse) { p.lse[2 * row] = m; p.lse[2 * row + 1] = ls; }
             }
         } else {
-            const float lse = p.lse[row], f = p.g[row] * p.T;
+            const float m = p.lse[2 * row], ls = p.lse[2 * row + 1], f = p.g[row] * p.T;
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) x[j] = live ? __builtin_amdgcn_exp2f(x[j] - lse) : 0.f;
+            for (int j = 0; j < VPT; ++j) x[j] = live ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - m, p.c, -ls)) : 0.f;
             if (live)
                 for (int k = 0; k < p.K; ++k) {
                     const int a = tidx(p, row * p.K + k);
                     if (a < 0) continue;
-                    const float pk = exp2f(tval(p, row * p.K + k) * p.c - tm) * inv;
+                    const float pk = exp2f((tval(p, row * p.K + k) - tm) * p.c) * inv;
 #pragma unroll
                     for (int j = 0; j < VPT; ++j) x[j] -= (VEC ? t * VPT + j : j * G + t) == a ? pk : 0.f;
                 }

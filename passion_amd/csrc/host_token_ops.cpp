@@ -200,7 +200,7 @@ at::Tensor ds_forward(const at::Tensor& s, const at::Tensor& tv, const at::Tenso
     const c10::DeviceGuard guard(s.device());
     const int64_t R = s.size(0);
     at::Tensor loss = at::empty({R}, s.options().dtype(at::kFloat));
-    if (lse) *lse = at::empty({R}, s.options().dtype(at::kFloat));
+    if (lse) *lse = at::empty({R, 2}, s.options().dtype(at::kFloat));
     if (R)
         check(g.ds_fwd(s.data_ptr(), code(s), tv.data_ptr(), code(tv), ti.data_ptr(), ti.scalar_type() == at::kLong, R, (int)s.size(1), (int)tv.size(1), (float)temp, fptr(loss),
                        lse ? fptr(*lse) : nullptr, cur_stream()),

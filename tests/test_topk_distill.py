@@ -111,6 +111,37 @@ def test_masked_classes(V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F, H])
+@pytest.mark.parametrize("T", [0.5, 1.0, 8.0])
+@pytest.mark.parametrize("V", [3, 40, 500, 900, 4099, 40000])
+def test_runs_of_masked_classes(V, T, dt):
+    """whole runs of classes at their type's lowest value (a padded or restricted set of classes), as far as a row that holds nothing else (all classes alike) and a
+    teacher's entries that do (all shares alike): log2(e) / T times that value is past the type's range below T = 1.44.  Same tolerances as ever: the differences of
+    logits are exact or overflow to -inf, whose share is 0 on both sides"""
+    s, t, i, g = _make(24, V, 2, dt, seed=11)
+    s[:, V // 4:V // 2] = torch.finfo(dt).min
+    s[5:9, : V - 1] = torch.finfo(dt).min
+    s[9, 1:] = torch.finfo(dt).min
+    s[10] = torch.finfo(dt).min
+    i = V - 1 - i % max(1, V // 4)              # classes that every row but those few keeps
+    i[5:9], i[9] = V - 1, 0
+    t[11:13] = torch.finfo(F).min
+    t[13, 0] = torch.finfo(F).min
+    _check(s, t, i, g, T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 3000])
+def test_a_common_offset_of_a_row_costs_nothing(V):
+    """softmax does not know it: logits of 1e5 and a little, exact in f32 as given"""
+    s, t, i, g = _make(12, V, 3, F, seed=12)
+    s[::2] += 1e5
+    s[1::2] -= 1e5
+    t += 3e4
+    _check(s, t, i, g, 1.0)
+
+
+@pytest.mark.gpu
 def test_views_and_leading_shapes():
     """(B, D, H, W, C) voxels, transposed storage, a base that is not 16-byte aligned"""
     from passion_amd import ops
