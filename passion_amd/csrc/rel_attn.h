@@ -15,7 +15,7 @@ struct RelP {
     const int* buckets;                   // [nd]; NULL: an offset is its own bucket
     float* slab;                          // the table's partial gradients (LINE: rows of slab_len, else the dense sums); NULL: not wanted
     long slab_len;
-    int QC, KC, parts;                    // dense sums: distinct query and key cells, parts of the passes
+    int QC, KC, parts;                    // dense sums: queries and keys of one pass (whole copies of the cells), parts of the passes
     float *po, *pm, *pl;                  // split forward: [nsplit][B][H][Nq](D), f32
     int B, Nq, Nk, H, Hkv, D;
     int gd, gh, gw, vol, nd, omax, q0, nb, tdt;

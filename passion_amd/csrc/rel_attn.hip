@@ -210,6 +210,23 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     }
 }
 
+// a grid smaller than a tile: out[h][a][c] = sum of M over its parts and over the copies of cells a < qc, c < kc.  A workgroup a pair, in a fixed order
+__global__ __launch_bounds__(256) void rel_copies_kernel(RelP p, int ld, int qc, int kc, float* out) {
+    __shared__ float red[4];
+    const int a0 = blockIdx.x / kc, c0 = blockIdx.x % kc, h = blockIdx.y;
+    const int ma = (p.QC - a0 + p.vol - 1) / p.vol, mc = (p.KC - c0 + p.vol - 1) / p.vol, n = p.parts * ma * mc;
+    float s = 0.f;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int c = i % mc, a = i / mc % ma, z = i / mc / ma;
+        s += p.slab[(((long)z * p.H + h) * p.QC + a0 + a * p.vol) * ld + c0 + c * p.vol];
+    }
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) out[((long)h * qc + a0) * kc + c0] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 // dtable[c][h] = sum of G[h][o] over the offsets of bucket c.  Few buckets: a workgroup a bucket; many: a thread a bucket, the map in LDS
 template <typename TT>
 __global__ __launch_bounds__(256) void rel_bucket_few_kernel(const float* G, const int* buckets, TT* dt, int nd, int H) {
@@ -311,7 +328,7 @@ long slab_floats(RelP& p, int dtype) {
         p.slab_len = (nqb + p.ksplit - 1) / p.ksplit * blk + 32;
         return (long)p.B * p.H * tiles32(p.Nk) * p.ksplit * p.slab_len;
     }
-    p.QC = (int)hmin(p.Nq, p.vol); p.KC = (int)hmin(p.Nk, p.vol);
+    p.QC = (int)hmin(p.Nq, p.vol * hmax(1, 128 / p.vol)); p.KC = (int)hmin(p.Nk, p.vol * hmax(1, 64 / p.vol));
     const long passes = (long)p.B * ((p.Nq + p.QC - 1) / p.QC) * ((p.Nk + p.KC - 1) / p.KC), nkb = (p.KC + blk - 1) / blk, waves = tiles32(p.QC) * nkb * p.H;
     p.parts = (int)hmax(1, hmin(passes, 2048 / waves));            // about two wavefronts a SIMD
     return (long)p.parts * p.H * p.QC * nkb * blk;
@@ -320,7 +337,7 @@ long slab_floats(RelP& p, int dtype) {
 int run(const RelP& p, int dtype, int what, int nw, hipStream_t st) { return dtype == PASSION_BF16 ? rel_run_bf16(p, what, nw, st) : rel_run_f32(p, what, nw, st); }
 
 // layout of the workspaces, in floats
-struct Ws { long e, po, pm, pl, delta, slab, G, total; };
+struct Ws { long e, po, pm, pl, delta, slab, cells, G, total; };
 Ws fwd_ws(RelP& p, int dtype) {
     p.few = few_rows(p);
     p.pack = p.few && p.H > p.Hkv;
@@ -350,6 +367,7 @@ Ws bwd_ws(RelP& p, int dtype, bool want_table) {
     w.pm = take(p.nsplit > 1 ? p.nsplit * rows : 0);
     if (p.bias == 2 || (p.bias && want_table)) {           // (1D: the key-major kernel forms its sums on the way)
         w.slab = take(slab_floats(p, dtype));
+        w.cells = take(p.bias != 2 && hmax(p.QC, p.KC) > p.vol ? p.H * hmin(p.QC, p.vol) * hmin(p.KC, p.vol) : 0);
         w.G = take(p.buckets ? (long)p.H * p.nd : 0);
     }
     w.total = at;
@@ -451,8 +469,17 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
         const long nkb = p.bias == 2 ? 0 : (p.KC + blk_of(dtype) - 1) / blk_of(dtype);
         if (p.bias != 2 && (rc = run(p, dtype, 3, pick_waves(tiles32(p.QC), nkb * H * p.parts), st))) return rc;
         float* G = workspace + w.G;
-        const FoldP f{p.slab, G, buckets ? nullptr : dtable, p.slab_len, table_dtype, B, H, p.nd, (int)tiles32(Nk), p.gw - 1 + p.q0, p.gd, p.gh, p.gw, p.vol, p.q0, p.QC, p.KC,
-                      (int)(nkb * blk_of(dtype)), p.parts, p.ksplit, __builtin_ctz(p.ksplit), (Nq + blk_of(dtype) - 1) / blk_of(dtype), blk_of(dtype)};
+        FoldP f{p.slab, G, buckets ? nullptr : dtable, p.slab_len, table_dtype, B, H, p.nd, (int)tiles32(Nk), p.gw - 1 + p.q0, p.gd, p.gh, p.gw, p.vol, p.q0, p.QC, p.KC,
+                (int)(nkb * blk_of(dtype)), p.parts, p.ksplit, __builtin_ctz(p.ksplit), (Nq + blk_of(dtype) - 1) / blk_of(dtype), blk_of(dtype)};
+        if (p.bias != 2 && hmax(p.QC, p.KC) > p.vol) {
+            f.QC = (int)hmin(p.QC, p.vol);
+            f.KC = (int)hmin(p.KC, p.vol);
+            hipLaunchKernelGGL(rel_copies_kernel, dim3(f.QC * f.KC, H), dim3(256), 0, st, p, f.ld, f.QC, f.KC, workspace + w.cells);
+            LAUNCH_RET();
+            f.slab = workspace + w.cells;
+            f.ld = f.KC;
+            f.parts = 1;
+        }
         if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<true>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
         else hipLaunchKernelGGL(rel_fold_kernel<false>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
         LAUNCH_RET();

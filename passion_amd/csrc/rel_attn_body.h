@@ -771,8 +771,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// dS summed over the batch and over repeated cells, for every pair of cells: M[z][h][a][c], a < QC = min(Nq, vol) the queries a, a + QC, ..., c < KC = min(Nk, vol)
-// the keys c, c + KC, ....  grid (query tiles of 32 NW x key blocks, H, parts z of the passes (batch, query copy, key copy)).  Tiles as in rel_q_kernel
+// dS summed over the batch and over repeated cells, for every pair of cells: M[z][h][a][c], a < QC the queries a, a + QC, ..., c < KC the keys c, c + KC, ....  QC and KC
+// are the grid's cells (or all tokens, if they are fewer); of a grid smaller than a tile, as many of its copies as a tile holds.
+// grid (query tiles of 32 NW x key blocks, H, parts z of the passes (batch, query copy, key copy)).  Tiles as in rel_q_kernel
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_d_kernel(RelP p) {
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32;
@@ -782,8 +783,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     const int nkb = (p.KC + BLKN - 1) / BLKN, head = blockIdx.y, hk = head / (p.H / p.Hkv);
     const int a = ((blockIdx.x / nkb) * NW + wv) * 32 + (lane & 31), c0 = (blockIdx.x % nkb) * BLKN;
     const int MQ = (p.Nq + p.QC - 1) / p.QC, MK = (p.Nk + p.KC - 1) / p.KC;
-    const long passes = (long)p.B * MQ * MK;
-    const int t0 = (int)(passes * blockIdx.z / gridDim.z), t1 = (int)(passes * (blockIdx.z + 1) / gridDim.z);
+    const long passes = (long)p.B * MQ * MK;                       // (past 2^31 for long sequences over few cells)
+    const long t0 = passes * blockIdx.z / gridDim.z, t1 = passes * (blockIdx.z + 1) / gridDim.z;
+    struct Pass { int b, cq, ck; };                                // batch entry, copy of the queries, copy of the keys
+    auto next = [&](Pass t) {
+        if (++t.ck == MK) { t.ck = 0; if (++t.cq == MQ) { t.cq = 0; ++t.b; } }
+        return t;
+    };
 
     f32x16 acc[KT], bias[KT];
     const int aq = place(p, p.q0 + min(a, p.QC - 1)) + p.omax;
@@ -798,9 +804,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     Tile<T, DP, NT> kt_, vt_;
     uint64_t valid = 0;
     bool there = false;
-    auto fetch = [&](int t) {
+    auto fetch = [&](Pass t) {
         // (a copy of the cells may end before this block of them does: its rows are then the last token's, and none is valid)
-        const int b = t / (MQ * MK), j0 = min((t % MK) * p.KC + c0, p.Nk - 1), n = min(p.Nk, (t % MK + 1) * p.KC) - ((t % MK) * p.KC + c0), last = max(0, min(n, BLKN) - 1);
+        const int b = t.b, j0 = min(t.ck * p.KC + c0, p.Nk - 1), n = min(p.Nk, (t.ck + 1) * p.KC) - (t.ck * p.KC + c0), last = max(0, min(n, BLKN) - 1);
         kt_.fetch(static_cast<const T*>(p.k) + (long)b * p.ks[0] + (long)hk * p.ks[2] + j0 * p.ks[1], (int)(p.ks[1] * sizeof(T)), last, p.D, tid);
         vt_.fetch(static_cast<const T*>(p.v) + (long)b * p.vs[0] + (long)hk * p.vs[2] + j0 * p.vs[1], (int)(p.vs[1] * sizeof(T)), last, p.D, tid);
         there = lane < min(n, BLKN);
@@ -811,10 +817,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         kt_.commit(buf, tid, valid, p.D);
         vt_.commit(buf + IMG, tid, valid, p.D);
     };
-    auto step = [&](int t) {
-        const char* kimg = lds + ((t - t0) & 1) * BUF;
-        if (t == t0 || t % MK == 0) {                              // the next (batch, query copy)
-            const int b = t / (MQ * MK), i = (t / MK) % MQ * p.QC + a, ic = min(i, p.Nq - 1);
+    auto step = [&](Pass t, const char* kimg, bool first) {
+        if (first || t.ck == 0) {                                  // the next (batch, query copy)
+            const int b = t.b, i = t.cq * p.QC + a, ic = min(i, p.Nq - 1);
             const bool qok = a < p.QC && i < p.Nq;
             const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (long)b * p.qs[0] + (long)ic * p.qs[1] + (long)head * p.qs[2]);
             const char* dp = reinterpret_cast<const char*>(static_cast<const T*>(p.dout) + (((long)b * p.Nq + ic) * p.H + head) * p.D);
@@ -854,16 +859,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         }
     };
     if (t0 < t1) {
-        fetch(t0);
+        Pass at = {(int)(t0 / MK / MQ), (int)(t0 / MK % MQ), (int)(t0 % MK)};
+        fetch(at);
         commit(lds);
         __syncthreads();
-        for (int t = t0; t + 1 < t1; ++t) {
-            fetch(t + 1);
-            step(t);
+        for (long t = t0; t + 1 < t1; ++t) {
+            const Pass then = next(at);
+            fetch(then);
+            step(at, lds + ((t - t0) & 1) * BUF, t == t0);
             commit(lds + ((t + 1 - t0) & 1) * BUF);
             __syncthreads();
+            at = then;
         }
-        step(t1 - 1);
+        step(at, lds + ((t1 - 1 - t0) & 1) * BUF, t0 + 1 == t1);
     }
     if (a < p.QC) {
         float* dst = p.slab + (((long)blockIdx.z * p.H + head) * p.QC + a) * ((long)nkb * BLKN) + c0 + 4 * h;

@@ -379,6 +379,45 @@ def test_far_end_of_a_long_cache():
 
 
 @pytest.mark.gpu
+@BOTH
+@pytest.mark.parametrize("grid,B,Nq,Nk,heads,Hkv,D,nb,q0,mask", [((1,), 2, 300, 700, 2, 1, 16, None, 0, "random"), ((2, 2), 1, 1000, 257, 2, 2, 32, None, 3, None),
+                                                                   ((1, 3, 2), 3, 130, 900, 4, 4, 64, 4, 1, "runs"), ((4, 4, 4), 1, 700, 300, 1, 1, 40, None, 30, "empty"),
+                                                                   ((5, 13), 1, 300, 300, 2, 1, 8, None, 7, None), ((3,), 2, 2, 1000, 2, 2, 16, None, 4, None),
+                                                                   ((3, 9), 2, 1000, 20, 2, 2, 16, 9, 0, "random")])
+def test_many_copies_of_few_cells(grid, B, Nq, Nk, heads, Hkv, D, nb, q0, mask, dt):
+    """grids smaller than a tile: a pass of the table's sums takes several copies of the cells, and the copies fold afterwards"""
+    _check(_make(B, Nq, Nk, heads, Hkv, D, dt, grid, nb=nb, q0=q0, mask=mask))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cells", [1, 2, 3])
+def test_the_table_s_gradient_of_a_long_sequence_over_few_cells(cells):
+    """50000 tokens over one cell are 2.5e9 (query copy, key copy) pairs: once, they were counted in 32 bits and keys were read before their start.  Tolerance as above,
+    the 64-bit sums taken in ranges of queries"""
+    from passion_amd import ops
+    N, D = 50000, 8
+    c = {n: t.cuda() if torch.is_tensor(t) else t for n, t in _make(1, N, N, 1, 1, D, H, (cells,)).items()}
+    table = c["table"].clone().requires_grad_()
+    (got,) = torch.autograd.grad(ops.rel_attention(c["q"], c["k"], c["v"], table, (cells,)), table, c["dout"])
+    q, k, v, do = (c[n][0, :, 0].double() for n in ("q", "k", "v", "dout"))
+    u, cell = U[H], torch.arange(N, device="cuda") % cells
+    want, room = (torch.zeros(2 * cells - 1, 1, dtype=torch.float64, device="cuda") for _ in range(2))
+    step = 1200                                       # a multiple of the cells
+    for a in range(0, N, step):
+        rows = slice(a, min(N, a + step))
+        off = cell[rows, None] - cell[None] + cells - 1
+        p = torch.softmax(q[rows] @ k.t().contiguous() * c["scale"] + c["table"][:, 0].double()[off], 1)
+        dp = do[rows] @ v.t().contiguous()
+        ds = p * (dp - (p * dp).sum(1, keepdim=True))
+        err = u * ds.abs() + p * (do[rows].abs() * u * (p @ v.abs() + (p @ v).abs())).sum(1, keepdim=True)
+        for x in range(2 * cells - 1):
+            at = off == x
+            want[x] += ds[at].sum()
+            room[x] += err[at].sum() / u
+    near(got, want, u, "dtable", room=room)
+
+
+@pytest.mark.gpu
 def test_no_tokens():
     from passion_amd import ops
     for B, Nq, Nk in ((0, 3, 3), (2, 0, 4), (2, 4, 0)):
