@@ -392,11 +392,13 @@ int join(int dtype, const float* part, int n, long rows, int D, float scale, voi
 bool misaligned(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0; }
 int strides(RelP& p, int dtype, const int64_t* sq, const int64_t* sk, const int64_t* sv) {
     const int unit = dtype == PASSION_BF16 ? 8 : 4;
-    for (int i = 0; i < 3; ++i) {
-        if (sq[i] % unit || sk[i] % unit || sv[i] % unit) return -1005;
-        p.qs[i] = sq[i]; p.ks[i] = sk[i]; p.vs[i] = sv[i];
+    for (int i = 0; i < 3; ++i) {                                                 // (the stride of a dimension of one may be anything)
+        p.qs[i] = (i == 0 ? p.B : i == 1 ? p.Nq : p.H) > 1 ? sq[i] : 0;
+        p.ks[i] = (i == 0 ? p.B : i == 1 ? p.Nk : p.Hkv) > 1 ? sk[i] : 0;
+        p.vs[i] = (i == 0 ? p.B : i == 1 ? p.Nk : p.Hkv) > 1 ? sv[i] : 0;
+        if (p.qs[i] % unit || p.ks[i] % unit || p.vs[i] % unit) return -1005;
     }
-    for (const int64_t s : {sq[1], sk[1], sv[1], (int64_t)p.H * p.D})           // 32-bit lane offsets over a block of 64 tokens
+    for (const int64_t s : {(int64_t)p.qs[1], (int64_t)p.ks[1], (int64_t)p.vs[1], (int64_t)p.H * p.D})           // 32-bit lane offsets over a block of 64 tokens
         if (s < 0 || s >= (1 << 23)) return -1005;
     return 0;
 }

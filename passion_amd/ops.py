@@ -1829,7 +1829,7 @@ def relative_buckets(grid, num_buckets, max_distance=128, device=None):
 
 def _rel_view(t):
     """t as the kernels read it: dense last dimension, rows on 16-byte points, tokens less than 2^23 elements apart; a copy where it is not"""
-    a, b, c, d = t.stride()
+    a, b, c, d = (s if n > 1 else 0 for s, n in zip(t.stride(), t.shape))          # (the stride of a dimension of one may be anything)
     if d != 1 or b >= 2 ** 23 or (a | b | c) % (16 // t.element_size()) or t.data_ptr() % 16:
         return _dense(t)
     return t

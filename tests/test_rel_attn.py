@@ -274,6 +274,34 @@ def test_views_read_in_place(dt):
 
 
 @pytest.mark.gpu
+@BOTH
+def test_strides_of_dimensions_of_one(dt):
+    """a batch of one sliced out of odd rows, one token out of wider ones, one head out of a larger tensor: strides that no step takes may be anything"""
+    from passion_amd import ops
+    c = _make(1, 100, 100, 8, 8, 64, dt)
+    want = _run(c)
+    cut = {}
+    for n in ("q", "k", "v", "dout"):
+        store = torch.zeros(3, 100 * 512 + 3, dtype=dt, device="cuda")
+        store[0, :51200] = c[n].cuda().view(-1)
+        cut[n] = store[:, :51200].unflatten(1, (100, 8, 64))[0:1]
+        assert cut[n].stride(0) == 51203
+    got = _run(c, **cut)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    c = _make(1, 1, 1, 8, 8, 64, dt)
+    want = _run(c)
+    for width in (516, 1 << 24):
+        wide = {n: torch.as_strided(c[n].cuda().view(-1), (1, 1, 8, 64), (width + 1, width + 3, 64, 1)) for n in ("q", "k", "v")}
+        got = _run(c, **wide)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+    c = _make(2, 40, 40, 1, 1, 32, dt)
+    want = _run(c)
+    one = {n: torch.as_strided(c[n].cuda().view(-1), (2, 40, 1, 32), (1280, 32, 33, 1)) for n in ("q", "k", "v")}
+    got = _run(c, **one)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("grid", [(5, 5, 5), (125,), (70, 70)])
 def test_table_types_meet_either_operand_type(grid):
     for dt, tdt in ((F, H), (H, F)):
@@ -487,6 +515,22 @@ def test_c_entry_refuses_on_the_host():
     size = lambda *a: lib.passion_rel_attn_workspace_floats(*a)
     assert size(0, 0, 1, 4, 4, 2, 2, 12, 1, 1, 4, 0, 1, 0, 7) == -1003
     assert size(1, 1, 1, 400, 400, 2, 2, 64, 1, 1, 400, 0, 1, 0, 799) > 0
+
+
+def test_strides_of_dimensions_of_one_on_the_host():
+    """rows that are there to be read in place stay as they are; the C entry looks at no stride of a dimension of one (its next refusal is the missing workspace)"""
+    import ctypes
+    from passion_amd import _lib, ops
+    t = torch.zeros(3, 100 * 512 + 3)[:, :51200].unflatten(1, (100, 8, 64))[0:1]
+    if t.data_ptr() % 16 == 0:
+        assert ops._rel_view(t).data_ptr() == t.data_ptr()
+    odd = lambda n: torch.as_strided(torch.zeros(64 * 9 * 2), (n, 1, 1, 64), (67, 33, 5, 1))
+    assert ops._rel_view(odd(1)).stride(0) == 67 and ops._rel_view(odd(2)).stride(0) == 64
+    lib = _lib.load()
+    fwd = lambda B, *strides: lib.passion_rel_attn_fwd(256, *[(ctypes.c_int64 * 3)(*strides), 256] * 2, (ctypes.c_int64 * 3)(*strides), 0, B, 64, 64, 1, 1, 64, 1, 1, 64, 0,
+                                                       256, 0, None, 127, None, 1.0, 256, None, None, None)
+    assert fwd(2, 51203, 64, 64) == -1005 and fwd(1, 51204, 65, 64) == -1005 and fwd(1, 51204, 1 << 24, 64) == -1005
+    assert fwd(1, 51203, 64, 7) == -1003
 
 
 def test_workspace_sizes_past_32_bits():
