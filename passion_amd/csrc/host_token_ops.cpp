@@ -4,7 +4,10 @@
 // Nothing is kept between calls: workspaces are tensors of the call, so streams, captured graphs and threads share nothing.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "passion_hip.h"
 
@@ -34,6 +37,18 @@ inline float* fptr(const OptT& t) { return static_cast<float*>(ptr(t)); }
 inline float* fptr(const at::Tensor& t) { return static_cast<float*>(ptr(t)); }
 inline bool wants(const OptT& t) { return t && t->requires_grad(); }
 inline void bound(const void* f) { TORCH_CHECK(f, "passion_amd host extension is not bound to libpassion_hip.so"); }
+// The kernels are launched outside torch's dispatcher: what follows calls there instead of the autograd node would go on without them (a tangent lost, a trace or an exported
+// graph that holds the allocation of the result and nothing else).  Such calls are refused
+inline bool refused(const at::Tensor& t) { return t.defined() && (t._fw_grad(/*level=*/0).defined() || t.unsafeGetTensorImpl()->is_python_dispatch()); }
+inline bool refused(const OptT& t) { return t && refused(*t); }
+template <typename... Ts> void eager_only(const char* what, const Ts&... ts) {
+    using Mode = c10::impl::TorchDispatchModeKey;
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " can not be traced: its kernels are no torch operators");
+    for (const Mode m : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL})
+        TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(m), what, " can not be traced: its kernels are no torch operators");
+    TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode), what, " does not support torch.func transforms");
+    TORCH_CHECK(!(refused(ts) || ...), what, " takes plain tensors: no forward-mode derivatives, no tensor subclasses that dispatch to Python");
+}
 inline void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "this operator has no second derivative"); }
 inline OptT opt(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 // as the kernels read a whole tensor: dense and on a 16-byte point
@@ -116,6 +131,7 @@ struct RelNode : public torch::autograd::Function<RelNode> {
 at::Tensor rel_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptT& table, const OptT& buckets, const OptT& mask, std::vector<int64_t> geo,
                          double scale) {
     bound(reinterpret_cast<const void*>(g.rel_fwd));
+    eager_only("rel_attention", q, k, v, table, buckets, mask);
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || wants(table)))
         return RelNode::apply(q, k, v, table, buckets, mask, std::move(geo), scale)[0];
     return rel_forward(q, k, v, table, buckets, mask, geo, scale, nullptr);
@@ -189,6 +205,7 @@ struct RnNode : public torch::autograd::Function<RnNode> {
 variable_list residual_norm(const at::Tensor& x, const at::Tensor& h, const OptT& gate, const OptT& scale, const OptT& w1, const OptT& b1, const OptT& w2, const OptT& b2,
                             std::vector<int64_t> meta, std::vector<double> eps) {
     bound(reinterpret_cast<const void*>(g.rn_fwd));
+    eager_only("residual_norm", x, h, gate, scale, w1, b1, w2, b2);
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || h.requires_grad() || wants(gate) || wants(scale) || wants(w1) || wants(b1) || wants(w2) || wants(b2)))
         return RnNode::apply(x, h, gate, scale, w1, b1, w2, b2, std::move(meta), std::move(eps));
@@ -234,6 +251,7 @@ struct DsNode : public torch::autograd::Function<DsNode> {
 
 at::Tensor topk_distill(const at::Tensor& s, const at::Tensor& tv, const at::Tensor& ti, double temp) {
     bound(reinterpret_cast<const void*>(g.ds_fwd));
+    eager_only("topk_distill", s, tv, ti);
     if (at::GradMode::is_enabled() && s.requires_grad()) return DsNode::apply(s, tv, ti, temp)[0];
     return ds_forward(s, tv, ti, temp, nullptr);
 }
