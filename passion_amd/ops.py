@@ -1722,14 +1722,14 @@ def _dense(t):
     return t.clone() if t.data_ptr() % 16 else t
 
 
-def _norm_spec(m, C, dtype, what):
+def _norm_spec(m, C, what):
     """(kind, weight, bias, eps) of an nn.LayerNorm / nn.RMSNorm over the last dimension; None: no norm"""
     if m is None:
         return 0, None, None, 0.0
     kind = 1 if isinstance(m, torch.nn.LayerNorm) else 2 if isinstance(m, torch.nn.RMSNorm) else 0
     if not kind or tuple(m.normalized_shape) != (C,):
         raise ValueError(f"residual_norm: {what} has to be nn.LayerNorm({C}), nn.RMSNorm({C}) or None, got {m}")
-    eps = m.eps if m.eps is not None else torch.finfo(dtype).eps       # nn.RMSNorm's own default
+    eps = m.eps if m.eps is not None else torch.finfo(torch.float32).eps       # nn.RMSNorm's own default, that of the type it sums in (bf16 inputs too)
     f32 = lambda p: p if p is None or p.dtype == torch.float32 else p.float()
     return kind, f32(m.weight), f32(m.bias) if kind == 1 else None, float(eps)
 
@@ -1746,8 +1746,8 @@ def residual_norm(x, h, post=None, pre=None, gate=None, scale=None):
     C = x.shape[-1]
     if not 1 <= C <= 8192:
         raise ValueError(f"residual_norm: {C} channels, 1 to 8192 are supported")
-    post, w1, b1, eps1 = _norm_spec(post, C, h.dtype, "post")
-    pre, w2, b2, eps2 = _norm_spec(pre, C, x.dtype, "pre")
+    post, w1, b1, eps1 = _norm_spec(post, C, "post")
+    pre, w2, b2, eps2 = _norm_spec(pre, C, "pre")
     rows = x.numel() // C
     B, N, gmode = 1, rows, 0
     if gate is not None:

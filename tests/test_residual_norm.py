@@ -237,6 +237,32 @@ def test_captured_and_replayed():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tx,th", [(F, F), (F, H), (H, H)])
+def test_the_default_eps_of_an_rms_norm(tx, th):
+    """nn.RMSNorm(C) without eps adds f32's epsilon, whatever the input's type: rows about as large as its root, where it decides the result"""
+    from passion_amd import ops
+    C = 64
+    d = _inputs(1, 5, C, tx, th, None, False)
+    x, h = (4e-4 * d["x"].double()).to(tx), (4e-4 * d["h"].double()).to(th)
+    m = torch.nn.RMSNorm(C).cuda()
+    r, y = ops.residual_norm(x.cuda(), torch.zeros_like(h).cuda(), None, m)
+    assert torch.equal(r.cpu(), x)
+    near(y, m(x.cuda().float()).detach().double().cpu(), 1e-5, "pre")
+    r = ops.residual_norm(torch.zeros_like(x).cuda(), h.cuda(), m)
+    near(r, m(h.cuda().float()).detach().double().cpu(), 1e-5, "post")
+
+
+def test_the_default_eps_is_the_module_s():
+    from passion_amd import ops
+    for dt in (F, H):
+        x = torch.full((1, 64), 1e-4).to(dt)
+        eps = ops._norm_spec(torch.nn.RMSNorm(64), 64, "pre")[3]
+        want = torch.nn.RMSNorm(64).to(dt)(x).detach().double()
+        got = x.double() / (x.double().square().mean(-1, keepdim=True) + eps).sqrt()
+        assert float((got - want).abs().max()) <= 2.0 ** -7 * float(want.abs().max())
+
+
+@pytest.mark.gpu
 def test_no_rows():
     from passion_amd import ops
     x = torch.zeros(2, 0, 64, device="cuda", requires_grad=True)
