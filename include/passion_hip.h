@@ -492,15 +492,16 @@ int passion_topk_distill_bwd(const void* logits, int dtype, const void* values, 
 
 /* ---- attention with a learned relative position bias ---------------------------------------
  * The token grid form of SelfAttention (reference code/models/mmformer.py:192-227, which has learned absolute positions instead).  q (and out, dout, dq):
- * [B][Nq][H][D]; k, v (and dk, dv): [B][Nk][Hkv][D], head h reads key / value head h / (H / Hkv).  q, k, v by element strides of (batch, token, head), last dimension
+ * [B][Nq][H][D]; k, v (and dk, dv): [B][Nk][Hkv][D], head h reads key / value head h / (H / Hkv).  q, k, v by element strides of (batch, token, head) (of a dimension of one: anything), last dimension
  * dense, 16-byte aligned rows, tokens (and H D) less than 2^23 elements apart (-1005); all else contiguous.  f32 or bf16; D a multiple of 8 up to 128; B, H <= 65535.
  * Token t lies at cell t mod (gd gh gw) of a raster grid, query i is token q_start + i; the pair's offset is ((dz + gd - 1)(2 gh - 1) + dy + gh - 1)(2 gw - 1) + dx + gw - 1
  * with (dz, dy, dx) = cell of the query - cell of the key, its bias table[buckets[offset]][head] (buckets NULL: the offset itself, nb = number of offsets;
  * a bucket outside [0, nb): no bias; an entry at or below -1e30: the pair is excluded).  table: [nb][H] f32 or bf16, NULL: no bias.  mask: [B][Nk], 0 = key masked (its k and v are
  * not used, whatever they hold), or NULL.  A row without a key gives out 0, lse +inf and zero gradients.
  * lse: f32 [B][H][Nq] in log2 units (NULL: not kept).  workspace: passion_rel_attn_workspace_floats(...) floats, 16-byte aligned, owned by this call until the
- * stream has passed it.  Backward recomputes the probabilities; dtable of the table's shape and dtype, NULL: not wanted.  No atomics between
- * wavefronts: results repeat bit for bit. */
+ * stream has passed it; backward: 0 forward, 1 backward with the table's gradient (whose partial sums are most of it: over a grid as large as a head's scores, over a
+ * 1D raster about 1/32 of the scores of all heads), 2 backward without (dtable NULL).  Backward recomputes the probabilities; dtable of the table's shape and dtype,
+ * NULL: not wanted.  No atomics between wavefronts: results repeat bit for bit. */
 int64_t passion_rel_attn_workspace_floats(int dtype, int backward, int B, int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start,
                                           int has_table, int has_buckets, int nb);
 int passion_rel_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype, int B,

@@ -117,7 +117,7 @@ struct RelNode : public torch::autograd::Function<RelNode> {
             if (dt.defined()) dt.zero_();
         } else {
             const at::Tensor dout = dense(grads[0]);
-            const at::Tensor ws = c.workspace(q, 1, table.has_value(), buckets.has_value());
+            const at::Tensor ws = c.workspace(q, dt.defined() ? 1 : 2, table.has_value(), buckets.has_value());
             check(g.rel_bwd(q.data_ptr(), c.sq, k.data_ptr(), c.sk, v.data_ptr(), c.sv, c.dt, c.B, c.Nq, c.Nk, c.H, c.Hkv, c.D, c.geo[0], c.geo[1], c.geo[2], c.geo[3], ptr(table),
                             table ? code(*table) : 0, static_cast<const int*>(ptr(buckets)), c.nb, static_cast<const uint8_t*>(ptr(mask)),
                             (float)ctx->saved_data["scale"].toDouble(), s[6].data_ptr(), dout.data_ptr(), fptr(s[7]), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ptr(dt),

@@ -365,7 +365,7 @@ Ws bwd_ws(RelP& p, int dtype, bool want_table) {
     const long rows = (long)p.B * p.H * p.Nq, krows = (long)p.B * p.Nk * p.Hkv;
     w.po = take(hmax(p.nsplit > 1 ? p.nsplit * rows * p.D : 0, p.ksplit > 1 ? 2 * p.ksplit * krows * p.D : 0));       // dQ's parts, then those of dK and dV
     w.pm = take(p.nsplit > 1 ? p.nsplit * rows : 0);
-    if (p.bias == 2 || (p.bias && want_table)) {           // (1D: the key-major kernel forms its sums on the way)
+    if (p.bias && want_table) {
         w.slab = take(slab_floats(p, dtype));
         w.cells = take(p.bias != 2 && hmax(p.QC, p.KC) > p.vol ? p.H * hmin(p.QC, p.vol) * hmin(p.KC, p.vol) : 0);
         w.G = take(p.buckets ? (long)p.H * p.nd : 0);
@@ -411,7 +411,7 @@ extern "C" int64_t passion_rel_attn_workspace_floats(int dtype, int backward, in
     static const int dummy = 0;
     const int rc = setup(p, dtype, B, Nq, Nk, H, Hkv, D, gd, gh, gw, q_start, has_table ? &dummy : nullptr, PASSION_F32, has_buckets ? &dummy : nullptr, nb, nullptr, 1.f);
     if (rc) return rc;
-    return backward ? bwd_ws(p, dtype, true).total : fwd_ws(p, dtype).total;
+    return backward ? bwd_ws(p, dtype, backward == 1).total : fwd_ws(p, dtype).total;
 }
 
 extern "C" int passion_rel_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype, int B,
@@ -459,7 +459,7 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
     const Ws w = bwd_ws(p, dtype, dtable != nullptr);
     p.delta = workspace + w.delta;
     if ((rc = pre(p, dtype, p.bias ? workspace + w.e : nullptr, st))) return rc;
-    p.slab = workspace + w.slab;
+    p.slab = dtable ? workspace + w.slab : nullptr;
     p.po = workspace + w.po;
     p.pm = workspace + w.pm;
     if ((rc = run(p, dtype, 1, pick_waves(tiles32(Nq), (long)H * B * p.nsplit), st))) return rc;

@@ -541,8 +541,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // key-major backward: dK, dV.  grid (ceil(Nk / (32 NW)) * ksplit, Hkv, B); a wavefront owns 32 keys and walks the queries (of its part, where they are split) of all
-// the heads that share its key / value head, BLK at a time: their gradients sum in registers
-template <typename T, int DP, int NW, int BIAS>
+// the heads that share its key / value head, BLK at a time: their gradients sum in registers.  SUM (LINE): the table's gradient is wanted, its partials go to the slab
+template <typename T, int DP, int NW, int BIAS, bool SUM>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || sizeof(T) == 4 ? 1 : 2))) void rel_k_kernel(RelP p) {
     constexpr int NT = 64 * NW, BLKN = blk<T>(), KT = BLKN / 32, NCH = DP * (int)sizeof(T) / 32, ND = DP / 32;
     constexpr int IMG = BLKN * DP * (int)sizeof(T), WIN = (32 * NW + BLKN) * 4;
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     constexpr int SK = 68, SKEW = 32 * SK + 36;
     float* skew = reinterpret_cast<float*>(lds + 2 * BUF) + wv * SKEW;
     float run = 0.f;                                                    // running sum of offset (query tile) - (key tile) + lane - 32
-    if (BIAS == LINE)
+    if (SUM)
         for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
     const int ktile = kt0 + wv, ktiles = (p.Nk + 31) / 32;
     const bool any = __syncthreads_or(kok);                             // a workgroup whose keys are all masked has only zeros to store
@@ -631,7 +631,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 if (i * NT + tid < 32 * NW + BLKN) side[2 * BLKN + i * NT + tid] = win[i];
         }
     };
-    if (BIAS == LINE && !any && ktile < ktiles)                         // its slab rows are folded all the same
+    if (SUM && !any && ktile < ktiles)                         // its slab rows are folded all the same
         for (int g = 0; g < rep; ++g) {
             float* row = p.slab + ((((long)b * p.H + hk * rep + g) * ktiles + ktile) * p.ksplit + split) * p.slab_len;
             for (int i = lane; i < p.slab_len; i += 64) row[i] = 0.f;
@@ -689,15 +689,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 sa[qt][r] = pr * da[qt][r];                             // dS
                 da[qt][r] = pr;                                         // P   (a lane's columns are its own key's: a masked key's are not stored)
             }
-            if (BIAS == LINE) {
+            if (SUM) {
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
                     const f32x4 v = {sa[qt][4 * g4], sa[qt][4 * g4 + 1], sa[qt][4 * g4 + 2], sa[qt][4 * g4 + 3]};
                     *reinterpret_cast<f32x4*>(skew + (lane & 31) * SK + 36 + 8 * g4 + 4 * h) = kok ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
                 }
             }
-            float diag[BIAS == LINE ? 32 : 1];
-            if (BIAS == LINE) {
+            float diag[SUM ? 32 : 1];
+            if (SUM) {
                 // along the diagonals: lane l takes query - key = l - 32 of every key kk.  The lower half's offsets end with this tile of queries, the upper half's
                 // are the lower half's of the next one
 #pragma unroll
@@ -707,7 +707,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             td.product(da[qt], dv, lane);
             tq.product(sa[qt], dk, lane);
             if constexpr (sizeof(T) == 2 && DP == 32) tq.product(rest(sa[qt]), dk, lane);
-            if (BIAS == LINE) {
+            if (SUM) {
 #pragma unroll
                 for (int kk = 0; kk < 32; ++kk) run += diag[kk];
                 float* row = p.slab + ((((long)b * p.H + head) * ktiles + min(ktile, ktiles - 1)) * p.ksplit + split) * p.slab_len + (it % nqb) * BLKN + qt * 32;
@@ -900,15 +900,15 @@ int launch_q(const RelP& p, hipStream_t st) {
     LAUNCH_RET();
     return 0;
 }
-template <typename T, int DP, int NW, int BIAS>
+template <typename T, int DP, int NW, int BIAS, bool SUM>
 int launch_k(const RelP& p, hipStream_t st) {
     constexpr int BLKN = blk<T>();
     int bytes = 2 * (2 * BLKN * DP * (int)sizeof(T) + 2 * BLKN * 4 + (BIAS == LINE ? (32 * NW + BLKN) * 4 : BIAS == NONE ? 0 : BLKN * 4));
     if (BIAS == BOX) bytes += p.nd * 4;
-    if (BIAS == LINE) bytes += NW * (32 * 68 + 36) * 4;
-    const int rc = grant_lds(rel_k_kernel<T, DP, NW, BIAS>, bytes);
+    if (SUM) bytes += NW * (32 * 68 + 36) * 4;
+    const int rc = grant_lds(rel_k_kernel<T, DP, NW, BIAS, SUM>, bytes);
     if (rc) return rc;
-    hipLaunchKernelGGL((rel_k_kernel<T, DP, NW, BIAS>), dim3((p.Nk + 32 * NW - 1) / (32 * NW) * p.ksplit, p.Hkv, p.B), dim3(64 * NW), bytes, st, p);
+    hipLaunchKernelGGL((rel_k_kernel<T, DP, NW, BIAS, SUM>), dim3((p.Nk + 32 * NW - 1) / (32 * NW) * p.ksplit, p.Hkv, p.B), dim3(64 * NW), bytes, st, p);
     LAUNCH_RET();
     return 0;
 }
@@ -926,7 +926,8 @@ int launch_d(const RelP& p, hipStream_t st) {
 template <typename T, int DP, int NW>
 int pick_bias(const RelP& p, int what, hipStream_t st) {
     if (what == 3) return launch_d<T, DP, NW>(p, st);
-#define REL_ONE(BIAS) (what == 0 ? launch_q<T, DP, NW, 0, BIAS>(p, st) : what == 1 ? launch_q<T, DP, NW, 1, BIAS>(p, st) : launch_k<T, DP, NW, BIAS>(p, st))
+    if (what == 2 && p.bias == LINE && p.slab) return launch_k<T, DP, NW, LINE, true>(p, st);
+#define REL_ONE(BIAS) (what == 0 ? launch_q<T, DP, NW, 0, BIAS>(p, st) : what == 1 ? launch_q<T, DP, NW, 1, BIAS>(p, st) : launch_k<T, DP, NW, BIAS, false>(p, st))
     switch (p.bias) {
         case NONE: return REL_ONE(NONE);
         case BOX: return REL_ONE(BOX);

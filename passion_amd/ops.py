@@ -1844,8 +1844,8 @@ def rel_attention(q, k, v, table=None, grid=None, buckets=None, key_mask=None, s
     bucket of each of the prod(2 n - 1) offsets (see relative_buckets), None: one table row per offset, in raster order of (query cell - key cell).  A bucket outside the table has no bias, an entry
     at or below -1e30 excludes its pairs.  key_mask (B, Nk) bool / uint8: False = the key does not take part, whatever its k and v hold.  A query without a key gives 0 and zero gradients.
     scale: default D ** -0.5.  One query against many keys (a new token) runs split over the keys.
-    The table's gradient takes a workspace of about B H Nq Nk / 8 bytes over a 1D raster, of 4 H bytes for every pair of cells (and up to the batch times that while it
-    is small) over a grid.  -> (B, Nq, H, D)."""
+    The table's gradient, where it is wanted (table.requires_grad), takes a workspace of about B H Nq Nk / 8 bytes over a 1D raster, of 4 H bytes for every pair of cells
+    (and up to the batch times that while it is small) over a grid.  -> (B, Nq, H, D)."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"rel_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
     B, Nq, H, D = q.shape

@@ -446,6 +446,35 @@ def test_the_table_s_gradient_of_a_long_sequence_over_few_cells(cells):
 
 
 @pytest.mark.gpu
+@BOTH
+@pytest.mark.parametrize("grid,B,N,heads,D,nb", [((700,), 2, 700, 4, 64, 32), ((9, 9, 9), 1, 729, 4, 32, None), ((5, 5, 5), 4, 250, 4, 64, None), ((40, 40), 1, 1600, 2, 128, 12)])
+def test_a_frozen_table_pays_nothing_for_its_gradient(grid, B, N, heads, D, nb, dt):
+    """table without requires_grad: the other gradients bit for bit the same, and no memory for the partial sums (an eighth of a byte for every score of a 1D
+    raster's heads, four bytes for every pair of a grid's cells)"""
+    from passion_amd import ops
+    c = _make(B, N, N, heads, heads, D, dt, grid, nb=nb, mask="random")
+    want = _run(c)
+    on = {n: c[n].cuda() for n in ("q", "k", "v", "dout", "table", "mask")}
+    ins = [on[n].requires_grad_() for n in ("q", "k", "v")]
+    buckets = None if nb is None else c["buckets"].cuda()
+    peak = {}
+    for learned in (True, False):
+        table = on["table"].clone().requires_grad_(learned)
+        out = ops.rel_attention(*ins, table, grid, buckets, on["mask"], c["scale"])
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        stats = lambda which: torch.cuda.memory_stats()["requested_bytes.all." + which]        # (what is counted as allocated includes whole cached blocks, up to 1 MB more)
+        before = stats("current")
+        grads = torch.autograd.grad(out, ins + [table] * learned, on["dout"])
+        torch.cuda.synchronize()
+        peak[learned] = stats("peak") - before
+        assert all(torch.equal(g, want[n]) for n, g in zip(("dq", "dk", "dv"), grads))
+        del out, grads
+    slab = B * heads * N * N / 8 if len(grid) == 1 else 4 * heads * min(N, math.prod(grid)) ** 2
+    assert peak[True] - peak[False] >= 0.9 * slab
+
+
+@pytest.mark.gpu
 def test_no_tokens():
     from passion_amd import ops
     for B, Nq, Nk in ((0, 3, 3), (2, 0, 4), (2, 4, 0)):
@@ -540,3 +569,12 @@ def test_workspace_sizes_past_32_bits():
     assert size(40000, 33, 33, 60000, (1, 1, 40)) >= 40000 * 60000 * 2 * (64 + 32)                    # 1D: batch x heads x key tiles x (queries in blocks + 32)
     assert size(1, 1 << 22, 1 << 22, 1024, (4, 1, 1 << 20)) >= 1024 << 44                               # dense: heads x query cells x key cells
     assert size(1, 1 << 22, 10, 1024, (4, 1, 1 << 20)) >= (1024 << 22) * 64
+
+
+def test_workspace_without_the_table_s_gradient():
+    from passion_amd import _lib
+    size = lambda backward, grid, N, nb: _lib.load().passion_rel_attn_workspace_floats(1, backward, 1, N, N, 8, 8, 64, *grid, 0, 1, 1, nb)
+    for grid, N, slab in (((20, 20, 20), 8000, 8 * 8000 * 8000), ((1, 1, 65536), 65536, 8 * 65536 * 65536 // 32)):
+        assert size(1, grid, N, 32) >= slab
+        offsets = math.prod(2 * g - 1 for g in grid)
+        assert 0 < size(2, grid, N, 32) <= 8 * (offsets + N) + 256
