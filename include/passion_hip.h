@@ -464,7 +464,7 @@ int passion_prof_peek(passion_prof_rec_t* rec, int cap);
  * u = post(h), r = x + scale * gate * u, y = pre(r): the end of one block and the norm of the next (reference code/models/mmformer.py:230-256,
  * 284-300 has x + f(norm(x)); gate, scale and the norm after the block are this form's own).  x, r (and dr, dx): [B][N][C] of x_dtype; h, y (and dy, dh):
  * [B][N][C] of h_dtype; (f32, f32), (f32, bf16) or (bf16, bf16).  post / pre: 0 none, 1 LayerNorm, 2 RMSNorm, with f32 [C] weights (NULL: 1) and
- * biases (NULL: 0; LayerNorm only).  gate_mode: 0 none, 1 [B][C], 2 [B][N][C].  scale: f32 [C] or NULL.  1 <= C <= 8192, B <= 65530.
+ * biases (NULL: 0; LayerNorm only).  gate_mode: 0 none, 1 [B][C], 2 [B][N][C].  scale: f32 [C] or NULL.  1 <= C <= 8192, B <= 65530, N < 2^31 - 2^27.
  * stat: f32 [B][N][4] (NULL: not kept).  pre = 0: y is not written and may be NULL.
  * Backward: dr / dy may be NULL (zero).  dgate: of gate's shape and dtype.  dw_* / db_* / dscale: f32 [C], overwritten, NULL: not wanted.
  * part: passion_residual_norm_part_floats(B, N, C) floats.  Column sums are folded in a fixed order (no atomics). */

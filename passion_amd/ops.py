@@ -1761,8 +1761,8 @@ def residual_norm(x, h, post=None, pre=None, gate=None, scale=None):
             raise ValueError(f"residual_norm: gate {tuple(gate.shape)} has to be {tuple(x.shape)} or (B, 1, {C}) with x (B, N, {C})")
     if scale is not None and tuple(scale.shape) != (C,):
         raise ValueError(f"residual_norm: scale {tuple(scale.shape)} has to be ({C},)")
-    if N >= 2 ** 31 or B > 65530:
-        raise ValueError(f"residual_norm: {B} samples of {N} rows")
+    if N >= 2 ** 31 - 2 ** 27 or B > 65530:
+        raise ValueError(f"residual_norm: {B} samples of {N} rows (below 2^31 - 2^27)")
     if scale is not None and scale.dtype != torch.float32:
         scale = scale.float()
     ins = [_dense(t) for t in (x, h, gate, scale, w1, b1, w2, b2)]

@@ -263,6 +263,30 @@ def test_the_default_eps_is_the_module_s():
 
 
 @pytest.mark.gpu
+def test_as_many_rows_as_are_taken():
+    """the last rows of the longest sample there may be"""
+    from passion_amd import ops
+    N = 2 ** 31 - 2 ** 27 - 1
+    x = torch.zeros(N, 1, dtype=H, device="cuda")
+    h = torch.full_like(x, 2.0)
+    x[-5000:, 0] = torch.arange(5000, device="cuda") % 100
+    r = ops.residual_norm(x, h)
+    assert bool((r[:-5000] == 2).all()) and torch.equal(r[-5000:], x[-5000:] + 2)
+
+
+def test_more_rows_are_refused():
+    """the kernels count a sample's rows, and the steps past its end, in 32 bits"""
+    from passion_amd import _lib, ops
+    lib, N = _lib.load(), 2 ** 31 - 2 ** 27
+    assert 0 < lib.passion_residual_norm_part_floats(1, N - 1, 1) <= 2048 * 6 and lib.passion_residual_norm_part_floats(65530, N - 1, 8) > 0
+    fwd = lambda n: lib.passion_residual_norm_fwd(256, 0, 256, 0, None, None, 0, 0.0, None, 0, 0, None, None, None, 0, 0.0, 1, n, 1, 256, None, None, None)
+    assert lib.passion_residual_norm_part_floats(1, N, 1) == -1003 and fwd(N) == -1003 and fwd(2 ** 31 - 1) == -1003
+    x = torch.zeros(1, 1).expand(N, 1)
+    with pytest.raises(ValueError):
+        ops.residual_norm(x, x)
+
+
+@pytest.mark.gpu
 def test_no_rows():
     from passion_amd import ops
     x = torch.zeros(2, 0, 64, device="cuda", requires_grad=True)
