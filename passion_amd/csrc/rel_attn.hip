@@ -21,36 +21,39 @@
 
 namespace {
 
+constexpr int MAX_WG = 1 << 21;         // workgroups along x of the small kernels' launches: below 2^32 threads, past which a launch is cut off without an error
 constexpr int BOX_MAX = 4096;           // offsets whose table fits LDS beside the tiles (16 KB)
 
 // before the large kernels: workgroups [0, eb) form e[h][o] = log2 units of the head's bias at offset o, 256 / 8 offsets x 8 heads at a time; the others (backward)
-// delta[b][h][q] = dout . out, 16 lanes a row
+// delta[b][h][q] = dout . out, 16 lanes a row.  Both go on by their number of workgroups, at most MAX_WG
 template <typename T>
 __global__ __launch_bounds__(256) void rel_pre_kernel(RelP p, float* e, int eb) {
     if ((int)blockIdx.x < eb) {
-        const int o = blockIdx.x * 32 + (threadIdx.x & 31);
-        if (o >= p.nd) return;
-        const int c = p.buckets ? p.buckets[o] : o;
-        for (int h = threadIdx.x >> 5; h < p.H; h += 8) e[(long)h * p.nd + o] = rel_log2_bias(p.table, p.tdt, c, p.nb, h, p.H);
+        for (int o = blockIdx.x * 32 + (threadIdx.x & 31); o < p.nd; o += eb * 32) {
+            const int c = p.buckets ? p.buckets[o] : o;
+            for (int h = threadIdx.x >> 5; h < p.H; h += 8) e[(long)h * p.nd + o] = rel_log2_bias(p.table, p.tdt, c, p.nb, h, p.H);
+        }
         return;
     }
     const T *o = static_cast<const T*>(p.o), *dout = static_cast<const T*>(p.dout);
-    const int B = p.B, Nq = p.Nq, H = p.H, D = p.D;
-    const long row = ((long)(blockIdx.x - eb) * 256 + threadIdx.x) >> 4;             // (b Nq + q) H + h
+    const int Nq = p.Nq, H = p.H, D = p.D;
+    const long rows = (long)p.B * Nq * H;
     const int c = (threadIdx.x & 15) * 8;
-    float s = 0.f;
-    if (row < (long)B * Nq * H && c < D) {
+    for (long row = (long)(blockIdx.x - eb) * 16 + (threadIdx.x >> 4); row < rows; row += (long)(gridDim.x - eb) * 16) {             // (b Nq + q) H + h
+        float s = 0.f;
+        if (c < D) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const f32x4 a = load4(o + row * D + c + 4 * u), g = load4(dout + row * D + c + 4 * u);
+            for (int u = 0; u < 2; ++u) {
+                const f32x4 a = load4(o + row * D + c + 4 * u), g = load4(dout + row * D + c + 4 * u);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s = __builtin_fmaf(a[j], g[j], s);
+                for (int j = 0; j < 4; ++j) s = __builtin_fmaf(a[j], g[j], s);
+            }
         }
-    }
-    s = group16_sum(s);
-    if ((threadIdx.x & 15) == 0 && row < (long)B * Nq * H) {
-        const long bq = row / H;
-        p.delta[((bq / Nq) * H + row % H) * Nq + bq % Nq] = s;
+        s = group16_sum(s);
+        if ((threadIdx.x & 15) == 0) {
+            const long bq = row / H;
+            p.delta[((bq / Nq) * H + row % H) * Nq + bq % Nq] = s;
+        }
     }
 }
 
@@ -155,7 +158,9 @@ struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, n
 template <bool LINE_>
 __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, run = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), o = blockIdx.x * 64 + lane, h = blockIdx.y;
+    const int lane = threadIdx.x & 63, run = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
+    const int o0 = (blockIdx.z * gridDim.x + blockIdx.x) * 64, o = o0 + lane;                   // (z: past MAX_WG workgroups)
+    if (o0 >= f.nd) return;
     float s = 0.f;
     if constexpr (LINE_) {
         // the key tiles that may hold one of the workgroup's offsets, W of them from ta on, for every batch entry and part
@@ -166,7 +171,7 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
         for (int i = i0; i < i1; ++i) {
             const int part = bp & (f.ksplit - 1), b = bp >> f.klog;
             const int q0 = (int)((unsigned)(part * f.nqb) >> f.klog), q1 = (int)((unsigned)((part + 1) * f.nqb) >> f.klog);       // (in blocks)
-            const int from = f.base - 32 + q0 * f.blk, ta = (from - (int)blockIdx.x * 64 - 63 + 31) >> 5, t = ta + j, u = o - from + 32 * t;
+            const int from = f.base - 32 + q0 * f.blk, ta = (from - o0 - 63 + 31) >> 5, t = ta + j, u = o - from + 32 * t;
             const bool in = (unsigned)t < (unsigned)f.tiles && (unsigned)u < (unsigned)((q1 - q0) * f.blk + 32);
             const float v = f.slab[in ? ((((long)b * f.H + h) * f.tiles + t) * f.ksplit + part) * f.len + u : 0];
             s += in ? v : 0.f;
@@ -362,6 +367,7 @@ Ws bwd_ws(RelP& p, int dtype, bool want_table) {
     w.delta = take((long)p.B * p.H * p.Nq);
     p.nsplit = pick_split_bwd(tiles32(p.Nq) * p.H * p.B, p.Nk);
     p.ksplit = pick_split_bwd(tiles32(p.Nk) * p.Hkv * p.B, p.Nq);
+    while ((long)p.ksplit * ((p.Nq + 31) / 32) > (1 << 30)) p.ksplit /= 2;            // (rel_fold_kernel multiplies parts by blocks in 32 bits)
     const long rows = (long)p.B * p.H * p.Nq, krows = (long)p.B * p.Nk * p.Hkv;
     w.po = take(hmax(p.nsplit > 1 ? p.nsplit * rows * p.D : 0, p.ksplit > 1 ? 2 * p.ksplit * krows * p.D : 0));       // dQ's parts, then those of dK and dV
     w.pm = take(p.nsplit > 1 ? p.nsplit * rows : 0);
@@ -374,8 +380,8 @@ Ws bwd_ws(RelP& p, int dtype, bool want_table) {
     return w;
 }
 int pre(RelP& p, int dtype, float* e, hipStream_t st) {
-    const int eb = e ? (p.nd + 31) / 32 : 0;
-    const long db = p.delta ? ((long)p.B * p.Nq * p.H * 16 + 255) / 256 : 0;
+    const int eb = e ? (int)hmin((p.nd + 31) / 32, MAX_WG) : 0;
+    const long db = p.delta ? hmin(((long)p.B * p.Nq * p.H + 15) / 16, MAX_WG) : 0;
     if (dtype == PASSION_BF16) hipLaunchKernelGGL(rel_pre_kernel<bf16_t>, dim3((unsigned)(eb + db)), dim3(256), 0, st, p, e, eb);
     else hipLaunchKernelGGL(rel_pre_kernel<float>, dim3((unsigned)(eb + db)), dim3(256), 0, st, p, e, eb);
     LAUNCH_RET();
@@ -482,8 +488,10 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
             f.ld = f.KC;
             f.parts = 1;
         }
-        if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<true>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
-        else hipLaunchKernelGGL(rel_fold_kernel<false>, dim3((p.nd + 63) / 64, H), dim3(1024), 0, st, f);
+        const int groups = (p.nd + 63) / 64, wide = (int)hmin(groups, MAX_WG);
+        const dim3 wgs(wide, H, (groups + wide - 1) / wide);
+        if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<true>, wgs, dim3(1024), 0, st, f);
+        else hipLaunchKernelGGL(rel_fold_kernel<false>, wgs, dim3(1024), 0, st, f);
         LAUNCH_RET();
         if (buckets) {
             const bool few = nb <= 256;

@@ -475,6 +475,41 @@ def test_a_frozen_table_pays_nothing_for_its_gradient(grid, B, N, heads, D, nb, 
 
 
 @pytest.mark.gpu
+def test_more_query_rows_than_a_launch_has_sixteenths_of_its_threads():
+    """2^25 + 100 queries of 8 heads against 200 keys: the pass over out and dout before the backward takes 16 threads a row, past 2^32 in one launch.  All queries but the
+    last hundred are 0 with a gradient of 0, so the gradients are those of the short call"""
+    from passion_amd import ops
+    N, n = (1 << 25) + 100, 100
+    c = {k: v.cuda() if torch.is_tensor(v) else v for k, v in _make(1, n, 200, 8, 8, 8, H, seed=5).items()}
+    wide = {m: torch.zeros(1, N, 8, 8, dtype=H, device="cuda") for m in ("q", "dout")}
+    for m in wide:
+        wide[m][:, -n:] = c[m]
+    long = [t.requires_grad_() for t in (wide["q"], c["k"].clone(), c["v"].clone())]
+    out = ops.rel_attention(*long)
+    dq, dk, dv = torch.autograd.grad(out, long, wide["dout"])
+    assert not bool(dq[:, :-n].any())
+    want = _reference(c)
+    for name, got in (("out", out[:, -n:]), ("dq", dq[:, -n:]), ("dk", dk), ("dv", dv)):
+        near(got, want[name][0], U[H], name, room=want[name][1])
+
+
+@pytest.mark.gpu
+def test_more_offsets_than_a_launch_has_sixteenths_of_its_threads():
+    """a line of 2^27 + 1 places, 200 tokens on it: the expansion of the buckets and the sums by offset run over 2^28 + 1 offsets; the same as on a line of 300"""
+    from passion_amd import ops
+    L, n = (1 << 27) + 1, 300
+    c = {k: v.cuda() if torch.is_tensor(v) else v for k, v in _make(1, 200, 200, 1, 1, 16, H, (n,), nb=6, seed=6).items()}
+    step = lambda grid, buckets: torch.autograd.grad(ops.rel_attention(*leaves, grid, buckets), leaves, c["dout"])
+    leaves = [c[m].clone().requires_grad_() for m in ("q", "k", "v", "table")]
+    want = step((n,), c["buckets"])
+    buckets = torch.zeros(2 * L - 1, dtype=torch.int32, device="cuda")
+    buckets[L - n:L + n - 1] = c["buckets"]
+    got = step((L,), buckets)
+    assert all(torch.equal(a, b) for a, b in zip(got[:3], want[:3]))
+    near(got[3], want[3].double(), 2.0 ** -8, "dtable")
+
+
+@pytest.mark.gpu
 def test_no_tokens():
     from passion_amd import ops
     for B, Nq, Nk in ((0, 3, 3), (2, 0, 4), (2, 4, 0)):
