@@ -153,18 +153,21 @@ __global__ __launch_bounds__(256) void rel_join_kernel(const float* part, int n,
 // its own bucket (dt).
 //   LINE: slab rows (b, key tile, part of the queries) of len places: row t of the part that begins at query q holds offset o at place
 //         o - (gw - 1) - q_start + 32 + 32 t - q
-//   dense: M[z][h][a][c]: the pairs of a query cell a and the key cell = its cell - offset, where both lie on the grid
+//   DENSE: M[z][h][a][c]: the pairs of a query cell a and the key cell = its cell - offset, where both lie on the grid
+//   FEW:   the same, of tokens on few cells of a large grid: only the cells that hold a query whose key cell holds a key are walked (most offsets have none)
 struct FoldP { const float* slab; float* G; void* dt; long len; int tdt, B, H, nd, tiles, base; int gd, gh, gw, vol, q0, QC, KC, ld, parts, ksplit, klog, nqb, blk; };
-template <bool LINE_>
+enum { FOLD_LINE = 0, FOLD_DENSE = 1, FOLD_FEW = 2 };
+template <int MODE>
 __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, run = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
     const int o0 = (blockIdx.z * gridDim.x + blockIdx.x) * 64, o = o0 + lane;                   // (z: past MAX_WG workgroups)
     if (o0 >= f.nd) return;
     float s = 0.f;
-    if constexpr (LINE_) {
+    if constexpr (MODE == FOLD_LINE) {
         // the key tiles that may hold one of the workgroup's offsets, W of them from ta on, for every batch entry and part
-        const int W = (int)(f.len / 32) + 3, n = f.B * f.ksplit * W, i0 = (int)((long)n * run / 16), i1 = (int)((long)n * (run + 1) / 16);
+        const bool any = o0 + 63 >= f.base - 32 * f.tiles && o0 <= f.base + f.nqb * f.blk;           // (a line may be far longer than the tokens on it)
+        const int W = (int)(f.len / 32) + 3, n = any ? f.B * f.ksplit * W : 0, i0 = (int)((long)n * run / 16), i1 = (int)((long)n * (run + 1) / 16);
         int bp = i0 / W, j = i0 - bp * W;
 // (loads unconditional, eight in flight: a load under a condition is waited for before the next one)
 #pragma unroll 8
@@ -180,27 +183,39 @@ __global__ __launch_bounds__(1024) void rel_fold_kernel(FoldP f) {
     } else {
         const int sx = 2 * f.gw - 1, sy = 2 * f.gh - 1;
         const int dx = o % sx - (f.gw - 1), dy = o / sx % sy - (f.gh - 1), dz = o / sx / sy - (f.gd - 1);
-        // units of 8 cells along x of the rows (z, y) that have a partner; the query's cell counts from q_start (the raster may begin inside the grid)
-        const int nz = f.gd - abs(dz), ny = f.gh - abs(dy), z0 = max(0, dz), y0 = max(0, dy), XC = (f.gw + 7) / 8;
-        const int shift = (dz * f.gh + dy) * f.gw + dx, n = o < f.nd ? nz * ny * XC : 0, first = f.q0 % f.vol;
+        const int shift = (dz * f.gh + dy) * f.gw + dx, first = f.q0 % f.vol;              // the query's cell counts from q_start (the raster may begin inside the grid)
         const long part = (long)f.H * f.QC * f.ld;
         const float* m = f.slab + (long)h * f.QC * f.ld;
-        for (int z = 0; z < f.parts; ++z, m += part)
-            for (int u = run; __any(u < n); u += 16) {
-                const int row = u / XC, x8 = (u - row * XC) * 8, rz = row / ny, ry = row - rz * ny, cell = ((z0 + rz) * f.gh + y0 + ry) * f.gw + x8;
-                float v[8];
-                bool in[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int x = x8 + i, c = cell + i - shift;
-                    int a = cell + i - first;
-                    a = a < 0 ? a + f.vol : a;
-                    in[i] = u < n && x < f.gw && (unsigned)(x - dx) < (unsigned)f.gw && a < f.QC && c < f.KC;
-                    v[i] = m[in[i] ? (long)a * f.ld + c : 0];
+        if constexpr (MODE == FOLD_FEW) {
+            for (int seg = 0; seg < 2; ++seg) {                                              // the queries' cells [first, ..) and, where they go round, [0, ..)
+                const int lo = max(seg ? 0 : first, max(0, shift)), hi = min(seg ? first + f.QC - f.vol : min(first + f.QC, f.vol), min(f.vol, f.KC + shift));
+                for (int cell = lo + run; __any(cell < hi && o < f.nd); cell += 16) {
+                    const int r = cell / f.gw, x = cell - r * f.gw, z = r / f.gh, y = r - z * f.gh, a = cell - first + (seg ? f.vol : 0);
+                    if (cell >= hi || o >= f.nd || (unsigned)(x - dx) >= (unsigned)f.gw || (unsigned)(y - dy) >= (unsigned)f.gh || (unsigned)(z - dz) >= (unsigned)f.gd) continue;
+                    for (int i = 0; i < f.parts; ++i) s += m[i * part + (long)a * f.ld + cell - shift];
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s += in[i] ? v[i] : 0.f;
             }
+        } else {
+            // units of 8 cells along x of the rows (z, y) that have a partner
+            const int nz = f.gd - abs(dz), ny = f.gh - abs(dy), z0 = max(0, dz), y0 = max(0, dy), XC = (f.gw + 7) / 8;
+            const int n = o < f.nd ? nz * ny * XC : 0;
+            for (int z = 0; z < f.parts; ++z, m += part)
+                for (int u = run; __any(u < n); u += 16) {
+                    const int row = u / XC, x8 = (u - row * XC) * 8, rz = row / ny, ry = row - rz * ny, cell = ((z0 + rz) * f.gh + y0 + ry) * f.gw + x8;
+                    float v[8];
+                    bool in[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int x = x8 + i, c = cell + i - shift;
+                        int a = cell + i - first;
+                        a = a < 0 ? a + f.vol : a;
+                        in[i] = u < n && x < f.gw && (unsigned)(x - dx) < (unsigned)f.gw && a < f.QC && c < f.KC;
+                        v[i] = m[in[i] ? (long)a * f.ld + c : 0];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s += in[i] ? v[i] : 0.f;
+                }
+        }
     }
     red[run][lane] = s;
     __syncthreads();
@@ -278,6 +293,10 @@ int bias_mode(const RelP& p) {
 }
 // few query rows: all heads of a key / value head in one tile, the bias read straight from the table (an expansion of all offsets would cost more)
 bool few_rows(const RelP& p) { return (long)p.Nq * (p.H / p.Hkv) <= 32 && p.Nq <= 16; }
+
+// tokens on few of the grid's cells: the sums by offset walk the tokens' cells and not the grid's.  8 heads, the grid's cells / the tokens': 200 tokens on 64^3 cells 510 ms /
+// 0.92 ms (and times 64 with every doubling of the sides), 300 or 500 on 16^3 190 us / 27 to 43 us, 120 on 10^3 33 / 9 us
+bool few_cells(int QC, int KC, int vol) { return 8 * hmin(QC, KC) < vol; }
 
 // the forward's key ranges.  Few rows: a block of keys a workgroup up to 2048 of them (all of a short cache in flight at once); else until there is a wavefront a SIMD,
 // two blocks each at least
@@ -490,8 +509,9 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
         }
         const int groups = (p.nd + 63) / 64, wide = (int)hmin(groups, MAX_WG);
         const dim3 wgs(wide, H, (groups + wide - 1) / wide);
-        if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<true>, wgs, dim3(1024), 0, st, f);
-        else hipLaunchKernelGGL(rel_fold_kernel<false>, wgs, dim3(1024), 0, st, f);
+        if (p.bias == 2) hipLaunchKernelGGL(rel_fold_kernel<FOLD_LINE>, wgs, dim3(1024), 0, st, f);
+        else if (few_cells(f.QC, f.KC, f.vol)) hipLaunchKernelGGL(rel_fold_kernel<FOLD_FEW>, wgs, dim3(1024), 0, st, f);
+        else hipLaunchKernelGGL(rel_fold_kernel<FOLD_DENSE>, wgs, dim3(1024), 0, st, f);
         LAUNCH_RET();
         if (buckets) {
             const bool few = nb <= 256;

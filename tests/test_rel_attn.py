@@ -510,6 +510,16 @@ def test_more_offsets_than_a_launch_has_sixteenths_of_its_threads():
 
 
 @pytest.mark.gpu
+@BOTH
+@pytest.mark.parametrize("grid,Nq,Nk,q0,nb", [((200, 200, 200), 300, 300, 0, 7), ((300, 4, 500), 130, 700, 597900, 64), ((30, 40, 50), 700, 90, 59500, None), ((5000,), 64, 64, 4970, 12),
+                                              ((6, 7, 8), 40, 336, 320, None), ((6, 7, 8), 336, 41, 100, None), ((20, 30), 74, 600, 570, 9), ((20000003,), 100, 130, 40, 5)])
+def test_few_tokens_of_a_large_grid(grid, Nq, Nk, q0, nb, dt):
+    """queries on few of the cells, and such that go round the raster's end: the sums by offset walk the tokens' cells alone (once, all cells for every offset: 40 s over
+    200^3 cells by count, hours at the largest grid that is taken)"""
+    _check(_make(1, Nq, Nk, 2, 1, 16, dt, grid, nb=nb, q0=q0, mask="random"))
+
+
+@pytest.mark.gpu
 def test_no_tokens():
     from passion_amd import ops
     for B, Nq, Nk in ((0, 3, 3), (2, 0, 4), (2, 4, 0)):
