@@ -288,7 +288,7 @@ long tiles32(long n) { return (n + 31) / 32; }
 // which way to the bias: a 1D raster without wrap-around by windows, a small box of offsets from LDS, else from memory
 int bias_mode(const RelP& p) {
     if (!p.table) return 0;
-    if (p.gd == 1 && p.gh == 1 && p.Nk <= p.gw && p.q0 + p.Nq <= p.gw) return 2;
+    if (p.gd == 1 && p.gh == 1 && p.Nk <= p.gw && (long)p.q0 + p.Nq <= p.gw) return 2;
     return p.nd <= BOX_MAX ? 1 : 3;
 }
 // few query rows: all heads of a key / value head in one tile, the bias read straight from the table (an expansion of all offsets would cost more)

@@ -616,6 +616,14 @@ def test_workspace_sizes_past_32_bits():
     assert size(1, 1 << 22, 10, 1024, (4, 1, 1 << 20)) >= (1024 << 22) * 64
 
 
+def test_a_line_is_chosen_in_64_bits():
+    """queries q_start .. q_start + Nq - 1 with a last one past 2^31 go round a line of 40 places: the sums of a line (about a float a query) are not theirs"""
+    from passion_amd import _lib
+    size = lambda q0: _lib.load().passion_rel_attn_workspace_floats(1, 1, 1, 1 << 30, 1, 1, 1, 8, 1, 1, 40, q0, 1, 0, 79)
+    delta = 1 << 30
+    assert delta < size(1 << 29) < delta + (1 << 25) and size(1 << 30) == size(1 << 29)
+
+
 def test_workspace_without_the_table_s_gradient():
     from passion_amd import _lib
     size = lambda backward, grid, N, nb: _lib.load().passion_rel_attn_workspace_floats(1, backward, 1, N, N, 8, 8, 64, *grid, 0, 1, 1, nb)
