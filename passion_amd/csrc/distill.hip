@@ -22,6 +22,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 constexpr int SMALL_V = 512, MAX_K = 1024;
+constexpr float MIN_T = 0.99e-18f, MAX_T = 1.01e18f;          // T^2 and log2(e) / T are normal f32 values
 
 struct DsP {
     const void* s;            // [R][V] student logits
@@ -359,7 +360,7 @@ int launch(const DsP& p, hipStream_t st) {
 }
 
 bool bad(int64_t R, int V, int K, float T, int dt, int tvdt) {
-    return R < 1 || V < 1 || K < 1 || K > MAX_K || !(T > 0.f) || (dt != PASSION_F32 && dt != PASSION_BF16) || (tvdt != PASSION_F32 && tvdt != PASSION_BF16);
+    return R < 1 || V < 1 || K < 1 || K > MAX_K || !(T >= MIN_T && T <= MAX_T) || (dt != PASSION_F32 && dt != PASSION_BF16) || (tvdt != PASSION_F32 && tvdt != PASSION_BF16);
 }
 
 }  // namespace

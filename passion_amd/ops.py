@@ -1787,8 +1787,8 @@ def topk_distill(logits, values, index, temp=1.0):
         if t.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"topk_distill: dtype {t.dtype}")
     temp = float(temp)
-    if not 0.0 < temp < float("inf"):
-        raise ValueError(f"topk_distill: temperature {temp}")
+    if not 1e-18 <= temp <= 1e18:
+        raise ValueError(f"topk_distill: temperature {temp} (1e-18 to 1e18)")
     lead = logits.shape[:-1]
     s = _dense(logits.reshape(-1, V))
     tv, ti = values.detach().reshape(-1, K).contiguous(), index.reshape(-1, K).contiguous()

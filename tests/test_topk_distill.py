@@ -234,6 +234,28 @@ def test_refusals():
         ops.topk_distill(s, t, i)
 
 
+def test_temperatures_past_f32_are_refused():
+    """the kernels hold T^2 and log2(e) / T in f32: temperatures whose square or reciprocal leaves its normal range gave NaN or 0"""
+    from passion_amd import _lib, ops
+    s, t, i = torch.zeros(3, 8), torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.long)
+    for T in (1e-300, 1e-40, 1e-20, 2e19, 1e300):
+        with pytest.raises(ValueError):
+            ops.topk_distill(s, t, i, T)
+    lib = _lib.load()
+    for T in (1e-40, 1e-20, 2e19, float("inf"), float("nan"), -1.0):
+        assert lib.passion_topk_distill_fwd(256, 0, 256, 0, 256, 0, 2, 8, 2, T, 256, None, None) == -1003
+        assert lib.passion_topk_distill_bwd(264, 0, 256, 0, 256, 0, 2, 1000, 2, T, 256, 256, 256, None) == -1003
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1e-18, 1e18])
+@pytest.mark.parametrize("V", [9, 700])
+def test_the_extreme_temperatures(V, T):
+    """logits in proportion to T: the loss is T^2 times that of T = 1"""
+    s, t, i, g = _make(6, V, 3, F, seed=3)
+    _check(s * T, t * T, i, g, T)
+
+
 def test_c_entry_refuses_on_the_host():
     from passion_amd import _lib
     lib = _lib.load()
