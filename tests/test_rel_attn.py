@@ -201,6 +201,31 @@ def test_many_workgroups_of_four(B, dt):
 
 @pytest.mark.gpu
 @BOTH
+@pytest.mark.parametrize("D", [96, 128])
+@pytest.mark.parametrize("grid,nb,N", [((1003,), 32, 1000), ((8, 8, 8), None, 1000), ((10, 10, 10), None, 1000), (None, None, 1000)])
+def test_wide_heads_by_workgroups_of_four(grid, nb, N, D, dt):
+    """widths over 64 in enough tiles for four wavefronts a workgroup in every kernel (the registers that the width leaves differ by their number)"""
+    _check(_make(4, N, N, 8, 8, D, dt, grid, nb=nb, mask="runs"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grid,B,Nq,Nk,heads,Hkv,D,nb,q0,mask", [((5, 5, 5), 1, 125, 125, 8, 8, 64, None, 0, None), ((500,), 2, 500, 500, 4, 2, 128, 32, 0, "runs"),
+                                                                   ((40, 40), 1, 300, 1600, 2, 2, 32, 12, 100, "random"), (None, 1, 700, 700, 2, 1, 96, None, 0, None),
+                                                                   ((3000,), 3, 1, 3000, 8, 2, 64, 32, 2999, "random"), ((6, 7, 8), 2, 336, 336, 4, 4, 8, None, 0, None)])
+def test_f32_is_f32(grid, B, Nq, Nk, heads, Hkv, D, nb, q0, mask):
+    """the Euclidean norm of the error, where independent roundings add as squares.  A score sums D <= 128 products one after another: sqrt(128) * 2^-24 of partial sums of
+    order 3, 2e-6 of error, and so much relative error in a probability; products with v, dout, q, k add as much again, and dP - delta cancels up to a few times.  1e-5 and
+    3e-5 of the norm leave a factor of a few; operands of 11 bits would be off by sqrt(128) * 2^-12 / 3 = 1e-3"""
+    c = _make(B, Nq, Nk, heads, Hkv, D, F, grid, nb=nb, q0=q0, mask=mask)
+    got, want = _run(c), _reference(c)
+    for n in got:
+        w = want[n][0]
+        off = float((got[n].double() - w).norm() / w.norm())
+        assert off <= (1e-5 if n in ("out", "dv") else 3e-5), (n, off)
+
+
+@pytest.mark.gpu
+@BOTH
 @pytest.mark.parametrize("grid", [(300,), (5, 6, 10), (40, 40), None])
 @pytest.mark.parametrize("Nq", [1, 300])
 def test_masked_keys_may_hold_anything(grid, Nq, dt):

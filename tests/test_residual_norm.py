@@ -134,6 +134,14 @@ def test_widths(C, tx, th):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tx,th", [(F, F), (F, H), (H, H)])
+@pytest.mark.parametrize("C,kind,gate", [(2051, "layer", "token"), (4095, "rms", "sample"), (4099, "layer", "sample"), (6001, "rms", "token"), (8191, "layer", None), (6008, "rms", "token")])
+def test_wide_rows_of_odd_widths(C, kind, gate, tx, th):
+    """rows of more than 2048 channels that start off the 16-byte points: the scalar forms of 512 and 1024 threads, forward and backward"""
+    _check(_inputs(2, 7, C, tx, th, gate, True), _mods(C, kind, 1, "cuda"), _mods(C, "layer", 2, "cuda"))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 @pytest.mark.parametrize("gate", [None, "sample", "token"])
 @pytest.mark.parametrize("scale", [False, True])
