@@ -14,7 +14,8 @@
 //    lane, one 16-byte load a row).
 // Sums and exponentials are f32; the gradient rounds once.  Exponents are differences of logits times log2(e) / T, and a row's largest logit and the log of its sum stay
 // apart: masked classes may hold their type's lowest value (log2(e) / T times that is past the type's range below T = 1.44), and a large common offset costs no bits.
-// 4096 x 50000 bf16, K = 32: forward 119 us (3.45 TB/s: what a read-only pass reaches on this card), backward 157 (5.2 TB/s of reads and writes).
+// 4096 x 50000 bf16, K = 32: forward 119 us (3.44 TB/s; a large library maximum or sum, reading alone as well, reaches 3.7 to 4.0), backward 160 (5.1 TB/s of reads and writes).
+// The row form against the register form at V <= 512, f32, K = 4, with the gradient: 200000 x 104 689 / 92 us, 100000 x 512 383 / 193, 64 x 512 8.2 / 10.1.
 #include "common.h"
 #include "passion_hip.h"
 
@@ -344,7 +345,8 @@ int launch(const DsP& p, hipStream_t st) {
         }
     } else {
         if (BWD && !aligned) return -1005;
-        // few long rows: 1024 threads a row keep the whole row in flight; many rows: 256 threads, several rows a CU
+        // few long rows: 1024 threads a row keep the whole row in flight; many rows: 256 threads, several rows a CU.  bf16, K = 8, with the gradient, 1024 / 256 threads: 64 x 32001 13.7 / 14.2 us,
+        // 256 x 130000 39.6 / 42.0, 2000 x 32001 109 / 72.  Between (more rows than CUs, fewer than 1024) 256 are faster already: 512 x 32001 32.6 / 23.1, 1000 x 32001 60 / 38.5
         const bool wide = p.R < 1024 && p.V >= 4096;
         const dim3 grid((unsigned)hmin(p.R, 1L << 20));
         if (BWD) {

@@ -4,17 +4,19 @@
 // q_start + i.  With o(i, j) the index of cell_i - cell_j among the (2 gd - 1)(2 gh - 1)(2 gw - 1) offsets:
 //     s_ij = scale q_i . k_j + table[buckets[o(i, j)]][head]       (masked keys and entries at or below -1e30 are excluded)
 //     p_i = softmax_j(s_ij), out_i = sum_j p_ij v_j                 (a row with nothing left: 0)
-// backward, from the saved row log-sum-exp, with nothing of size Nq x Nk in memory:
+// backward, from the saved row log-sum-exp, the probabilities formed again (only the table's gradient keeps partial sums: over a grid one f32 a pair of cells and head, as
+// large as a head's scores where every cell holds one token, and up to the batch times that while it is small; over a 1D raster 1/32 of the scores of all heads):
 //     delta_i = dout_i . out_i,  dS = p (dout v^T - delta),  dq = scale dS k,  dk = scale dS^T q,  dv = p^T dout,  dtable[c] = sum over pairs of bucket c of dS
 // The reference's SelfAttention (code/models/mmformer.py:192-227) has learned absolute positions instead; its tokens are such a grid.
 //
 // Two backward kernels as in flash_attn.hip: query-major (dq) and key-major (dk, dv: the heads that share a key / value head sum in registers), and the table's sums
 // (rel_attn_body.h); all free of atomics.
 //
-// Bound: long sequences by the matrix pipe and the vector arithmetic per score (exponential, bias, conversions), one token by the latency of a chain of loads.  Measured, bf16:
-//   8000 x 8000 tokens, 8 heads of 128 on 4, 1D table: forward 331 us (792 TF), dq 546 (720 TF), dk / dv / diagonal sums 810 (647 TF), fold 44;
-//   4 x 2048 x 2048, 8 heads of 64, 8^3 cells, 30 % of the keys masked: forward 75, dq 85, dk / dv 93, the table's dense sums 84, fold 17 us;
-//   4 x 1 x 6000, 8 heads of 64 on 2: 10 + 6 us (12.4 MB of cache).
+// Bound: long sequences by the matrix pipe and the vector arithmetic per score (exponential, bias, conversions), one token by the latency of a chain of loads.  Measured, bf16
+// (kernel times; they follow the clock, 331 to 372 us for the first from box to box):
+//   8000 x 8000 tokens, 8 heads of 128 on 4, 1D table: forward 329 us (797 TF), dq 509 (772 TF), dk / dv / diagonal sums 797 (658 TF), fold 42;
+//   4 x 2048 x 2048, 8 heads of 64, 8^3 cells, 30 % of the keys masked: forward 74, dq 84, dk / dv 93, the table's dense sums 80, fold 17 us;
+//   4 x 1 x 6000, 8 heads of 64 on 2: 9.5 + 6 us (12.4 MB of cache).
 #include "common.h"
 #include "passion_hip.h"
 #include "rel_attn.h"
@@ -22,7 +24,7 @@
 namespace {
 
 constexpr int MAX_WG = 1 << 21;         // workgroups along x of the small kernels' launches: below 2^32 threads, past which a launch is cut off without an error
-constexpr int BOX_MAX = 4096;           // offsets whose table fits LDS beside the tiles (16 KB)
+constexpr int BOX_MAX = 4096;           // offsets whose table is read from LDS (16 KB beside the tiles)
 
 // before the large kernels: workgroups [0, eb) form e[h][o] = log2 units of the head's bias at offset o, 256 / 8 offsets x 8 heads at a time; the others (backward)
 // delta[b][h][q] = dout . out, 16 lanes a row.  Both go on by their number of workgroups, at most MAX_WG
@@ -285,21 +287,26 @@ __global__ __launch_bounds__(256) void rel_bucket_many_kernel(const float* G, co
 int blk_of(int dtype) { return dtype == PASSION_BF16 ? 64 : 32; }
 long tiles32(long n) { return (n + 31) / 32; }
 
-// which way to the bias: a 1D raster without wrap-around by windows, a small box of offsets from LDS, else from memory
+// which way to the bias: a 1D raster without wrap-around by windows, a small box of offsets from LDS, else from memory.  Forward + backward, 8 heads of 64, from LDS / from memory:
+// 4 x 2048^2 over 8^3 cells 370 / 397 us (forward alone 71 / 82), 2 x 2000^2 of 32 over 5^3 280 / 352, f32 2048^2 547 / 570; 2 x 512^2 over 8^3 97 / 95.  Tables over 16 KB cost a
+// workgroup a CU: 9^3 cells 138 / 137 (heads of 128: 236 / 211), 12^3 592 / 396
 int bias_mode(const RelP& p) {
     if (!p.table) return 0;
     if (p.gd == 1 && p.gh == 1 && p.Nk <= p.gw && (long)p.q0 + p.Nq <= p.gw) return 2;
     return p.nd <= BOX_MAX ? 1 : 3;
 }
-// few query rows: all heads of a key / value head in one tile, the bias read straight from the table (an expansion of all offsets would cost more)
+// few query rows: all heads of a key / value head in one tile, the bias read straight from the table.  Against the ordinary way (expansion of all offsets first), whole call, bf16:
+// 4 x 1 x 6000 tokens, 8 heads of 64 on 2: 14.9 / 19.9 us (f32 26.5 / 33.2), 1 x 16 x 6000 14.2 / 17.8.  Not better where heads share nothing and workgroups are many: 16 x 1 x 1000,
+// 8 heads on 8, 30 / 24 us, f32 1 x 16 x 6000 27 / 23
 bool few_rows(const RelP& p) { return (long)p.Nq * (p.H / p.Hkv) <= 32 && p.Nq <= 16; }
 
 // tokens on few of the grid's cells: the sums by offset walk the tokens' cells and not the grid's.  8 heads, the grid's cells / the tokens': 200 tokens on 64^3 cells 510 ms /
 // 0.92 ms (and times 64 with every doubling of the sides), 300 or 500 on 16^3 190 us / 27 to 43 us, 120 on 10^3 33 / 9 us
 bool few_cells(int QC, int KC, int vol) { return 8 * hmin(QC, KC) < vol; }
 
-// the forward's key ranges.  Few rows: a block of keys a workgroup up to 2048 of them (all of a short cache in flight at once); else until there is a wavefront a SIMD,
-// two blocks each at least
+// the forward's key ranges.  Few rows: a block of keys a workgroup up to 2048 of them (all of a short cache in flight at once: 4 x 1 x 6000 14.9 us, up to 512 of them 16.7; a long cache pays
+// for the join: 1 x 1 x 60000 51 and 31 us); else until there is a wavefront on three of four SIMDs, two blocks each at least: 128 x 2048, 8 heads of 64, whole / in parts 73 / 23 us,
+// 1000^2 40 / 21 (41 with a limit of 256 wavefronts, 29 with one of 2048), 64 x 8000 276 / 21
 int pick_split(const RelP& p, int dtype) {
     const long tiles = (p.pack ? tiles32((long)p.Nq * (p.H / p.Hkv)) * p.Hkv : tiles32(p.Nq) * p.H) * p.B;
     const int nblk = (p.Nk + blk_of(dtype) - 1) / blk_of(dtype);
@@ -316,7 +323,8 @@ int pick_split_bwd(long tiles, int n) {
     while (tiles * s < 768 && n / (2 * s) >= 128) s *= 2;
     return s;
 }
-// wavefronts a workgroup: as many as leave every CU a workgroup; they share the staged tiles.  Key-major with heads over 64 wide: LDS and registers hold one workgroup a CU,
+// wavefronts a workgroup, which share the staged tiles: forward + backward over a line, 8 heads of 64, bf16, by one / two / four: 512^2 74 / 59 / 57 us, 1024^2 143 / 93 / 80, 4 x 1024^2
+// 365 / 163 / 131 (f32 675 / 501 / 431); the limits are those of one workgroup a CU, and below them two are the choice, though four are faster there too (3 x 1024^2, 768 wavefronts: 160 / 127).  Key-major with heads over 64 wide: LDS and registers hold one workgroup a CU,
 // and a workgroup more than there are CUs is a second round: four as soon as two would begin one (1077^2, 8 heads of 96 on 2, f32, 544 wavefronts: forward + backward 804 us by two, 481 by four)
 int pick_waves(long rows32, long others, bool alone = false) {
     const long waves = rows32 * others;

@@ -181,9 +181,10 @@ template <typename T, int DP, int NT> struct Tile {
     }
     static __device__ __forceinline__ constexpr uint64_t all_rows() { return blk<T>() == 64 ? ~0ull : 0xffffffffull; }
 };
-// what the rounding of dS to a bf16 operand leaves.  dS is rounded once for dQ and dK (2^-9 of each term, the largest error there is beside the rounding of the result);
-// heads up to 32 wide add the product of the rest (4000^2, 8 heads of 32: dQ off by 1.7e-3 of its norm instead of
-// 2.4e-3, forward + backward 339 us instead of 311); wider ones would pay a product as large as the first for the same bits
+// what the rounding of dS to a bf16 operand leaves.  In bf16 the probabilities (for out and dV) and dS (for dQ and dK) are rounded once to the matrix operand's type, as much as the
+// result itself is: out, dV, dQ and dK are off by 2.3 to 2.4e-3 of their norm where the rounding of the result alone is 1.7e-3.  Heads up to 32 wide add the product of dS's
+// rest, which brings dQ and dK to 1.7e-3 (4000^2, 8 heads of 32: forward + backward 339 us instead of 311).  For wider ones it was measured and left: dQ and dK at 1.7e-3 as well, but
+// 1D 2000^2, 8 heads of 64: dQ 31 -> 35 us, dK / dV 53 -> 69 (no registers left); 8000^2, 8 heads of 128 on 4: 1690 -> 1815 us in all
 __device__ __forceinline__ f32x16 rest(const f32x16& a) {
     f32x16 r;
 #pragma unroll

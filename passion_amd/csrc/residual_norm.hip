@@ -4,7 +4,7 @@
 // and channel or per token and channel, scale: per channel.  The glue of the reference's Transformer (code/models/mmformer.py:230-256,
 // 284-300: x + dropout(f(norm(x))), norm of the next block) in the form a gated, post-normed block has it.
 //
-// Bound by HBM: forward reads x, h (, a token gate) and writes r, y once; backward reads x, h, dr, dy and writes dx, dh.  The backward
+// Bound by memory: forward reads x, h (, a token gate) and writes r, y once; backward reads x, h, dr, dy and writes dx, dh.  The backward
 // forms r again from x and h instead of reading it: the same bytes, and the parameter gradients see the unrounded r.
 //
 // Layout: a row = C channels over TPR threads (a power of two, 8 channels a thread: one 16-byte access a thread and bf16 tensor), 256 / TPR
@@ -14,7 +14,10 @@
 // Column sums of the backward: in registers over the workgroup's rows (of one sample), one partial per workgroup, folded in
 // workgroup order by a second kernel: no atomics, results repeat bit for bit.
 // All arithmetic and every sum is f32; x, h, y, r and the gradients round once when they are stored.
-// 8 x 4096 x 2048 bf16 with a sample's gate: forward 118 us, backward 179 (4.5 TB/s), fold of the column sums 12.
+// 8 x 4096 x 2048 bf16 with a sample's gate: forward 117 us (4.6 TB/s), backward 180 (4.5 TB/s; two wavefronts a SIMD with one row of each in flight), fold of the column sums 13.
+// 3 x 4001 x 765 f32 with a token's gate: 38 + 68 + 9 us; rows of an odd width are read and written 4 bytes a thread.
+// Rows of more than 4096 channels: 1024 threads have 128 registers each, the backward wants about 230 and spills 210 to 254 (odd widths 417 to 538; their forward 287): 67 million elements
+// bf16 forward / backward at 4096 wide 207 / 201 us, 8192 wide 209 / 1657, 4104 wide 295 / 2783, 6001 wide 1127 / 2694.
 #include "common.h"
 #include "passion_hip.h"
 
@@ -438,7 +441,8 @@ int threads_per_row(int C) {
     return t;
 }
 
-// rows of one sample a workgroup: enough workgroups for two to four per CU, whole rounds of its rows
+// rows of one sample a workgroup, whole rounds of its rows: at most 2048 workgroups forward (8 x 4096 x 2048 bf16 145 us, by 1024 157, by 4096 137; 12003 x 768 f32 49, 40, 42; 20000 x 256 bf16
+// 13.3, 17.2, 19.9) and 1024 backward, each of which leaves a row of column sums (forward + backward there 319 us, by 512 307, by 2048 326; 104, 97, 117; 39.6, 34.8, 42.5)
 int pick_chunk(int B, int N, int rpb, int target) {
     const long want = (long)target / B > 0 ? target / B : 1;
     long chunk = (N + want - 1) / want;

@@ -1704,6 +1704,7 @@ def region_mix(prob, mask, w, ys):
 
 # ------------------------------------------------------------------------------------------------
 # the residual step between two transformer blocks, distillation from a teacher's top logits
+# (these and rel_attention take plain eager tensors and have first derivatives only: dual tensors, traces and torch.func transforms are refused)
 # ------------------------------------------------------------------------------------------------
 def _one_device(*tensors):
     """all that are there on one GPU"""
