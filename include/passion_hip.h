@@ -501,7 +501,7 @@ int passion_topk_distill_bwd(const void* logits, int dtype, const void* values, 
  * lse: f32 [B][H][Nq] in log2 units (NULL: not kept).  workspace: passion_rel_attn_workspace_floats(...) floats, 16-byte aligned, owned by this call until the
  * stream has passed it; backward: 0 forward, 1 backward with the table's gradient (whose partial sums are most of it: over a grid as large as a head's scores, over a
  * 1D raster about 1/32 of the scores of all heads), 2 backward without (dtable NULL).  Backward recomputes the probabilities; dtable of the table's shape and dtype,
- * NULL: not wanted.  No atomics between wavefronts: results repeat bit for bit. */
+ * NULL: not wanted; with buckets, nb > 256 and offsets x max(nb H, 2^19) past 2^46 it is refused (-1003).  No atomics between wavefronts: results repeat bit for bit. */
 int64_t passion_rel_attn_workspace_floats(int dtype, int backward, int B, int Nq, int Nk, int H, int Hkv, int D, int gd, int gh, int gw, int q_start,
                                           int has_table, int has_buckets, int nb);
 int passion_rel_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype, int B,

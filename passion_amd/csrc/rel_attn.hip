@@ -249,7 +249,8 @@ __global__ __launch_bounds__(256) void rel_copies_kernel(RelP p, int ld, int qc,
     if (threadIdx.x == 0) out[((long)h * qc + a0) * kc + c0] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// dtable[c][h] = sum of G[h][o] over the offsets of bucket c.  Few buckets: a workgroup a bucket; many: a thread a bucket, the map in LDS
+// dtable[c][h] = sum of G[h][o] over the offsets of bucket c, in their order.  Few buckets: a workgroup a bucket; many: a thread a bucket, the map through LDS, four offsets a read
+// (an offset at a time waited for each read: 52 ns an offset)
 template <typename TT>
 __global__ __launch_bounds__(256) void rel_bucket_few_kernel(const float* G, const int* buckets, TT* dt, int nd, int H) {
     __shared__ float red[4];
@@ -267,8 +268,8 @@ __global__ __launch_bounds__(256) void rel_bucket_few_kernel(const float* G, con
 }
 template <typename TT>
 __global__ __launch_bounds__(256) void rel_bucket_many_kernel(const float* G, const int* buckets, TT* dt, int nd, int nb, int H) {
-    __shared__ int bk[1024];
-    __shared__ float gv[1024];
+    __shared__ __attribute__((aligned(16))) int bk[1024];
+    __shared__ __attribute__((aligned(16))) float gv[1024];
     const int c = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
     float s = 0.f;
     for (int o0 = 0; o0 < nd; o0 += 1024) {
@@ -278,8 +279,15 @@ __global__ __launch_bounds__(256) void rel_bucket_many_kernel(const float* G, co
             gv[i] = o0 + i < nd ? G[(long)h * nd + o0 + i] : 0.f;
         }
         __syncthreads();
-        for (int i = 0; i < 1024; ++i)
-            if (bk[i] == c) s += gv[i];
+#pragma unroll 4
+        for (int i = 0; i < 1024; i += 4) {
+            const int4 b = *reinterpret_cast<const int4*>(bk + i);
+            const f32x4 g = *reinterpret_cast<const f32x4*>(gv + i);
+            s += b.x == c ? g[0] : 0.f;
+            s += b.y == c ? g[1] : 0.f;
+            s += b.z == c ? g[2] : 0.f;
+            s += b.w == c ? g[3] : 0.f;
+        }
     }
     if (c < nb) dt[(long)c * H + h] = from_f32<TT>(s);
 }
@@ -366,6 +374,10 @@ long slab_floats(RelP& p, int dtype) {
     return (long)p.parts * p.H * p.QC * nkb * blk;
 }
 
+// more than 256 buckets: the last sum reads every offset for every 256 of them: 11.5 ns an offset (2 10^6 offsets, 10^4 to 10^5 buckets: 24 ms in all; 52 ns by one offset a read: 106 ms), and
+// 1.4 10^13 pairs of offset and bucket a second where they fill the card.  Past 2^46 pairs, seconds, the gradient is refused
+bool too_many_pairs(const RelP& p) { return p.buckets && p.nb > 256 && (double)p.nd * (double)hmax((long)p.nb * p.H, 1L << 19) > (double)(1L << 46); }
+
 int run(const RelP& p, int dtype, int what, int nw, hipStream_t st) { return dtype == PASSION_BF16 ? rel_run_bf16(p, what, nw, st) : rel_run_f32(p, what, nw, st); }
 
 // layout of the workspaces, in floats
@@ -444,6 +456,7 @@ extern "C" int64_t passion_rel_attn_workspace_floats(int dtype, int backward, in
     static const int dummy = 0;
     const int rc = setup(p, dtype, B, Nq, Nk, H, Hkv, D, gd, gh, gw, q_start, has_table ? &dummy : nullptr, PASSION_F32, has_buckets ? &dummy : nullptr, nb, nullptr, 1.f);
     if (rc) return rc;
+    if (backward == 1 && too_many_pairs(p)) return -1003;
     return backward ? bwd_ws(p, dtype, backward == 1).total : fwd_ws(p, dtype).total;
 }
 
@@ -483,7 +496,7 @@ extern "C" int passion_rel_attn_bwd(const void* q, const int64_t* q_strides, con
     RelP p{};
     int rc = setup(p, dtype, B, Nq, Nk, H, Hkv, D, gd, gh, gw, q_start, table, table_dtype, buckets, nb, mask, scale);
     if (rc) return rc;
-    if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace || !q_strides || !k_strides || !v_strides || (dtable && !table)) return -1003;
+    if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace || !q_strides || !k_strides || !v_strides || (dtable && (!table || too_many_pairs(p)))) return -1003;
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(dout) || misaligned(dq) || misaligned(dk) || misaligned(dv) || misaligned(workspace))
         return -1005;
     if ((rc = strides(p, dtype, q_strides, k_strides, v_strides))) return rc;

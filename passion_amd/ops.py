@@ -1875,6 +1875,8 @@ def rel_attention(q, k, v, table=None, grid=None, buckets=None, key_mask=None, s
                 raise ValueError(f"rel_attention: table of {table.shape[0]} rows without buckets, grid {g} has {offsets} offsets")
         elif tuple(buckets.shape) != (offsets,) or buckets.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"rel_attention: buckets {tuple(buckets.shape)} {buckets.dtype}, grid {g} has {offsets} offsets")
+        elif table.requires_grad and torch.is_grad_enabled() and table.shape[0] > 256 and offsets * max(table.numel(), 2 ** 19) > 2 ** 46:
+            raise ValueError(f"rel_attention: the gradient of {table.shape[0]} buckets over {offsets} offsets: offsets x max(buckets x heads, 2^19) has to stay within 2^46")
         table = table.contiguous()
         nb = table.shape[0]
         if buckets is not None:

@@ -656,3 +656,19 @@ def test_workspace_without_the_table_s_gradient():
         assert size(1, grid, N, 32) >= slab
         offsets = math.prod(2 * g - 1 for g in grid)
         assert 0 < size(2, grid, N, 32) <= 8 * (offsets + N) + 256
+
+
+def test_a_gradient_of_too_many_buckets_over_too_many_offsets_is_refused():
+    """the last sum is a product of the two: at the largest sizes that are taken otherwise it would run for minutes.  Without the gradient, or with few buckets, the call goes on (to the next
+    refusal: tensors that are not on a GPU)"""
+    from passion_amd import _lib, ops
+    lib = _lib.load()
+    size = lambda backward, side, nb, heads=8: lib.passion_rel_attn_workspace_floats(1, backward, 1, 100, 100, heads, heads, 8, side, side, side, 0, 1, 1, nb)
+    assert size(1, 400, 300) == -1003 and size(1, 200, 10 ** 6) == -1003
+    assert size(2, 400, 300) > 0 and size(0, 400, 300) > 0 and size(1, 400, 256) > 0 and size(1, 200, 10 ** 4) > 0 and size(1, 20, 30000) > 0
+    q = torch.zeros(1, 5, 2, 8)
+    buckets = torch.zeros(1, dtype=torch.int32).expand(599 ** 3)
+    for nb, learned in ((300, True), (300, False), (200, True)):
+        table = torch.zeros(nb, 2, requires_grad=learned)
+        with pytest.raises(ValueError if learned and nb == 300 else _lib.PassionHipError):
+            ops.rel_attention(q, q, q, table, (300, 300, 300), buckets)
